@@ -6,9 +6,11 @@ be put on ``sys.path`` to make ``import snnlib`` work for reference-style code):
 * ``libsnnlif_gfx950.so`` -- HIP kernels + C ABI (``csrc/lif_kernels.h`` instantiated by
   ``csrc/lif_f32.hip``, ``lif_f64.hip``, ``lif_bf16.hip``, and ``csrc/lif_bn_kernels.h`` by
   ``lif_bn_f32.hip``, ``lif_bn_f64.hip``; entry points in ``csrc/lif_abi.hip``,
-  declared in ``include/snnlib_lif.h``), compiled by hipcc for gfx950 only;
-* ``snnlib.so``           -- the Python extension module ``snnlib`` (``csrc/snnlib_ext.cpp``), host
-  C++ against PyTorch-ROCm's headers, linked to the library above through ``$ORIGIN``.
+  declared in ``include/snnlib_lif.h``; the token-layer operators of ``include/snnlib_seq.h`` in
+  ``csrc/seq_*.hip``, kernels and entry points together), compiled by hipcc for gfx950 only;
+* ``snnlib.so``           -- the Python extension module ``snnlib`` (``csrc/snnlib_ext.cpp`` and, for the
+  token layers, ``csrc/snnlib_seq_ext.cpp``), host C++ against PyTorch-ROCm's headers, linked to the
+  library above through ``$ORIGIN``.
 
 This replaces the reference's ``CUDAExtension('snnlib', ..., nvcc -arch=sm_70)`` recipe
 (snnlib/setup.py:4-13).  Run ``python -m snn_gpu_training_bptt_amd.build``.
@@ -37,7 +39,8 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 KERNEL_SOURCES = ["lif_abi.hip", "lif_f32.hip", "lif_f64.hip", "lif_bf16.hip", "lif_bn_f32.hip",
-                  "lif_bn_f64.hip"]
+                  "lif_bn_f64.hip", "seq_abi.hip", "seq_embed.hip", "seq_gn.hip"]
+EXTENSION_SOURCES = ["snnlib_ext.cpp", "snnlib_seq_ext.cpp"]
 
 
 def _run(cmd, verbose):
@@ -91,19 +94,28 @@ def build_extension(verbose=False):
     tlib = os.path.join(tdir, "lib")
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     cxx = os.environ.get("CXX", "g++")
-    cmd = [
-        cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         "-DTORCH_EXTENSION_NAME=snnlib", "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         f"-I{INCLUDE}", f"-I{tinc}", f"-I{os.path.join(tinc, 'torch', 'csrc', 'api', 'include')}",
         f"-I{os.path.join(rocm, 'include')}", f"-I{sysconfig.get_paths()['include']}",
-        os.path.join(CSRC, "snnlib_ext.cpp"), "-o", EXT_LIB,
+    ]
+    link = [
         f"-L{tlib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip",
         f"-L{LIB_DIR}", "-l:libsnnlif_gfx950.so",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}",
     ]
-    _run(cmd, verbose)
+    with tempfile.TemporaryDirectory(prefix="snnlib_build_") as tmp:
+        def compile_one(src):
+            obj = os.path.join(tmp, os.path.splitext(src)[0] + ".o")
+            _run([cxx, *flags, "-c", os.path.join(CSRC, src), "-o", obj], verbose)
+            return obj
+
+        with ThreadPoolExecutor(max_workers=len(EXTENSION_SOURCES)) as pool:
+            objects = list(pool.map(compile_one, EXTENSION_SOURCES))
+        _run([cxx, "-shared", *objects, "-o", EXT_LIB, *link], verbose)
     return EXT_LIB
 
 

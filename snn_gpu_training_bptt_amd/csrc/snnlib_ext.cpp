@@ -937,6 +937,8 @@ std::vector<Tensor> bn_fire_conv_bp_dist1(Tensor spatial, Tensor weight_bn, Tens
 
 }  // namespace
 
+void bind_token_layers(pybind11::module_& m);  // snnlib_seq_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "snnlib layer operators for MI355X (gfx950): LIF fire kernels + PyTorch-ROCm dense ops";
     m.attr("__backend__") = "hip-gfx950";
@@ -981,4 +983,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("bn_fire_bp_dist2", &bn_fire_bp_dist2, "bn fire backward, sharded batch: after the all-reduce");
     m.def("bn_fire_fc_bp_dist1", &bn_fire_fc_bp_dist1, "bn fire fc backward, sharded batch: before the all-reduce");
     m.def("bn_fire_conv_bp_dist1", &bn_fire_conv_bp_dist1, "bn fire conv backward, sharded batch: before the all-reduce");
+
+    bind_token_layers(m);
 }

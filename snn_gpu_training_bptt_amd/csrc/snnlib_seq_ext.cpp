@@ -1,0 +1,223 @@
+// The token-layer operators of module `snnlib`: embedding, group norm with an activation, gated delta rule.
+//
+//   embed_fp(tokens, weight, scale) -> out
+//   embed_bp(tokens, grad_out, vocab, scale) -> grad_weight
+//   gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act) -> [mean, rstd, y]
+//   gn_act_bp(x, weight_gn, bias_gn, mean, rstd, groups, act, grad_y) -> [grad_x, grad_weight_gn, grad_bias_gn]
+//
+// As in snnlib_ext.cpp: this file validates tensors, allocates outputs and workspaces and forwards raw device
+// pointers to the C ABI (include/snnlib_seq.h) on the current stream of the tensors' device; it holds no device
+// code and no fallback.
+#include <torch/extension.h>
+
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <string>
+#include <vector>
+
+#include "snnlib_seq.h"
+
+namespace {
+
+using torch::Tensor;
+using DeviceGuard = c10::hip::HIPGuardMasqueradingAsCUDA;
+
+void check_on_gpu(const Tensor& t, const char* op, const char* name) {
+    TORCH_CHECK(t.defined(), "snnlib.", op, ": ", name, " is undefined");
+    TORCH_CHECK(t.is_cuda(), "snnlib.", op, ": ", name,
+                " must live on a ROCm GPU (this build has no CPU path), got device ", t.device());
+}
+
+int storage_dtype(const Tensor& t, const char* op, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return SNNLIF_DTYPE_F32;
+        case at::kDouble: return SNNLIF_DTYPE_F64;
+        case at::kBFloat16: return SNNLIF_DTYPE_BF16;
+        default:
+            TORCH_CHECK(false, "snnlib.", op, ": unsupported dtype ", t.scalar_type(), " of ", name,
+                        " (supported: float32, float64, bfloat16)");
+    }
+    return -1;
+}
+
+void check_like(const Tensor& t, const Tensor& like, const char* op, const char* name, const char* like_name) {
+    check_on_gpu(t, op, name);
+    TORCH_CHECK(t.device() == like.device(), "snnlib.", op, ": ", name, " (", t.device(), ") must be on the device of ",
+                like_name, " (", like.device(), ")");
+    TORCH_CHECK(t.scalar_type() == like.scalar_type(), "snnlib.", op, ": ", name, " (", t.scalar_type(),
+                ") must have the dtype of ", like_name, " (", like.scalar_type(), ")");
+}
+
+void check_rc(int rc, const char* op) {
+    TORCH_CHECK(rc == SNNLIF_OK, "snnlib.", op, ": ", snnlif_strerror(rc), " (code ", rc, ")");
+}
+
+void* current_stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+
+Tensor dense(const Tensor& t) { return t.contiguous(); }
+
+// A workspace from the caching allocator: it goes back on return and stays valid for the work already queued,
+// because later users are ordered on the same stream.
+Tensor workspace_of(size_t bytes, const Tensor& like) {
+    return torch::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+
+// ---- embedding ----------------------------------------------------------------------------------
+
+int token_dtype(const Tensor& tokens, const char* op) {
+    check_on_gpu(tokens, op, "tokens");
+    TORCH_CHECK(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "snnlib.", op,
+                ": tokens must be int64 or int32, got ", tokens.scalar_type());
+    return tokens.scalar_type() == at::kLong ? SNNSEQ_TOKEN_I64 : SNNSEQ_TOKEN_I32;
+}
+
+Tensor embed_fp(Tensor tokens, Tensor weight, double scale) {
+    const char* op = "embed_fp";
+    const int tdtype = token_dtype(tokens, op);
+    check_on_gpu(weight, op, "weight");
+    TORCH_CHECK(weight.device() == tokens.device(), "snnlib.", op, ": weight (", weight.device(),
+                ") must be on the device of tokens (", tokens.device(), ")");
+    const int dtype = storage_dtype(weight, op, "weight");
+    TORCH_CHECK(weight.dim() == 2 && weight.size(0) > 0, "snnlib.", op,
+                ": weight must be [vocab, cout] with at least one row, got ", weight.sizes());
+    const DeviceGuard guard(weight.device());
+    Tensor ids = dense(tokens);
+    Tensor table = weight.size(1) > 1 && weight.stride(1) != 1 ? dense(weight) : weight;  // rows may lie apart
+    std::vector<int64_t> sizes = tokens.sizes().vec();
+    sizes.push_back(weight.size(1));
+    Tensor out = torch::empty(sizes, weight.options());
+    check_rc(snnseq_embed_fp(ids.data_ptr(), table.data_ptr(), out.data_ptr(), dtype, tdtype, ids.numel(),
+                             table.size(0), table.size(1), table.stride(0), scale, current_stream()),
+             op);
+    return out;
+}
+
+Tensor embed_bp(Tensor tokens, Tensor grad_out, int64_t vocab, double scale) {
+    const char* op = "embed_bp";
+    const int tdtype = token_dtype(tokens, op);
+    check_on_gpu(grad_out, op, "grad_out");
+    TORCH_CHECK(grad_out.device() == tokens.device(), "snnlib.", op, ": grad_out (", grad_out.device(),
+                ") must be on the device of tokens (", tokens.device(), ")");
+    const int dtype = storage_dtype(grad_out, op, "grad_out");
+    TORCH_CHECK(vocab > 0, "snnlib.", op, ": vocab must be positive, got ", vocab);
+    TORCH_CHECK(grad_out.dim() == tokens.dim() + 1 &&
+                    grad_out.sizes().slice(0, tokens.dim()) == tokens.sizes(),
+                "snnlib.", op, ": grad_out must be [", tokens.sizes(), ", cout], got ", grad_out.sizes());
+    const DeviceGuard guard(grad_out.device());
+    Tensor ids = dense(tokens), g = dense(grad_out);
+    const int64_t C = g.size(-1);
+    Tensor grad_weight = torch::empty({vocab, C}, g.options());
+    const size_t ws_bytes = snnseq_embed_bp_workspace_bytes(dtype, ids.numel(), vocab, C);
+    Tensor workspace = workspace_of(ws_bytes, g);
+    check_rc(snnseq_embed_bp(ids.data_ptr(), g.data_ptr(), grad_weight.data_ptr(), dtype, tdtype, ids.numel(), vocab, C,
+                             scale, workspace.data_ptr(), ws_bytes, current_stream()),
+             op);
+    return grad_weight;
+}
+
+// ---- group norm with an activation --------------------------------------------------------------
+
+int act_code(const std::string& act, const char* op) {
+    if (act == "none") return SNNSEQ_ACT_NONE;
+    if (act == "relu") return SNNSEQ_ACT_RELU;
+    if (act == "silu") return SNNSEQ_ACT_SILU;
+    if (act == "gelu") return SNNSEQ_ACT_GELU;
+    TORCH_CHECK(false, "snnlib.", op, ": unknown activation '", act, "' (none, relu, silu, gelu)");
+    return -1;
+}
+
+struct GnOperands {
+    int64_t S, P, C;
+    int dtype;
+    Tensor x, weight, bias;
+};
+
+GnOperands gn_operands(const Tensor& x, const Tensor& weight_gn, const Tensor& bias_gn, int64_t groups,
+                       const char* op) {
+    check_on_gpu(x, op, "x");
+    GnOperands o;
+    o.dtype = storage_dtype(x, op, "x");
+    TORCH_CHECK(x.dim() >= 3, "snnlib.", op, ": x must be shaped [T, B, ..., C], got ", x.sizes());
+    o.C = x.size(-1);
+    o.S = x.size(0) * x.size(1);
+    o.P = 1;
+    for (int64_t d = 2; d + 1 < x.dim(); ++d) o.P *= x.size(d);
+    TORCH_CHECK(groups > 0 && o.C % groups == 0, "snnlib.", op, ": groups (", groups,
+                ") must divide the channels (", o.C, ")");
+    TORCH_CHECK(o.S == 0 || (o.P > 0 && o.C > 0), "snnlib.", op, ": no values per group in a tensor shaped ",
+                x.sizes());
+    for (const auto& p : {std::make_pair(&weight_gn, "weight_gn"), std::make_pair(&bias_gn, "bias_gn")}) {
+        check_like(*p.first, x, op, p.second, "x");
+        TORCH_CHECK(p.first->dim() == 1 && p.first->size(0) == o.C, "snnlib.", op, ": ", p.second,
+                    " must have one value per channel (", o.C, "), got ", p.first->sizes());
+    }
+    o.x = dense(x);
+    o.weight = dense(weight_gn);
+    o.bias = dense(bias_gn);
+    return o;
+}
+
+std::vector<Tensor> gn_act_fp(Tensor x, Tensor weight_gn, Tensor bias_gn, int64_t groups, double eps_gn,
+                              const std::string& act) {
+    const char* op = "gn_act_fp";
+    const int code = act_code(act, op);
+    TORCH_CHECK(eps_gn >= 0, "snnlib.", op, ": eps_gn must not be negative, got ", eps_gn);
+    check_on_gpu(x, op, "x");
+    const DeviceGuard guard(x.device());
+    const GnOperands o = gn_operands(x, weight_gn, bias_gn, groups, op);
+    Tensor y = torch::empty(o.x.sizes(), o.x.options());
+    const auto stat = o.x.options().dtype(o.dtype == SNNLIF_DTYPE_F64 ? at::kDouble : at::kFloat);
+    Tensor mean = torch::empty({o.x.size(0), o.x.size(1), groups}, stat);
+    Tensor rstd = torch::empty({o.x.size(0), o.x.size(1), groups}, stat);
+    const size_t ws_bytes = snnseq_gn_act_workspace_bytes(o.dtype, o.S, o.P, o.C, groups, 0);
+    Tensor workspace;
+    if (ws_bytes > 0) workspace = workspace_of(ws_bytes, o.x);
+    check_rc(snnseq_gn_act_fp(o.x.data_ptr(), o.weight.data_ptr(), o.bias.data_ptr(), y.data_ptr(), mean.data_ptr(),
+                              rstd.data_ptr(), o.dtype, o.S, o.P, o.C, groups, eps_gn, code,
+                              ws_bytes ? workspace.data_ptr() : nullptr, ws_bytes, current_stream()),
+             op);
+    return {mean, rstd, y};
+}
+
+std::vector<Tensor> gn_act_bp(Tensor x, Tensor weight_gn, Tensor bias_gn, Tensor mean, Tensor rstd, int64_t groups,
+                              const std::string& act, Tensor grad_y) {
+    const char* op = "gn_act_bp";
+    const int code = act_code(act, op);
+    check_on_gpu(x, op, "x");
+    const DeviceGuard guard(x.device());
+    const GnOperands o = gn_operands(x, weight_gn, bias_gn, groups, op);
+    check_like(grad_y, x, op, "grad_y", "x");
+    TORCH_CHECK(grad_y.sizes() == x.sizes(), "snnlib.", op, ": grad_y ", grad_y.sizes(), " and x ", x.sizes(),
+                " must have the same shape");
+    const auto stat = o.dtype == SNNLIF_DTYPE_F64 ? at::kDouble : at::kFloat;
+    for (const auto& p : {std::make_pair(&mean, "mean"), std::make_pair(&rstd, "rstd")}) {
+        check_on_gpu(*p.first, op, p.second);
+        TORCH_CHECK(p.first->device() == x.device() && p.first->scalar_type() == stat &&
+                        p.first->numel() == o.S * groups,
+                    "snnlib.", op, ": ", p.second, " must be what gn_act_fp returned for this x");
+    }
+    Tensor m = dense(mean), r = dense(rstd), g = dense(grad_y);
+    Tensor grad_x = torch::empty(o.x.sizes(), o.x.options());
+    // an empty batch contributes nothing to the parameter gradients; otherwise every channel is written
+    Tensor grad_weight = o.S == 0 ? torch::zeros({o.C}, o.x.options()) : torch::empty({o.C}, o.x.options());
+    Tensor grad_bias = torch::empty_like(grad_weight);
+    if (o.S == 0) grad_bias.zero_();
+    const size_t ws_bytes = snnseq_gn_act_workspace_bytes(o.dtype, o.S, o.P, o.C, groups, 1);
+    Tensor workspace = workspace_of(ws_bytes, o.x);
+    check_rc(snnseq_gn_act_bp(o.x.data_ptr(), o.weight.data_ptr(), o.bias.data_ptr(), m.data_ptr(), r.data_ptr(),
+                              g.data_ptr(), grad_x.data_ptr(), grad_weight.data_ptr(), grad_bias.data_ptr(), o.dtype,
+                              o.S, o.P, o.C, groups, code, workspace.data_ptr(), ws_bytes, current_stream()),
+             op);
+    return {grad_x, grad_weight, grad_bias};
+}
+
+}  // namespace
+
+void bind_token_layers(pybind11::module_& m) {
+    m.attr("__seq_abi_version__") = snnseq_abi_version();
+    m.def("embed_fp", &embed_fp, "embedding lookup with a scale");
+    m.def("embed_bp", &embed_bp, "gradient of the embedding table, by sorted tokens");
+    m.def("gn_act_fp", &gn_act_fp, "group norm with an activation, channels last: [mean, rstd, y]");
+    m.def("gn_act_bp", &gn_act_bp, "its backward: [grad_x, grad_weight_gn, grad_bias_gn]");
+}

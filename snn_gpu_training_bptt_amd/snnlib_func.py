@@ -15,6 +15,7 @@ recomputes what it needs.  Hyper-parameters are module globals read at call time
 ``snnlib_func.thresh = 0.5`` takes effect on the next call.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._loader import load_snnlib
 
@@ -286,6 +287,60 @@ class BnFireConvDistFunc(BnFireConvFunc):
         g_spatial = _sharded_bn_fire_input_grad(ctx, bn_saved, g_spike, local_xhat, local_xhatx)
         return _conv_grads(ctx, g_spatial, g_weight_conv, g_bias_conv,
                            leading=(g_spatial, g_weight_bn, g_bias_bn, None, None, None)) + (None,)
+
+
+class EmbedFunc(torch.autograd.Function):
+    """out = scale * weight[tokens]; a token outside the table (-1, say) gives a row of zeros."""
+
+    @staticmethod
+    def forward(ctx, tokens, weight, scale):
+        ctx.save_for_backward(tokens)
+        ctx.vocab, ctx.scale = weight.shape[0], scale
+        return snnlib.embed_fp(tokens, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        (tokens,) = ctx.saved_tensors
+        return None, snnlib.embed_bp(tokens, grad_out, ctx.vocab, ctx.scale), None
+
+
+class GnActFunc(torch.autograd.Function):
+    """y = act(group_norm(x)) over the last axis of ``[T, B, ..., C]``; saves the statistics with its inputs."""
+
+    @staticmethod
+    def forward(ctx, x, weight_gn, bias_gn, groups, eps_gn, act):
+        mean, rstd, y = snnlib.gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act)
+        ctx.save_for_backward(x, weight_gn, bias_gn, mean, rstd)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        # saved: x, weight_gn, bias_gn, mean, rstd
+        return _pad(snnlib.gn_act_bp(*ctx.saved_tensors, ctx.groups, ctx.act, grad_y), 6)
+
+
+def _records(*tensors):
+    """Whether autograd would record an operator on these tensors; without that the token layers call the
+    native op directly (a call on a few tokens is over in less time than a recorded node takes)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def embed_func(tokens, weight, scale=1.0):
+    """``scale * weight[tokens]`` for integer ``tokens`` of any shape, ``[*tokens.shape, cout]``."""
+    if _records(weight):
+        return EmbedFunc.apply(tokens, weight, scale)
+    return snnlib.embed_fp(tokens, weight, scale)
+
+
+def gn_act_func(x, weight_gn, bias_gn, groups, eps_gn=1e-5, act="none"):
+    """Group norm over the last axis of ``[T, B, ..., C]`` (per time step, batch entry and group of ``C / groups``
+    channels), then ``act``: "none", "relu", "silu" or "gelu"."""
+    if _records(x, weight_gn, bias_gn):
+        return GnActFunc.apply(x, weight_gn, bias_gn, groups, eps_gn, act)
+    return snnlib.gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act)[2]
 
 
 fire_func = FireFunc.apply
