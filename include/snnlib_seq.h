@@ -87,6 +87,57 @@ int snnseq_gn_act_bp(const void* x, const void* weight, const void* bias, const 
 /* Bytes of device workspace of the two calls above (backward = 0 / 1); 0 also where none is needed. */
 size_t snnseq_gn_act_workspace_bytes(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, int backward);
 
+/* Most values of a key and of a value, and most heads times batch entries, of a gated delta call. */
+#define SNNSEQ_MAX_KEY   128
+#define SNNSEQ_MAX_VALUE 65536
+#define SNNSEQ_MAX_HEADS 65535
+
+/*
+ * Operands of the gated delta rule, F32 or BF16 (F64: SNNLIF_ERR_UNSUPPORTED).  With S [Dk, Dv] per batch entry and
+ * value head, zero or `state` before the first step,
+ *   S_t = exp(g_t) S_{t-1} + beta_t k_t (v_t - exp(g_t) S_{t-1}^T k_t)^T,   o_t = scale * S_t^T q_t
+ * q, k [T, B, Hk, Dk] and v [T, B, Hv, Dv] with the given strides (in elements: step, batch entry, head; the Dk or Dv
+ * values of a row are dense); g, beta dense [T, B, Hv] fp32; states dense [B, Hv, Dk, Dv] fp32.  Hv is a multiple
+ * of Hk; value head h uses key head h / (Hv / Hk).  g <= 0 is the decay's logarithm (-inf forgets everything);
+ * keys are expected at length one or below, as the recurrence multiplies by up to |k|^2 - 1 otherwise.
+ * `lengths` ([B] int32, may be NULL): the time steps of batch entry b at or behind lengths[b] do not exist.  They leave the
+ * state alone, their outputs and gradients are zero, and what the operands hold there is not looked at.
+ */
+typedef struct snnseq_delta {
+    int64_t T, B, Hk, Hv, Dk, Dv;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    double scale;
+    const void *q, *k, *v;
+    const float *g, *beta;
+    const float* state;       /* may be NULL */
+    const int32_t* lengths;   /* may be NULL */
+    int dtype;
+} snnseq_delta;
+
+/* Bytes the forward writes for the backward: per chunk of 64 steps and value head the fp32 state before it, the rows
+ * added to it and a 64 x 64 matrix.  A caller that wants no backward passes the same memory as scratch.  0 for invalid arguments. */
+size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call);
+
+/* o dense [T, B, Hv, Dv]; state_out [B, Hv, Dk, Dv] (may be NULL): the state after the last step. */
+int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved, size_t saved_bytes,
+                          void* stream);
+
+size_t snnseq_gated_delta_bp_workspace_bytes(const snnseq_delta* call);
+
+/*
+ * Backward, from the forward's operands and what it saved.  grad_o [T, B, Hv, Dv] with strides; grad_state_out (may be
+ * NULL: zero) the gradient of the last state.  Gradients are dense and shaped as their operands (grad_q, grad_k over
+ * Hk heads, summed over the value heads that share them); grad_state (may be NULL) that of the initial state.
+ */
+int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved, size_t saved_bytes, const void* grad_o,
+                          const int64_t* grad_o_strides, const float* grad_state_out, void* grad_q, void* grad_k,
+                          void* grad_v, float* grad_g, float* grad_beta, float* grad_state, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* One time step (T == 1, `state` given, no lengths): o [B, Hv, Dv], and the state after it in state_out, which may be
+ * `state` itself (but must not overlap it otherwise).  One launch, no workspace. */
+int snnseq_gated_delta_step(const snnseq_delta* call, void* o, float* state_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

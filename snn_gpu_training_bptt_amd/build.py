@@ -39,7 +39,8 @@ HIPCC_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 KERNEL_SOURCES = ["lif_abi.hip", "lif_f32.hip", "lif_f64.hip", "lif_bf16.hip", "lif_bn_f32.hip",
-                  "lif_bn_f64.hip", "seq_abi.hip", "seq_embed.hip", "seq_gn.hip"]
+                  "lif_bn_f64.hip", "seq_abi.hip", "seq_embed.hip", "seq_gn.hip",
+                  "seq_delta.hip", "seq_delta_f32.hip", "seq_delta_bf16.hip"]
 EXTENSION_SOURCES = ["snnlib_ext.cpp", "snnlib_seq_ext.cpp"]
 
 

@@ -1,0 +1,312 @@
+// Entry points of the gated delta rule, and its form for single tokens.
+#include "seq_delta.h"
+
+namespace snnseq {
+namespace {
+
+// ---- one token ----------------------------------------------------------------------------------
+//
+// o = scale S'^T q with S' = a S + k e^T, e = beta (v - a S^T k):  S^T k and S^T q are taken in one sweep over the
+// state, and S'^T q = a S^T q + (k . q) e, so the state is read once, held in registers, and written once: 8 bytes
+// per value, the bound.  A workgroup owns 64 columns of a head's state: 16 lanes of four columns share a row, 16
+// rows at a time, and the sums over the rows go through shuffles and LDS.
+
+constexpr int kStepCols = 64, kStepThreads = 256, kStepRows = kStepThreads / (kStepCols / 4);
+
+struct StepArgs {
+    int B, Hk, Hv, Dk, Dv;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_b, q_h, k_b, k_h, v_b, v_h;
+    const float *g, *beta, *state;
+    void* o;
+    float* state_out;
+};
+
+template <typename E, int ROWS, bool WIDE>   // ROWS: rows of the state per thread;  WIDE: four columns in one access
+__global__ void __launch_bounds__(kStepThreads) delta_step_kernel(StepArgs a) {
+    __shared__ float qs[ROWS * kStepRows], ks[ROWS * kStepRows];
+    __shared__ float part[2][kStepThreads / 64][kStepCols];
+    const int head = blockIdx.y, b = head / a.Hv, hv = head - b * a.Hv, hk = hv / (a.Hv / a.Hk);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.x * kStepCols + (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
+    const int64_t base = static_cast<int64_t>(head) * a.Dk * a.Dv + c;
+    f32x4 s[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i * kStepRows;
+        s[i] = zero4();
+        if (r < a.Dk) {
+            const float* p = a.state + base + static_cast<int64_t>(r) * a.Dv;
+            if (WIDE) {
+                if (c < a.Dv) s[i] = *reinterpret_cast<const f32x4*>(p);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < a.Dv) s[i][j] = p[j];
+            }
+        }
+    }
+    const E* q = static_cast<const E*>(a.q) + b * a.q_b + hk * a.q_h;
+    const E* k = static_cast<const E*>(a.k) + b * a.k_b + hk * a.k_h;
+    const E* v = static_cast<const E*>(a.v) + b * a.v_b + hv * a.v_h;
+    if (static_cast<int>(threadIdx.x) < ROWS * kStepRows) {
+        const int r = threadIdx.x;
+        qs[r] = r < a.Dk ? widen(q[r]) : 0.f;
+        ks[r] = r < a.Dk ? widen(k[r]) : 0.f;
+    }
+    const float g = a.g[head], beta = a.beta[head];
+    float value[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) value[j] = c + j < a.Dv ? widen(v[c + j]) : 0.f;
+    __syncthreads();
+    f32x4 sk = zero4(), sq = zero4();
+    float kq = 0.f;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const float kr = ks[r0 + i * kStepRows], qr = qs[r0 + i * kStepRows];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sk[j] += kr * s[i][j];
+            sq[j] += qr * s[i][j];
+        }
+        kq += kr * qr;
+    }
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) {
+        kq += __shfl_xor(kq, d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sk[j] += __shfl_xor(sk[j], d);
+            sq[j] += __shfl_xor(sq[j], d);
+        }
+    }
+    __shared__ float kq_part[kStepThreads / 64];
+    if (lane < 16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            part[0][wave][lane * 4 + j] = sk[j];
+            part[1][wave][lane * 4 + j] = sq[j];
+        }
+        if (lane == 0) kq_part[wave] = kq;
+    }
+    __syncthreads();
+    const float decay = expf(g);
+    f32x4 add;
+    float out[4];
+    const float kq_all = kq_part[0] + kq_part[1] + kq_part[2] + kq_part[3];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int at = (threadIdx.x & 15) * 4 + j;
+        const float k_sum = part[0][0][at] + part[0][1][at] + part[0][2][at] + part[0][3][at];
+        const float q_sum = part[1][0][at] + part[1][1][at] + part[1][2][at] + part[1][3][at];
+        add[j] = beta * (value[j] - decay * k_sum);
+        out[j] = a.scale * (decay * q_sum + kq_all * add[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i * kStepRows;
+        if (r >= a.Dk) continue;
+        const float kr = ks[r];
+        f32x4 n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n[j] = decay * s[i][j] + kr * add[j];
+        float* p = a.state_out + base + static_cast<int64_t>(r) * a.Dv;
+        if (WIDE) {
+            if (c < a.Dv) *reinterpret_cast<f32x4*>(p) = n;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < a.Dv) p[j] = n[j];
+        }
+    }
+    if (threadIdx.x < 16) {
+        E* o = static_cast<E*>(a.o) + static_cast<int64_t>(head) * a.Dv + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < a.Dv) o[j] = narrow<E>(out[j]);
+    }
+}
+
+template <typename E>
+hipError_t step_as(const StepArgs& a, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.Dv, kStepCols)), static_cast<unsigned>(a.B * a.Hv));
+    const bool wide = a.Dv % 4 == 0 && aligned_to(a.state, 16) && aligned_to(a.state_out, 16);
+    // the rows a thread holds cost registers and, where the head has fewer, loads that do nothing
+    if (a.Dk <= 64)
+        return wide ? launch(delta_step_kernel<E, 4, true>, grid, dim3(kStepThreads), st, a)
+                    : launch(delta_step_kernel<E, 4, false>, grid, dim3(kStepThreads), st, a);
+    return wide ? launch(delta_step_kernel<E, 8, true>, grid, dim3(kStepThreads), st, a)
+                : launch(delta_step_kernel<E, 8, false>, grid, dim3(kStepThreads), st, a);
+}
+
+// ---- arguments ----------------------------------------------------------------------------------
+
+int delta_error(const snnseq_delta* c) {
+    if (c == nullptr) return SNNLIF_ERR_ARG;
+    if (c->dtype == SNNLIF_DTYPE_F64) return SNNLIF_ERR_UNSUPPORTED;
+    if (element_size(c->dtype) == 0) return SNNLIF_ERR_DTYPE;
+    if (c->T < 0 || c->B < 0 || c->Hk < 1 || c->Hv < 1 || c->Hv % c->Hk != 0) return SNNLIF_ERR_ARG;
+    if (c->T > SNNSEQ_MAX_TOKENS || c->Dk < 1 || c->Dk > SNNSEQ_MAX_KEY || c->Dv < 1 || c->Dv > SNNSEQ_MAX_VALUE)
+        return SNNLIF_ERR_ARG;
+    if (c->Hv > SNNSEQ_MAX_HEADS || c->B > SNNSEQ_MAX_HEADS / c->Hv) return SNNLIF_ERR_ARG;  // B * Hv is a grid size
+    return SNNLIF_OK;
+}
+
+bool empty(const snnseq_delta* c) { return c->B == 0; }
+
+int missing(const snnseq_delta* c) {
+    if (c->T > 0 && (c->q == nullptr || c->k == nullptr || c->v == nullptr || c->g == nullptr || c->beta == nullptr))
+        return SNNLIF_ERR_ARG;
+    const size_t es = element_size(c->dtype);
+    if (!aligned_to(c->q, es) || !aligned_to(c->k, es) || !aligned_to(c->v, es) || !aligned_to(c->g, 4) ||
+        !aligned_to(c->beta, 4) || !aligned_to(c->state, 4) || !aligned_to(c->lengths, 4))
+        return SNNLIF_ERR_ALIGN;
+    return SNNLIF_OK;
+}
+
+DeltaTensor tensor_of(const void* p, const int64_t* strides, int64_t D, size_t es) {
+    DeltaTensor x{p, strides[0], strides[1], strides[2], 0};
+    x.wide = D % 8 == 0 && common_bytes(address(p), static_cast<uint64_t>(strides[0]) * es,
+                                        static_cast<uint64_t>(strides[1]) * es, static_cast<uint64_t>(strides[2]) * es) == 16;
+    return x;
+}
+
+struct Sizes {
+    int64_t pieces, heads, chunks, cols, dkp;
+    size_t inverse, added, states;               // bytes of the forward's matrices
+    size_t inner, state_grads, partial;          // of the backward's
+};
+
+Sizes sizes_of(const snnseq_delta* c) {
+    Sizes s;
+    s.chunks = ceil_div(c->T, kChunk);
+    s.heads = c->B * c->Hv;
+    s.pieces = s.chunks * s.heads;
+    s.cols = ceil_div(c->Dv, kStateCols) * kStateCols;
+    s.dkp = c->Dk <= 64 ? 64 : 128;
+    const size_t n = static_cast<size_t>(s.pieces) * sizeof(float);
+    s.inverse = n * kChunk * kChunk;
+    s.added = s.inner = n * kChunk * static_cast<size_t>(s.cols);
+    s.states = s.state_grads = n * static_cast<size_t>(s.dkp * s.cols);
+    s.partial = c->Hv == c->Hk ? 0 : round_up(static_cast<size_t>(c->T * s.heads * c->Dk) * sizeof(float), 16);
+    return s;
+}
+
+DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved) {
+    const size_t es = element_size(c->dtype);
+    DeltaArgs a{};
+    a.T = static_cast<int>(c->T); a.B = static_cast<int>(c->B);
+    a.Hk = static_cast<int>(c->Hk); a.Hv = static_cast<int>(c->Hv);
+    a.Dk = static_cast<int>(c->Dk); a.Dv = static_cast<int>(c->Dv);
+    a.chunks = static_cast<int>(s.chunks); a.cols = static_cast<int>(s.cols);
+    a.scale = static_cast<float>(c->scale);
+    a.lengths = c->lengths;
+    a.q = tensor_of(c->q, c->q_strides, c->Dk, es);
+    a.k = tensor_of(c->k, c->k_strides, c->Dk, es);
+    a.v = tensor_of(c->v, c->v_strides, c->Dv, es);
+    a.g = c->g; a.beta = c->beta; a.state = c->state;
+    char* p = static_cast<char*>(saved);
+    a.inverse = reinterpret_cast<float*>(p);
+    a.added = reinterpret_cast<float*>(p + s.inverse);
+    a.states = reinterpret_cast<float*>(p + s.inverse + s.added);
+    return a;
+}
+
+}  // namespace
+}  // namespace snnseq
+
+using namespace snnseq;
+
+extern "C" size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call) {
+    if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
+    const Sizes s = sizes_of(call);
+    return s.inverse + s.added + s.states;
+}
+
+extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved,
+                                     size_t saved_bytes, void* stream) {
+    const int bad = delta_error(call);
+    if (bad != SNNLIF_OK) return bad;
+    if (empty(call)) return SNNLIF_OK;
+    const int lost = missing(call);
+    if (lost != SNNLIF_OK) return lost;
+    if (call->T > 0 && o == nullptr) return SNNLIF_ERR_ARG;
+    if (!aligned_to(o, element_size(call->dtype)) || !aligned_to(state_out, 4) || !aligned_to(saved, 16))
+        return SNNLIF_ERR_ALIGN;
+    const Sizes s = sizes_of(call);
+    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.inverse + s.added + s.states)) return SNNLIF_ERR_WORKSPACE;
+    DeltaArgs a = args_of(call, s, saved);
+    a.o = o;
+    a.state_out = state_out;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return static_cast<int>(call->dtype == SNNLIF_DTYPE_F32 ? delta_forward_f32(a, st) : delta_forward_bf16(a, st));
+}
+
+extern "C" size_t snnseq_gated_delta_bp_workspace_bytes(const snnseq_delta* call) {
+    if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
+    const Sizes s = sizes_of(call);
+    return s.inner + s.state_grads + 2 * s.partial;
+}
+
+extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved, size_t saved_bytes,
+                                     const void* grad_o, const int64_t* grad_o_strides, const float* grad_state_out,
+                                     void* grad_q, void* grad_k, void* grad_v, float* grad_g, float* grad_beta,
+                                     float* grad_state, void* workspace, size_t workspace_bytes, void* stream) {
+    const int bad = delta_error(call);
+    if (bad != SNNLIF_OK) return bad;
+    if (empty(call)) return SNNLIF_OK;
+    const int lost = missing(call);
+    if (lost != SNNLIF_OK) return lost;
+    if (grad_o_strides == nullptr) return SNNLIF_ERR_ARG;
+    if (call->T > 0 && (grad_o == nullptr || grad_q == nullptr || grad_k == nullptr || grad_v == nullptr ||
+                        grad_g == nullptr || grad_beta == nullptr))
+        return SNNLIF_ERR_ARG;
+    const size_t es = element_size(call->dtype);
+    if (!aligned_to(grad_o, es) || !aligned_to(grad_q, es) || !aligned_to(grad_k, es) || !aligned_to(grad_v, es) ||
+        !aligned_to(grad_g, 4) || !aligned_to(grad_beta, 4) || !aligned_to(grad_state, 4) ||
+        !aligned_to(grad_state_out, 4) || !aligned_to(saved, 16) || !aligned_to(workspace, 16))
+        return SNNLIF_ERR_ALIGN;
+    const Sizes s = sizes_of(call);
+    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.inverse + s.added + s.states || workspace == nullptr ||
+                         workspace_bytes < s.inner + s.state_grads + 2 * s.partial))
+        return SNNLIF_ERR_WORKSPACE;
+    DeltaArgs a = args_of(call, s, const_cast<void*>(saved));
+    char* p = static_cast<char*>(workspace);
+    a.grad_o = tensor_of(grad_o, grad_o_strides, call->Dv, es);
+    a.grad_state = grad_state_out;
+    a.inner = reinterpret_cast<float*>(p);
+    a.state_grads = reinterpret_cast<float*>(p + s.inner);
+    a.grad_q = s.partial ? p + s.inner + s.state_grads : grad_q;
+    a.grad_k = s.partial ? p + s.inner + s.state_grads + s.partial : grad_k;
+    a.grad_v = grad_v;
+    a.grad_g = grad_g;
+    a.grad_beta = grad_beta;
+    a.grad_initial = grad_state;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return static_cast<int>(call->dtype == SNNLIF_DTYPE_F32 ? delta_backward_f32(a, grad_q, grad_k, st)
+                                                            : delta_backward_bf16(a, grad_q, grad_k, st));
+}
+
+extern "C" int snnseq_gated_delta_step(const snnseq_delta* call, void* o, float* state_out, void* stream) {
+    const int bad = delta_error(call);
+    if (bad != SNNLIF_OK) return bad;
+    if (call->T != 1 || call->lengths != nullptr) return SNNLIF_ERR_ARG;
+    if (empty(call)) return SNNLIF_OK;
+    const int lost = missing(call);
+    if (lost != SNNLIF_OK) return lost;
+    if (call->state == nullptr || state_out == nullptr || o == nullptr) return SNNLIF_ERR_ARG;
+    if (!aligned_to(o, element_size(call->dtype)) || !aligned_to(state_out, 4)) return SNNLIF_ERR_ALIGN;
+    StepArgs a{};
+    a.B = static_cast<int>(call->B); a.Hk = static_cast<int>(call->Hk); a.Hv = static_cast<int>(call->Hv);
+    a.Dk = static_cast<int>(call->Dk); a.Dv = static_cast<int>(call->Dv);
+    a.scale = static_cast<float>(call->scale);
+    a.q = call->q; a.q_b = call->q_strides[1]; a.q_h = call->q_strides[2];
+    a.k = call->k; a.k_b = call->k_strides[1]; a.k_h = call->k_strides[2];
+    a.v = call->v; a.v_b = call->v_strides[1]; a.v_h = call->v_strides[2];
+    a.g = call->g; a.beta = call->beta; a.state = call->state;
+    a.o = o;
+    a.state_out = state_out;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return static_cast<int>(call->dtype == SNNLIF_DTYPE_F32 ? step_as<float>(a, st) : step_as<bf16_t>(a, st));
+}

@@ -4,6 +4,10 @@
 //   embed_bp(tokens, grad_out, vocab, scale) -> grad_weight
 //   gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act) -> [mean, rstd, y]
 //   gn_act_bp(x, weight_gn, bias_gn, mean, rstd, groups, act, grad_y) -> [grad_x, grad_weight_gn, grad_bias_gn]
+//   gated_delta_fp(q, k, v, g, beta, state, lengths, scale) -> [o, state_out, saved]
+//   gated_delta_bp(q, k, v, g, beta, state, lengths, scale, saved, grad_o, grad_state_out)
+//                  -> [grad_q, grad_k, grad_v, grad_g, grad_beta, grad_state]
+//   gated_delta_step(q, k, v, g, beta, state, scale, state_out) -> o
 //
 // As in snnlib_ext.cpp: this file validates tensors, allocates outputs and workspaces and forwards raw device
 // pointers to the C ABI (include/snnlib_seq.h) on the current stream of the tensors' device; it holds no device
@@ -212,6 +216,177 @@ std::vector<Tensor> gn_act_bp(Tensor x, Tensor weight_gn, Tensor bias_gn, Tensor
     return {grad_x, grad_weight, grad_bias};
 }
 
+// ---- gated delta rule ---------------------------------------------------------------------------
+
+using MaybeTensor = c10::optional<Tensor>;
+
+struct DeltaOperands {
+    snnseq_delta call;
+    Tensor q, k, v, g, beta, state, lengths;   // what the call points into
+    bool has_state = false;
+};
+
+// Rows of values must be dense; any other layout is taken as it lies.
+Tensor dense_rows(const Tensor& t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
+
+void strides_of(const Tensor& t, int64_t (&strides)[3]) {
+    const int64_t d = t.dim();
+    strides[0] = d == 4 ? t.stride(0) : 0;
+    strides[1] = t.stride(d - 3);
+    strides[2] = t.stride(d - 2);
+}
+
+// rank 4: [T, B, H, D] operands; rank 3: one step, [B, H, D].
+DeltaOperands delta_operands(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                             const MaybeTensor& state, const MaybeTensor& lengths, double scale, int64_t rank,
+                             const char* op) {
+    const char* shape = rank == 4 ? "[T, B, heads, D]" : "[B, heads, D]";
+    check_on_gpu(q, op, "q");
+    TORCH_CHECK(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16, "snnlib.", op,
+                ": only float32 and bfloat16 are supported, got ", q.scalar_type());
+    check_like(k, q, op, "k", "q");
+    check_like(v, q, op, "v", "q");
+    TORCH_CHECK(q.dim() == rank && v.dim() == rank, "snnlib.", op, ": q, k and v must be shaped ", shape, ", got ",
+                q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+    TORCH_CHECK(q.sizes() == k.sizes(), "snnlib.", op, ": q ", q.sizes(), " and k ", k.sizes(), " must have the same shape");
+    TORCH_CHECK(v.sizes().slice(0, rank - 2) == q.sizes().slice(0, rank - 2), "snnlib.", op, ": v ", v.sizes(),
+                " must share the time steps and batch entries of q ", q.sizes());
+    const int64_t Hk = q.size(-2), Hv = v.size(-2), Dk = q.size(-1), Dv = v.size(-1), B = q.size(rank - 3);
+    TORCH_CHECK(Hk > 0 && Hv > 0 && Hv % Hk == 0, "snnlib.", op, ": the heads of v (", Hv,
+                ") must be a multiple of the heads of q and k (", Hk, ")");
+    TORCH_CHECK(Dk > 0 && Dk <= SNNSEQ_MAX_KEY, "snnlib.", op, ": keys of 1 to ", SNNSEQ_MAX_KEY,
+                " values are supported, got ", Dk);
+    TORCH_CHECK(Dv > 0 && Dv <= SNNSEQ_MAX_VALUE, "snnlib.", op, ": values of 1 to ", SNNSEQ_MAX_VALUE,
+                " values are supported, got ", Dv);
+    TORCH_CHECK(B * Hv <= SNNSEQ_MAX_HEADS, "snnlib.", op, ": at most ", SNNSEQ_MAX_HEADS,
+                " batch entries times heads, got ", B * Hv);
+    for (const auto& p : {std::make_pair(&g, "g"), std::make_pair(&beta, "beta")}) {
+        check_on_gpu(*p.first, op, p.second);
+        TORCH_CHECK(p.first->device() == q.device(), "snnlib.", op, ": ", p.second, " must be on the device of q");
+        TORCH_CHECK(p.first->scalar_type() == at::kFloat, "snnlib.", op, ": ", p.second, " must be float32, got ",
+                    p.first->scalar_type());
+        TORCH_CHECK(p.first->sizes() == v.sizes().slice(0, rank - 1), "snnlib.", op, ": ", p.second,
+                    " must have one value per row of v (", v.sizes().slice(0, rank - 1), "), got ", p.first->sizes());
+    }
+    DeltaOperands o;
+    o.q = dense_rows(q);
+    o.k = dense_rows(k);
+    o.v = dense_rows(v);
+    o.g = dense(g);
+    o.beta = dense(beta);
+    if (state.has_value() && state->defined()) {
+        check_on_gpu(*state, op, "state");
+        TORCH_CHECK(state->device() == q.device() && state->scalar_type() == at::kFloat && state->dim() == 4 &&
+                        state->size(0) == B && state->size(1) == Hv && state->size(2) == Dk && state->size(3) == Dv,
+                    "snnlib.", op, ": state must be float32 [B, heads of v, Dk, Dv] on the device of q, got ",
+                    state->scalar_type(), " ", state->sizes());
+        o.state = dense(*state);
+        o.has_state = true;
+    }
+    if (lengths.has_value() && lengths->defined()) {
+        check_on_gpu(*lengths, op, "lengths");
+        TORCH_CHECK(lengths->device() == q.device() && lengths->scalar_type() == at::kInt && lengths->dim() == 1 &&
+                        lengths->size(0) == B,
+                    "snnlib.", op, ": lengths must be int32 [B] on the device of q, got ", lengths->scalar_type(), " ",
+                    lengths->sizes());
+        o.lengths = dense(*lengths);
+    }
+    snnseq_delta& c = o.call;
+    c = snnseq_delta{};
+    c.T = rank == 4 ? q.size(0) : 1;
+    c.B = B; c.Hk = Hk; c.Hv = Hv; c.Dk = Dk; c.Dv = Dv;
+    strides_of(o.q, c.q_strides);
+    strides_of(o.k, c.k_strides);
+    strides_of(o.v, c.v_strides);
+    c.scale = scale;
+    c.q = o.q.data_ptr(); c.k = o.k.data_ptr(); c.v = o.v.data_ptr();
+    c.g = o.g.data_ptr<float>(); c.beta = o.beta.data_ptr<float>();
+    c.state = o.has_state ? o.state.data_ptr<float>() : nullptr;
+    c.lengths = o.lengths.defined() ? o.lengths.data_ptr<int32_t>() : nullptr;
+    c.dtype = q.scalar_type() == at::kFloat ? SNNLIF_DTYPE_F32 : SNNLIF_DTYPE_BF16;
+    return o;
+}
+
+std::vector<Tensor> gated_delta_fp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, MaybeTensor state,
+                                   MaybeTensor lengths, double scale) {
+    const char* op = "gated_delta_fp";
+    check_on_gpu(q, op, "q");
+    const DeviceGuard guard(q.device());
+    const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
+    Tensor o = torch::empty(v.sizes(), v.options());
+    Tensor state_out = torch::empty({d.call.B, d.call.Hv, d.call.Dk, d.call.Dv}, d.g.options());
+    const size_t bytes = snnseq_gated_delta_saved_bytes(&d.call);
+    Tensor saved = workspace_of(bytes, o);
+    check_rc(snnseq_gated_delta_fp(&d.call, o.data_ptr(), state_out.data_ptr<float>(), saved.data_ptr(), bytes,
+                                   current_stream()),
+             op);
+    return {o, state_out, saved};
+}
+
+std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, MaybeTensor state,
+                                   MaybeTensor lengths, double scale, Tensor saved, Tensor grad_o,
+                                   MaybeTensor grad_state_out) {
+    const char* op = "gated_delta_bp";
+    check_on_gpu(q, op, "q");
+    const DeviceGuard guard(q.device());
+    const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
+    check_like(grad_o, q, op, "grad_o", "q");
+    TORCH_CHECK(grad_o.sizes() == v.sizes(), "snnlib.", op, ": grad_o ", grad_o.sizes(), " and v ", v.sizes(),
+                " must have the same shape");
+    TORCH_CHECK(saved.is_cuda() && saved.device() == q.device() && saved.scalar_type() == at::kByte &&
+                    saved.is_contiguous() &&
+                    static_cast<size_t>(saved.numel()) == snnseq_gated_delta_saved_bytes(&d.call),
+                "snnlib.", op, ": saved must be what gated_delta_fp returned for these operands");
+    Tensor go = dense_rows(grad_o), gs;
+    if (grad_state_out.has_value() && grad_state_out->defined()) {
+        gs = *grad_state_out;
+        TORCH_CHECK(gs.is_cuda() && gs.device() == q.device() && gs.scalar_type() == at::kFloat && gs.dim() == 4 &&
+                        gs.size(0) == d.call.B && gs.size(1) == d.call.Hv && gs.size(2) == d.call.Dk &&
+                        gs.size(3) == d.call.Dv,
+                    "snnlib.", op, ": grad_state_out must be shaped and typed as the state, got ", gs.scalar_type(), " ",
+                    gs.sizes());
+        gs = dense(gs);
+    }
+    Tensor grad_q = torch::empty(q.sizes(), q.options()), grad_k = torch::empty(q.sizes(), q.options());
+    Tensor grad_v = torch::empty(v.sizes(), v.options());
+    Tensor grad_g = torch::empty(g.sizes(), d.g.options()), grad_beta = torch::empty(g.sizes(), d.g.options());
+    Tensor grad_state;
+    if (d.has_state) grad_state = torch::empty(d.state.sizes(), d.state.options());
+    int64_t strides[3];
+    strides_of(go, strides);
+    const size_t bytes = snnseq_gated_delta_bp_workspace_bytes(&d.call);
+    Tensor workspace = workspace_of(bytes, q);
+    check_rc(snnseq_gated_delta_bp(&d.call, saved.data_ptr(), static_cast<size_t>(saved.numel()), go.data_ptr(), strides,
+                                   gs.defined() ? gs.data_ptr<float>() : nullptr, grad_q.data_ptr(), grad_k.data_ptr(),
+                                   grad_v.data_ptr(), grad_g.data_ptr<float>(), grad_beta.data_ptr<float>(),
+                                   d.has_state ? grad_state.data_ptr<float>() : nullptr, workspace.data_ptr(), bytes,
+                                   current_stream()),
+             op);
+    return {grad_q, grad_k, grad_v, grad_g, grad_beta, grad_state};
+}
+
+Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor state, double scale,
+                        MaybeTensor state_out) {
+    const char* op = "gated_delta_step";
+    check_on_gpu(q, op, "q");
+    check_on_gpu(state, op, "state");
+    const DeviceGuard guard(q.device());
+    const DeltaOperands d = delta_operands(q, k, v, g, beta, state, c10::nullopt, scale, 3, op);
+    Tensor out = state_out.has_value() && state_out->defined() ? *state_out : state;
+    TORCH_CHECK(state.is_contiguous() && out.is_contiguous() && out.device() == q.device() &&
+                    out.scalar_type() == at::kFloat && out.sizes() == state.sizes(),
+                "snnlib.", op, ": the state is updated in place, or into state_out: both must be dense float32 ",
+                state.sizes());
+    if (out.data_ptr() != state.data_ptr()) {
+        const char *a = static_cast<char*>(state.data_ptr()), *b = static_cast<char*>(out.data_ptr());
+        const int64_t bytes = state.numel() * 4;
+        TORCH_CHECK(a + bytes <= b || b + bytes <= a, "snnlib.", op, ": state_out must be state or not overlap it");
+    }
+    Tensor o = torch::empty(v.sizes(), v.options());
+    check_rc(snnseq_gated_delta_step(&d.call, o.data_ptr(), out.data_ptr<float>(), current_stream()), op);
+    return o;
+}
+
 }  // namespace
 
 void bind_token_layers(pybind11::module_& m) {
@@ -220,4 +395,7 @@ void bind_token_layers(pybind11::module_& m) {
     m.def("embed_bp", &embed_bp, "gradient of the embedding table, by sorted tokens");
     m.def("gn_act_fp", &gn_act_fp, "group norm with an activation, channels last: [mean, rstd, y]");
     m.def("gn_act_bp", &gn_act_bp, "its backward: [grad_x, grad_weight_gn, grad_bias_gn]");
+    m.def("gated_delta_fp", &gated_delta_fp, "gated delta rule over a sequence: [o, state_out, saved]");
+    m.def("gated_delta_bp", &gated_delta_bp, "its backward: [grad_q, grad_k, grad_v, grad_g, grad_beta, grad_state]");
+    m.def("gated_delta_step", &gated_delta_step, "gated delta rule, one time step: o, the state updated");
 }

@@ -322,6 +322,32 @@ class GnActFunc(torch.autograd.Function):
         return _pad(snnlib.gn_act_bp(*ctx.saved_tensors, ctx.groups, ctx.act, grad_y), 6)
 
 
+class GatedDeltaFunc(torch.autograd.Function):
+    """(o, last state) of the gated delta rule.  Unlike the fire layers this one keeps what its forward
+    computed on the way -- the state before every chunk of 64 steps and the rows added to it -- because the
+    state passes are bound by latency: running them again would cost a third of the backward, and the
+    memory is there."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, lengths, scale):
+        ctx.set_materialize_grads(False)
+        o, state_out, saved = snnlib.gated_delta_fp(q, k, v, g, beta, state, lengths, scale)
+        ctx.save_for_backward(q, k, v, g, beta, state, lengths, saved)
+        ctx.scale = scale
+        return o, state_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_o, grad_state_out):
+        q, k, v, g, beta, state, lengths, saved = ctx.saved_tensors
+        if grad_o is None:
+            if grad_state_out is None:
+                return (None,) * 8
+            grad_o = v.new_zeros(v.shape[-1]).expand(v.shape)
+        grads = snnlib.gated_delta_bp(q, k, v, g, beta, state, lengths, ctx.scale, saved, grad_o, grad_state_out)
+        return (*grads[:5], grads[5] if state is not None else None, None, None)
+
+
 def _records(*tensors):
     """Whether autograd would record an operator on these tensors; without that the token layers call the
     native op directly (a call on a few tokens is over in less time than a recorded node takes)."""
@@ -341,6 +367,32 @@ def gn_act_func(x, weight_gn, bias_gn, groups, eps_gn=1e-5, act="none"):
     if _records(x, weight_gn, bias_gn):
         return GnActFunc.apply(x, weight_gn, bias_gn, groups, eps_gn, act)
     return snnlib.gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act)[2]
+
+
+def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
+    """The gated delta rule over ``T`` steps: ``(o, last state)``.
+
+    Per batch entry and head of ``v``, with ``S`` (``[Dk, Dv]``) starting at ``state`` or zero,
+    ``S_t = exp(g_t) S_{t-1} + beta_t k_t (v_t - exp(g_t) S_{t-1}^T k_t)^T`` and ``o_t = scale * S_t^T q_t``.
+
+    ``q``, ``k`` ``[T, B, Hk, Dk]``, ``v`` ``[T, B, Hv, Dv]`` (float32 or bfloat16, any strides with dense rows; ``Hv``
+    a multiple of ``Hk``, ``Dk`` up to 128), ``g`` (at most zero) and ``beta`` ``[T, B, Hv]`` float32, ``state``
+    ``[B, Hv, Dk, Dv]`` float32, ``lengths`` ``[B]`` int32: steps at or behind a sequence's length do not exist.
+    ``scale`` defaults to ``Dk ** -0.5``."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if _records(q, k, v, g, beta, state):
+        return GatedDeltaFunc.apply(q, k, v, g, beta, state, lengths, scale)
+    return tuple(snnlib.gated_delta_fp(q, k, v, g, beta, state, lengths, scale)[:2])
+
+
+def gated_delta_step(q, k, v, g, beta, state, scale=None, state_out=None):
+    """One step of the gated delta rule for generation: ``q``, ``k`` ``[B, Hk, Dk]``, ``v`` ``[B, Hv, Dv]``, ``g``, ``beta``
+    ``[B, Hv]``; returns ``o`` ``[B, Hv, Dv]`` and updates ``state`` in place, or writes the new state to ``state_out``.
+    Not recorded by autograd: operands that require a gradient are refused unless gradients are off."""
+    if _records(q, k, v, g, beta, state):
+        raise RuntimeError("gated_delta_step is not differentiable: call it under torch.no_grad(), or use gated_delta_func")
+    return snnlib.gated_delta_step(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale, state_out)
 
 
 fire_func = FireFunc.apply

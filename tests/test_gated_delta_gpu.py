@@ -1,0 +1,389 @@
+"""The gated delta rule against its recurrence in 64 bits, step by step, differentiated by autograd.
+
+Tolerances.  The keys have length one and rates lie in [0, 1], so a step's transition has norm one at most: an error
+made in a chunk does not grow behind it, and errors of different chunks add up like independent ones, as the square
+root of their number.  A value passes at most 4 products forward and 8 more backward.  Relative to the norm of a product:
+  * bf16: operands are held to 16 bits (value and remainder, 2**-18 each way, the product of the remainders left out, 2**-18,
+    fp32 accumulation): 2**-16;
+  * fp32: sums of up to 128 products of unit 2**-24, which add up like independent errors: 11 * 2**-24 < 2**-20.
+So ``12 * 2**-16`` (fp32: ``12 * 2**-20``) times sqrt(chunks), normwise, and 8 times that of the largest value for every
+single one.  The gradient of g is a difference of sums of up to 64 rows; its terms can be larger than it is: 8 times.
+A bf16 store adds half a step, 2**-8 at most of the value (2**-9 of the power of two above it).
+"""
+import math
+
+import pytest
+import torch
+
+from snn_gpu_training_bptt_amd import lif_cabi  # noqa: F401
+
+gpu = pytest.mark.gpu
+NAMES = ("q", "k", "v", "g", "beta", "state")
+
+
+@pytest.fixture(scope="module")
+def sf():
+    from snn_gpu_training_bptt_amd import snnlib_func
+    return snnlib_func
+
+
+def make(T, B, Hk, Hv, Dk, Dv, dtype, seed=0, state=True):
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=gen)
+    unit = lambda x: x / x.norm(dim=-1, keepdim=True)
+    x = {"q": unit(rand(T, B, Hk, Dk)).to(dtype), "k": unit(rand(T, B, Hk, Dk)).to(dtype) * 1.0,
+         "v": rand(T, B, Hv, Dv).to(dtype), "g": -0.3 * rand(T, B, Hv).abs(), "beta": torch.sigmoid(rand(T, B, Hv)),
+         "state": 0.5 * rand(B, Hv, Dk, Dv) if state else None}
+    return x, rand(T, B, Hv, Dv).to(dtype), 0.5 * rand(B, Hv, Dk, Dv)
+
+
+def recurrence(x, lengths, scale):
+    """(o, last state) in 64 bits; ``x`` holds 64-bit host tensors."""
+    q, k, v, g, beta, S = (x[n] for n in NAMES)
+    T, B, Hv, Dv = v.shape
+    q, k = (t.repeat_interleave(Hv // k.shape[2], dim=2) for t in (q, k))
+    if S is None:
+        S = torch.zeros(B, Hv, k.shape[-1], Dv, dtype=torch.float64)
+    out = []
+    for t in range(T):
+        here = torch.ones(B, dtype=torch.bool) if lengths is None else t < lengths
+        m = here[:, None, None, None]
+        decayed = torch.exp(g[t])[..., None, None] * S
+        error = beta[t][..., None] * (v[t] - torch.einsum("bhkv,bhk->bhv", decayed, k[t]))
+        S = torch.where(m, decayed + k[t][..., :, None] * error[..., None, :], S)
+        out.append(torch.where(m[..., 0], scale * torch.einsum("bhkv,bhk->bhv", S, q[t]), 0.0))
+    o = torch.stack(out) if out else torch.zeros(0, B, Hv, Dv, dtype=torch.float64)
+    return o, S
+
+
+def reference(x, go, gs, lengths, scale):
+    leaf = {n: None if t is None else t.double().clone().requires_grad_(True) for n, t in x.items()}
+    o, last = recurrence(leaf, lengths, scale)
+    names = [n for n in NAMES if leaf[n] is not None]
+    loss = (o * go.double()).sum() + (last * gs.double()).sum()
+    grads = torch.autograd.grad(loss, [leaf[n] for n in names], allow_unused=True)
+    return {"o": o.detach(), "last": last.detach(),
+            **{"grad_" + n: torch.zeros_like(leaf[n]) if d is None else d for n, d in zip(names, grads)}}
+
+
+def run(sf, x, go, gs, lengths, scale):
+    leaf = {n: None if t is None else t.cuda().requires_grad_(True) for n, t in x.items()}
+    o, last = sf.gated_delta_func(*(leaf[n] for n in NAMES), None if lengths is None else lengths.cuda(), scale)
+    names = [n for n in NAMES if leaf[n] is not None]
+    grads = torch.autograd.grad((o, last), [leaf[n] for n in names], (go.cuda(), gs.cuda()))
+    return {"o": o.detach(), "last": last.detach(), **{"grad_" + n: d for n, d in zip(names, grads)}}
+
+
+def compare(got, want, T, dtype):
+    unit = 12 * (2.0 ** -20 if dtype == torch.float32 else 2.0 ** -16) * math.sqrt(max(1, math.ceil(T / 64)))
+    for name, e in want.items():
+        a = got[name].cpu().double()
+        assert a.shape == e.shape, name
+        assert bool(torch.isfinite(a).all()), name
+        if e.numel() == 0:
+            continue
+        tol = unit * (8 if name == "grad_g" else 1)
+        half = 2.0 ** -8 if got[name].dtype == torch.bfloat16 else 0.0
+        err = (a - e).abs()
+        over = err - half * e.abs() - 8 * tol * e.abs().max() - 1e-30
+        assert bool((over <= 0).all()), f"{name}: off by {float(err.max())} of {float(e.abs().max())}"
+        rel = float((a - e).norm() / (e.norm() + 1e-30))
+        assert rel <= tol + half or float(e.norm()) == 0.0, f"{name}: off by {rel} in norm, allowed {tol + half}"
+
+
+def check(sf, T, B, Hk, Hv, Dk, Dv, dtype, seed=0, state=True, lengths=None, scale=None):
+    x, go, gs = make(T, B, Hk, Hv, Dk, Dv, dtype, seed, state)
+    scale = Dk ** -0.5 if scale is None else scale
+    lengths = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    got = run(sf, x, go, gs, lengths, scale)
+    for n in ("o", "grad_q", "grad_k", "grad_v"):
+        assert got[n].dtype == dtype
+    for n in ("last", "grad_g", "grad_beta"):
+        assert got[n].dtype == torch.float32
+    compare(got, reference(x, go, gs, lengths, scale), T, dtype)
+
+
+DTYPES = [torch.float32, torch.bfloat16]
+both = pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+
+
+@gpu
+@both
+@pytest.mark.parametrize("T", [1, 2, 17, 63, 64, 65, 128, 200])
+def test_lengths_of_time(sf, T, dtype):
+    check(sf, T, 2, 2, 2, 64, 64, dtype, seed=T)
+
+
+@gpu
+@both
+@pytest.mark.parametrize("Dk,Dv", [(1, 1), (16, 200), (33, 7), (63, 32), (64, 33), (65, 65), (96, 80), (128, 128),
+                                   (127, 129), (8, 40)])
+def test_head_sizes(sf, Dk, Dv, dtype):
+    check(sf, 70, 1, 2, 2, Dk, Dv, dtype, seed=Dk)
+
+
+@gpu
+@both
+@pytest.mark.parametrize("Hk,Hv,Dk", [(1, 1, 64), (1, 3, 32), (2, 8, 128), (3, 6, 40)])
+def test_shared_key_heads(sf, Hk, Hv, Dk, dtype):
+    check(sf, 90, 2, Hk, Hv, Dk, 48, dtype, seed=Hv)
+
+
+@gpu
+@both
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("lengths", [[0, 130, 64, 1], [129, 200, -3, 65]])
+def test_ragged_batches(sf, lengths, state, dtype):
+    """Lengths of zero, one, a whole chunk, past the end, negative (none)."""
+    check(sf, 130, 4, 2, 2, 64, 32, dtype, seed=5, lengths=lengths, state=state)
+
+
+@gpu
+@both
+def test_what_lies_behind_a_length_is_not_looked_at(sf, dtype):
+    T, lengths = 150, torch.tensor([100, 3], dtype=torch.int32)
+    x, go, gs = make(T, 2, 1, 2, 64, 40, dtype, seed=6)
+    clean = run(sf, x, go, gs, lengths, 0.2)
+    for n in ("q", "k", "v", "g", "beta"):
+        x[n] = x[n].clone()
+        for b, fill in ((0, float("nan")), (1, float("inf"))):
+            x[n][int(lengths[b]):, b] = fill
+    go = go.clone()
+    go[100:, 0] = float("nan")
+    dirty = run(sf, x, go, gs, lengths, 0.2)
+    for n in clean:
+        assert torch.equal(clean[n], dirty[n]), n
+    assert bool((dirty["o"][100:, 0] == 0).all()) and bool((dirty["grad_g"][3:, 1] == 0).all())
+
+
+@gpu
+@both
+def test_decays_that_forget_everything(sf, dtype):
+    """g of -inf, of the type's lowest value and of -200 inside a chunk and at its borders; and no decay at all."""
+    T = 140
+    x, go, gs = make(T, 1, 1, 2, 64, 32, dtype, seed=7)
+    x["g"][:, :, 1] = 0.0
+    for t, value in ((0, -200.0), (20, float("-inf")), (63, float("-inf")), (64, torch.finfo(torch.float32).min), (100, -200.0)):
+        x["g"][t, 0, 0] = value
+    want = dict(x, g=x["g"].clamp_min(-200.0))          # e^-200 is zero to all purposes and has a derivative
+    compare(run(sf, x, go, gs, None, 0.2), reference(want, go, gs, None, 0.2), T, dtype)
+
+
+@gpu
+@both
+def test_rates_of_zero_and_one_and_repeated_keys(sf, dtype):
+    T = 100
+    x, go, gs = make(T, 1, 2, 2, 32, 32, dtype, seed=8)
+    x["beta"][::3] = 0.0
+    x["beta"][1::3] = 1.0
+    x["k"][10:40] = x["k"][10:11]                       # the same key, replaced again and again
+    compare(run(sf, x, go, gs, None, 0.3), reference(x, go, gs, None, 0.3), T, dtype)
+
+
+@gpu
+@both
+def test_operands_as_they_lie(sf, dtype):
+    """q, k and v cut out of one projection, batch-first tensors seen time-first, rows off 16 bytes, an expanded
+    gradient: the values of dense operands, up to the order of the loads (none)."""
+    T, B, H, D = 80, 3, 2, 64
+    x, go, gs = make(T, B, H, H, D, D, dtype, seed=9)
+    want = run(sf, x, go, gs, None, 0.125)
+    fused = torch.cat([x[n] for n in ("q", "k", "v")], dim=-1).cuda()
+    cut = {n: fused[..., i * D:(i + 1) * D] for i, n in enumerate(("q", "k", "v"))}
+    first = {n: x[n].cuda().transpose(0, 1).contiguous().transpose(0, 1) for n in ("q", "k", "v", "g", "beta")}
+    odd = {}
+    for n in ("q", "k", "v"):
+        wide = torch.zeros(T, B, H, D + 3, dtype=dtype, device="cuda")
+        wide[..., 1:D + 1] = x[n].cuda()
+        odd[n] = wide[..., 1:D + 1]
+    last = {n: x[n].cuda().transpose(2, 3).contiguous().transpose(2, 3) for n in ("q", "k", "v")}  # rows not dense
+    for views in (cut, first, odd, last):
+        y = {n: views.get(n, t) for n, t in x.items()}
+        got = run(sf, y, go, gs, None, 0.125)
+        for n in want:
+            assert torch.equal(got[n], want[n]), n
+    one = go[:1, :, :1].expand(T, B, H, D)
+    got, want = run(sf, x, one, gs, None, 0.125), run(sf, x, one.contiguous(), gs, None, 0.125)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
+@gpu
+@both
+def test_one_output_alone_has_a_gradient(sf, dtype):
+    T = 70
+    x, go, gs = make(T, 2, 1, 2, 32, 16, dtype, seed=10)
+    leaf = {n: t.cuda().requires_grad_(True) for n, t in x.items()}
+    for which, zero_o, zero_s in (("o", 1.0, 0.0), ("last", 0.0, 1.0)):
+        o, last = sf.gated_delta_func(*(leaf[n] for n in NAMES), None, 0.5)
+        out, g = (o, go) if which == "o" else (last, gs)
+        grads = torch.autograd.grad(out, [leaf[n] for n in NAMES], g.cuda())
+        compare({"grad_" + n: d for n, d in zip(NAMES, grads)},
+                {n: t for n, t in reference(x, go * zero_o, gs * zero_s, None, 0.5).items() if n.startswith("grad")},
+                T, dtype)
+
+
+@gpu
+def test_gradients_against_differences(sf):
+    """Along one direction per operand, by central differences of the fp32 forward.  Step 2**-6: the third derivative
+    contributes a relative 2**-12 / 6 times its ratio to the first (some tens), rounding 2**-20 / 2**-6."""
+    T = 75
+    x, go, gs = make(T, 1, 1, 2, 32, 24, torch.float32, seed=11)
+    cuda = {n: t.cuda() for n, t in x.items()}
+    grads = run(sf, x, go, gs, None, 0.4)
+    gen = torch.Generator().manual_seed(12)
+
+    def loss(**changed):
+        y = {**cuda, **changed}
+        o, last = sf.gated_delta_func(*(y[n] for n in NAMES), None, 0.4)
+        return float((o.double() * go.cuda().double()).sum() + (last.double() * gs.cuda().double()).sum())
+
+    for n in NAMES:
+        way = torch.randn(x[n].shape, generator=gen).cuda()
+        way = way / way.norm() * 4 if n != "state" else way
+        h = 2.0 ** -6
+        slope = (loss(**{n: cuda[n] + h * way}) - loss(**{n: cuda[n] - h * way})) / (2 * h)
+        exact = float((grads["grad_" + n].double() * way.double()).sum())
+        size = float(grads["grad_" + n].double().norm() * way.double().norm())
+        assert abs(slope - exact) <= 0.01 * size, (n, slope, exact, size)
+
+
+@gpu
+@both
+@pytest.mark.parametrize("B,Hk,Hv,Dk,Dv", [(1, 1, 1, 64, 64), (5, 2, 4, 128, 128), (3, 1, 2, 33, 70), (2, 2, 2, 1, 1),
+                                           (2, 1, 1, 65, 130), (2, 1, 1, 17, 63)])
+def test_steps_follow_the_sequence(sf, B, Hk, Hv, Dk, Dv, dtype):
+    """Token by token, from a state, in place: the outputs of the whole sequence and its last state."""
+    T = 9
+    x, _, _ = make(T, B, Hk, Hv, Dk, Dv, dtype, seed=13)
+    want_o, want_last = recurrence({n: t.double() for n, t in x.items()}, None, 0.7)
+    state = x["state"].cuda().clone()
+    out = [sf.gated_delta_step(*(x[n][t].cuda() for n in ("q", "k", "v", "g", "beta")), state, 0.7) for t in range(T)]
+    # fp32 throughout, whatever the storage
+    o = torch.stack(out).cpu().double()
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    assert bool(((o - want_o).abs() <= half * want_o.abs() + 1e-5 * want_o.abs().max()).all())
+    assert bool(((state.cpu().double() - want_last).abs() <= 1e-5 * want_last.abs().max()).all())
+
+
+@gpu
+@both
+def test_a_step_into_another_state_from_strided_rows(sf, dtype):
+    x, _, _ = make(1, 3, 2, 4, 64, 96, dtype, seed=14)
+    row = {n: x[n][0].cuda() for n in ("q", "k", "v", "g", "beta")}
+    state = x["state"].cuda()
+    kept = state.clone()
+    out = torch.full_like(state, float("nan"))
+    o = sf.gated_delta_step(*row.values(), state, None, out)
+    assert torch.equal(state, kept)
+    wide = {n: torch.zeros(3, t.shape[1], t.shape[2] + 5, dtype=dtype, device="cuda") for n, t in row.items() if t.dim() == 3}
+    for n, w in wide.items():
+        w[..., 5:] = row[n]
+    o2 = sf.gated_delta_step(wide["q"][..., 5:], wide["k"][..., 5:], wide["v"][..., 5:], row["g"], row["beta"], state)
+    assert torch.equal(o, o2) and torch.equal(out, state)
+
+
+@gpu
+@both
+def test_a_step_that_forgets_everything(sf, dtype):
+    x, _, _ = make(1, 1, 1, 1, 16, 16, dtype, seed=15)
+    row = [x[n][0].cuda() for n in ("q", "k", "v", "g", "beta")]
+    row[3] = torch.full_like(row[3], float("-inf"))
+    state = x["state"].cuda().clone()
+    sf.gated_delta_step(*row, state)
+    want = row[1][0, 0].float()[:, None] * row[4][0, 0] * row[2][0, 0].float()[None, :]
+    torch.testing.assert_close(state[0, 0], want, rtol=1e-6, atol=1e-7)
+
+
+@gpu
+@pytest.mark.parametrize("T,B", [(0, 2), (5, 0), (0, 0)])
+def test_nothing_to_do(sf, T, B):
+    x, go, gs = make(T, B, 1, 2, 16, 16, torch.float32)
+    got = run(sf, x, go, gs, None, 1.0)
+    assert got["o"].shape == (T, B, 2, 16)
+    assert torch.equal(got["last"].cpu(), x["state"]) and torch.equal(got["grad_state"].cpu(), gs)
+
+
+@gpu
+@both
+def test_reproducible_on_any_stream_and_under_no_grad(sf, dtype):
+    x, go, gs = make(200, 2, 1, 2, 128, 64, dtype, seed=16)
+    first = run(sf, x, go, gs, None, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run(sf, x, go, gs, None, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    for n in first:
+        assert torch.equal(first[n], second[n]), n
+    with torch.no_grad():
+        o, last = sf.gated_delta_func(*(x[n].cuda() for n in NAMES), None, 0.1)
+    assert torch.equal(o, first["o"]) and torch.equal(last, first["last"])
+
+
+@gpu
+def test_captured_and_replayed(sf):
+    x, go, gs = make(130, 2, 1, 2, 64, 64, torch.bfloat16, seed=17)
+    y = {n: t.cuda() for n, t in x.items()}
+    go, gs = go.cuda(), gs.cuda()
+    args = lambda: (*(y[n] for n in NAMES), None, 0.2)
+
+    def step():
+        o, last, saved = sf.snnlib.gated_delta_fp(*args())
+        return [o, last] + sf.snnlib.gated_delta_bp(*args(), saved, go, gs)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    gen = torch.Generator().manual_seed(1)
+    for _ in range(4):
+        y["v"].copy_(torch.randn(y["v"].shape, generator=gen))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(out, want))
+
+
+@gpu
+def test_refusals(sf):
+    x, go, gs = make(4, 2, 2, 4, 16, 8, torch.float32)
+    y = {n: t.cuda() for n, t in x.items()}
+    f = lambda **c: sf.gated_delta_func(*({**y, **c}[n] for n in NAMES), c.get("lengths"), 1.0)
+    for change, match in [({"q": y["q"].double(), "k": y["k"].double(), "v": y["v"].double()}, "only float32 and bfloat16"),
+                          ({"q": y["q"][:3]}, "same shape"), ({"k": y["k"].bfloat16()}, "dtype of q"),
+                          ({"v": y["v"][:, :, :3]}, "multiple of the heads"), ({"v": y["v"][:3]}, "must share"),
+                          ({"v": y["v"][0]}, "must be shaped"), ({"g": y["g"].bfloat16()}, "must be float32"),
+                          ({"beta": y["beta"][:, :, :1]}, "one value per row"), ({"k": y["k"].cpu()}, "ROCm GPU"),
+                          ({"state": y["state"].bfloat16()}, "state must be"), ({"state": y["state"][:1]}, "state must be"),
+                          ({"lengths": torch.tensor([1, 2]).cuda()}, "lengths must be int32"),
+                          ({"lengths": torch.tensor([1], dtype=torch.int32).cuda()}, "lengths must be int32"),
+                          ({"q": torch.zeros(4, 2, 2, 129).cuda(), "k": torch.zeros(4, 2, 2, 129).cuda()}, "1 to 128")]:
+        with pytest.raises(RuntimeError, match=match):
+            f(**change)
+    o, last, saved = sf.snnlib.gated_delta_fp(*(y[n] for n in NAMES), None, 1.0)
+    with pytest.raises(RuntimeError, match="what gated_delta_fp returned"):
+        sf.snnlib.gated_delta_bp(*(y[n] for n in NAMES), None, 1.0, saved[1:], o, None)
+    row = [y[n][0] for n in ("q", "k", "v", "g", "beta")]
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        sf.gated_delta_step(*row, y["state"].requires_grad_(True))
+    state = y["state"].detach()
+    with pytest.raises(RuntimeError, match="dense"):
+        sf.gated_delta_step(*row, torch.empty(2, 4, 8, 16).cuda().transpose(2, 3).copy_(state))
+    flat = torch.zeros(state.numel() + 4).cuda()
+    with pytest.raises(RuntimeError, match="not overlap"):
+        sf.gated_delta_step(*row, flat[:-4].view(state.shape), None, flat[4:].view(state.shape))
+    with pytest.raises(RuntimeError, match="must be shaped"):
+        sf.gated_delta_step(*(y[n] for n in ("q", "k", "v", "g", "beta")), state)
+
+
+def test_a_host_tensor_is_refused(sf):
+    x, _, _ = make(4, 1, 1, 1, 4, 4, torch.float32)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        sf.gated_delta_func(*(x[n] for n in NAMES))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        sf.gated_delta_step(*(x[n][0] for n in NAMES[:5]), x["state"])
