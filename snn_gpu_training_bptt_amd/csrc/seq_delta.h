@@ -25,7 +25,7 @@
 //
 // Kernels.  Everything that does not hang on the state runs over all chunks and heads at once; the two passes that do
 // (delta_state_kernel forwards, delta_state_grad_kernel backwards) walk the chunks of a head, one workgroup per head
-// and 32 columns of the state, which they hold in accumulators.
+// and 16 columns of the state, which they hold in accumulators.
 //   forward    delta_inverse_kernel -> Tm;   delta_state_kernel -> S of every chunk, R, last state;   delta_output_kernel -> O
 //   backward   delta_inner_grad_kernel -> P^T dO;   delta_state_grad_kernel -> dS' of every chunk, dX;
 //              delta_input_grad_kernel -> the gradients;   delta_shared_grad_kernel where heads share keys
@@ -33,10 +33,12 @@
 // through LDS), the others by memory.
 //
 // Numbers.  States, R, Tm, dX and every sum are fp32.  In bf16 storage the products run on the bf16 matrix
-// instructions; an input is exact there, and everything derived (Tm, X, R, P, the state, ...) is given as two bf16
-// parts, value and remainder, which together keep 16 bits: rounding it once would cost a relative 2^-9 in each
-// product and show up in the fp32 gradients and states.  The product of the two remainders is left out (2^-18).
-// In fp32 storage they run on the fp32 matrix instructions.  The sums c are held in 64 bits: G needs differences.
+// instructions; an input is exact there, and what is derived (Tm, X, R, P, the state, ...) is given as a sum of bf16
+// parts.  Three parts keep all 24 bits and are used wherever a product reaches an fp32 result (the state, the
+// gradients of g and beta): with two, their errors came out ten times those of an fp32 evaluation (4e-6 against 4e-7).
+// Two parts (16 bits) are used where all that follows is a bf16 store.  Products of parts below the last bit kept are
+// left out.  In fp32 storage the products run on the fp32 matrix instructions.  The sums c are held in 64 bits: G
+// needs their differences.
 //
 // Time steps at or behind a sequence's length have no row: they leave the state alone and their outputs are zero.
 #ifndef SNNLIF_SEQ_DELTA_H
@@ -47,7 +49,8 @@
 namespace snnseq {
 
 constexpr int kChunk = 64;
-constexpr int kStateCols = 32;  // columns of the state a workgroup of the state passes holds
+constexpr int kStateCols = 16;  // columns of the state a workgroup of the state passes holds
+constexpr int kCols = 32;       // columns of the state the other kernels take at a time
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -88,6 +91,28 @@ __device__ __forceinline__ float value_of(uint16_t bits) {
     return __builtin_bit_cast(float, static_cast<uint32_t>(bits) << 16);
 }
 
+// Eight consecutive values as they lie in memory.
+template <typename E> struct Raw8 { u32x4 r[sizeof(E) / 2]; };
+
+// n values as bf16 parts: words[part][j] holds values 2j and 2j + 1.
+template <int N, int n>
+__device__ __forceinline__ void split(const float (&x)[n], uint32_t (&words)[N][n / 2]) {
+    float rest[n];
+#pragma unroll
+    for (int j = 0; j < n; ++j) rest[j] = x[j];
+#pragma unroll
+    for (int part = 0; part < N; ++part)
+#pragma unroll
+        for (int j = 0; j < n; j += 2) {
+            const uint16_t lo = bits_of(rest[j]), hi = bits_of(rest[j + 1]);
+            words[part][j / 2] = lo | static_cast<uint32_t>(hi) << 16;
+            if (part + 1 < N) {
+                rest[j] -= value_of(lo);
+                rest[j + 1] -= value_of(hi);
+            }
+        }
+}
+
 // A matrix in LDS as N bf16 parts, row-major; 16 bytes of padding per row spread the rows over the banks.
 template <int N, int ROWS, int COLS>
 struct TileH {
@@ -97,22 +122,13 @@ struct TileH {
     // n consecutive columns, c a multiple of 4
     template <int n>
     __device__ __forceinline__ void put(int r, int c, const float (&x)[n]) {
-        float rest[n];
-#pragma unroll
-        for (int j = 0; j < n; ++j) rest[j] = x[j];
+        uint32_t words[N][n / 2];
+        split<N, n>(x, words);
 #pragma unroll
         for (int part = 0; part < N; ++part) {
-            uint32_t words[n / 2];
-#pragma unroll
-            for (int j = 0; j < n; j += 2) {
-                const uint16_t lo = bits_of(rest[j]), hi = bits_of(rest[j + 1]);
-                words[j / 2] = lo | static_cast<uint32_t>(hi) << 16;
-                rest[j] -= value_of(lo);
-                rest[j + 1] -= value_of(hi);
-            }
             uint16_t* p = &v[part][r * ld + c];
-            if constexpr (n == 8) *reinterpret_cast<u32x4*>(p) = u32x4{words[0], words[1], words[2], words[3]};
-            else *reinterpret_cast<u32x2*>(p) = u32x2{words[0], words[1]};
+            if constexpr (n == 8) *reinterpret_cast<u32x4*>(p) = u32x4{words[part][0], words[part][1], words[part][2], words[part][3]};
+            else *reinterpret_cast<u32x2*>(p) = u32x2{words[part][0], words[part][1]};
         }
     }
     __device__ __forceinline__ void put(int r, int c, float x) {
@@ -123,14 +139,14 @@ struct TileH {
             x -= value_of(b);
         }
     }
-    __device__ __forceinline__ void put_raw(int r, int c, u32x4 raw) {
-        static_assert(N == 1, "raw storage is one part");
-        *reinterpret_cast<u32x4*>(&v[0][r * ld + c]) = raw;
+    __device__ __forceinline__ void put(int r, int c, const Raw8<bf16_t>& x) {
+        static_assert(N == 1, "what lies in memory is one part");
+        *reinterpret_cast<u32x4*>(&v[0][r * ld + c]) = x.r[0];
     }
     __device__ __forceinline__ float get(int r, int c) const {
-        float x = 0.f;
+        float x = value_of(v[N - 1][r * ld + c]);
 #pragma unroll
-        for (int part = 0; part < N; ++part) x += value_of(v[part][r * ld + c]);
+        for (int part = N - 2; part >= 0; --part) x += value_of(v[part][r * ld + c]);
         return x;
     }
     // operand indexed by rows r0 .., contracted over columns k0 ..
@@ -175,6 +191,10 @@ struct TileF {
             *reinterpret_cast<f32x4*>(&v[r * ld + c + j]) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
     }
     __device__ __forceinline__ void put(int r, int c, float x) { v[r * ld + c] = x; }
+    __device__ __forceinline__ void put(int r, int c, const Raw8<float>& x) {
+        *reinterpret_cast<u32x4*>(&v[r * ld + c]) = x.r[0];
+        *reinterpret_cast<u32x4*>(&v[r * ld + c + 4]) = x.r[1];
+    }
     __device__ __forceinline__ float get(int r, int c) const { return v[r * ld + c]; }
     __device__ __forceinline__ FragF rows(int r0, int k0) const {
         const int lane = threadIdx.x & 63;
@@ -197,15 +217,20 @@ struct TileF {
     }
 };
 
-// What a storage type computes with: tiles of inputs and of derived values.
+// What a storage type computes with: tiles of inputs, and of derived values on the way to fp32 results (Fine) or to
+// results of the storage type (Coarse).  kSquareParts: how a 64 x 64 matrix is handed from kernel to kernel.
 template <typename E> struct Mode;
 template <> struct Mode<bf16_t> {
     template <int R, int C> using Input = TileH<1, R, C>;
-    template <int R, int C> using Derived = TileH<2, R, C>;
+    template <int R, int C> using Fine = TileH<3, R, C>;
+    template <int R, int C> using Coarse = TileH<2, R, C>;
+    static constexpr int square_bytes = 3 * 2 * kChunk * kChunk;
 };
 template <> struct Mode<float> {
     template <int R, int C> using Input = TileF<R, C>;
-    template <int R, int C> using Derived = TileF<R, C>;
+    template <int R, int C> using Fine = TileF<R, C>;
+    template <int R, int C> using Coarse = TileF<R, C>;
+    static constexpr int square_bytes = 4 * kChunk * kChunk;
 };
 
 // ---- arguments ----------------------------------------------------------------------------------
@@ -217,10 +242,17 @@ struct DeltaTensor {
     int wide;          // every row begins on 16 bytes and D is a multiple of 8
 };
 
+// Decay of a chunk: the sums c in 64 bits and in units of log 2, a = e^c, d = e^{c_last - c}, and beta.  A row that
+// does not exist has g = 0 and beta = 0.
+struct Decay {
+    double c[kChunk];
+    float a[kChunk], d[kChunk], beta[kChunk];
+};
+
 struct DeltaArgs {
     int T, B, Hk, Hv, Dk, Dv;
     int chunks;                 // ceil(T / 64)
-    int cols;                   // Dv rounded up to 32: row length of the workspace's matrices
+    int cols;                   // Dv rounded up to 32: columns of the matrices below
     float scale;
     const int32_t* lengths;     // [B] or nullptr
     DeltaTensor q, k, v, grad_o;
@@ -228,13 +260,15 @@ struct DeltaArgs {
     const float *state, *grad_state;   // [B, Hv, Dk, Dv] or nullptr: the initial state, the gradient of the last one
     void* o;                    // [T, B, Hv, Dv]
     float* state_out;           // [B, Hv, Dk, Dv] or nullptr
-    // per (batch entry, value head, chunk)
-    float* inverse;             // [64, 64] Tm
-    float* added;               // [64, cols] R
-    float* states;              // [DKP, cols] state before the chunk
+    // per (batch entry, value head, chunk); matrices with a column of the state are transposed, as the state passes
+    // hold them: each column of theirs is one run of memory
+    Decay* decay;
+    char* inverse;              // Tm [64, 64], Mode::square_bytes
+    float* added;               // R, [cols, 64]
+    float* states;              // state before the chunk, [cols, DKP]
     // backward
-    float* inner;               // [64, cols] P^T dO, then dX
-    float* state_grads;         // [DKP, cols] gradient of the state after the chunk
+    float* inner;               // P^T dO, then dX, [cols, 64]
+    float* state_grads;         // gradient of the state after the chunk, [cols, DKP]
     void *grad_q, *grad_k;      // [T, B, Hk, Dk] of the storage type, or fp32 [T, B, Hv, Dk] where heads share keys
     void* grad_v;               // [T, B, Hv, Dv]
     float *grad_g, *grad_beta;  // [T, B, Hv]
@@ -244,6 +278,7 @@ struct DeltaArgs {
 struct DeltaWhere {  // the chunk (or head) a workgroup works on
     int b, hv, hk, chunk, head;
     int t0, rows;    // first step and how many of its 64 rows exist
+    int64_t at;      // its place among the matrices
 };
 
 __device__ __forceinline__ int delta_length(const DeltaArgs& a, int b) {
@@ -262,6 +297,7 @@ __device__ __forceinline__ DeltaWhere delta_where(const DeltaArgs& a, int head, 
     w.t0 = chunk * kChunk;
     const int left = delta_length(a, w.b) - w.t0;
     w.rows = left < 0 ? 0 : left > kChunk ? kChunk : left;
+    w.at = static_cast<int64_t>(head) * a.chunks + chunk;
     return w;
 }
 
@@ -269,53 +305,109 @@ __device__ __forceinline__ DeltaWhere delta_where(const DeltaArgs& a, int head, 
 
 // Eight consecutive values of a row, zero behind `valid`.
 template <typename E>
-__device__ __forceinline__ void load8(const E* row, int c, int valid, bool wide, float (&x)[8]) {
-    constexpr int per = 16 / static_cast<int>(sizeof(E));
+__device__ __forceinline__ Raw8<E> load_raw8(const E* row, int c, int valid, bool wide) {
+    Raw8<E> x;
+#pragma unroll
+    for (u32x4& part : x.r) part = u32x4{0, 0, 0, 0};
     if (wide) {
         if (c < valid) {
 #pragma unroll
-            for (int h = 0; h < 8 / per; ++h) {
-                const Vec<E, 16> v = load_vec<E, 16>(row + c + h * per);
-#pragma unroll
-                for (int j = 0; j < per; ++j) x[h * per + j] = widen(v.e[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = 0.f;
+            for (int h = 0; h < static_cast<int>(sizeof(E) / 2); ++h) x.r[h] = reinterpret_cast<const u32x4*>(row + c)[h];
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = c + j < valid ? widen(row[c + j]) : 0.f;
+        for (int j = 0; j < 8; ++j)
+            if (c + j < valid) {
+                if constexpr (sizeof(E) == 4) x.r[j / 4][j % 4] = __builtin_bit_cast(uint32_t, row[c + j]);
+                else x.r[0][j / 2] |= static_cast<uint32_t>(row[c + j].bits) << (j % 2 * 16);
+            }
+    }
+    return x;
+}
+
+__device__ __forceinline__ void values_of(const Raw8<bf16_t>& x, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __builtin_bit_cast(float, x.r[0][j] << 16);
+        v[2 * j + 1] = __builtin_bit_cast(float, x.r[0][j] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void values_of(const Raw8<float>& x, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t bits = x.r[j / 4][j % 4];   // a bit cast of the vector's element itself reads element 0
+        v[j] = __builtin_bit_cast(float, bits);
     }
 }
 
-// ROWS x COLS of a tensor with `stride` values from row to row, of which `rows` x `valid` exist.
-template <int ROWS, int COLS, int THREADS, typename E, typename Tile>
-__device__ __forceinline__ void stage(Tile& tile, const E* base, int64_t stride, int rows, int valid, bool wide) {
+// ROWS x COLS of a tensor, eight values of a row per access, requested now (load) and put into LDS later (store), so
+// that a product can run in between.
+template <typename E, int ROWS, int COLS, int THREADS>
+struct Ahead {
+    static constexpr int total = ROWS * COLS / 8, n = (total + THREADS - 1) / THREADS;
+    Raw8<E> x[n];
+    // rows `stride` values apart, of which `rows` x `valid` exist
+    __device__ __forceinline__ void load(const E* base, int64_t stride, int rows, int valid, bool wide) {
 #pragma unroll
-    for (int i = 0; i < ROWS * COLS / 8; i += THREADS) {
-        const int seg = i + threadIdx.x;
-        if (ROWS * COLS / 8 % THREADS != 0 && seg >= ROWS * COLS / 8) break;
-        const int r = seg / (COLS / 8), c = seg % (COLS / 8) * 8;
-        float x[8];
-        load8<E>(base + (r < rows ? r : 0) * stride, c, r < rows ? valid : 0, wide, x);
-        tile.put(r, c, x);
+        for (int i = 0; i < n; ++i) {
+            const int seg = i * THREADS + threadIdx.x, r = seg / (COLS / 8), c = seg % (COLS / 8) * 8;
+            x[i] = load_raw8<E>(base + (r < rows ? r : 0) * stride, c, r < rows ? valid : 0, wide);
+        }
     }
-}
+    template <typename Tile>
+    __device__ __forceinline__ void store(Tile& tile) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int seg = i * THREADS + threadIdx.x;
+            if (total % THREADS != 0 && seg >= total) break;
+            tile.put(seg / (COLS / 8), seg % (COLS / 8) * 8, x[i]);
+        }
+    }
+    // through fp32 values, for tiles of several parts
+    template <typename Tile>
+    __device__ __forceinline__ void store_values(Tile& tile) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int seg = i * THREADS + threadIdx.x;
+            if (total % THREADS != 0 && seg >= total) break;
+            float v[8];
+            values_of(x[i], v);
+            tile.put(seg / (COLS / 8), seg % (COLS / 8) * 8, v);
+        }
+    }
+};
+
+// A 64 x 64 matrix in the form kernels hand to each other: its parts, without padding.
+template <typename E, int THREADS>
+struct SquareAhead {
+    static constexpr int n = Mode<E>::square_bytes / 16 / THREADS;
+    u32x4 x[n];
+    __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) x[i] = reinterpret_cast<const u32x4*>(p)[i * THREADS + threadIdx.x];
+    }
+    __device__ __forceinline__ void store(TileH<3, kChunk, kChunk>& tile) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int seg = i * THREADS + threadIdx.x, part = seg / 512, r = seg % 512 / 8, c = seg % 8 * 8;
+            *reinterpret_cast<u32x4*>(&tile.v[part][r * tile.ld + c]) = x[i];
+        }
+    }
+    __device__ __forceinline__ void store(TileF<kChunk, kChunk>& tile) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const int seg = i * THREADS + threadIdx.x, r = seg / 16, c = seg % 16 * 4;
+            *reinterpret_cast<u32x4*>(&tile.v[r * tile.ld + c]) = x[i];
+        }
+    }
+};
 
 template <typename E>
 __device__ __forceinline__ const E* row_of(const DeltaTensor& x, const DeltaWhere& w, int head) {
     return static_cast<const E*>(x.p) + w.t0 * x.t + w.b * x.b + head * x.h;
 }
 
-// Decay of a chunk: sums c (64 bits), a = e^c, d = e^{c_last - c}, and beta; by the first wavefront.  A row that does
-// not exist has g = 0 and beta = 0.
-struct Decay {
-    double c[kChunk];
-    float a[kChunk], d[kChunk], beta[kChunk];
-    float a_last;
-};
-
+// By the first wavefront.
 __device__ __forceinline__ void decay_of(const DeltaArgs& args, const DeltaWhere& w, Decay& out) {
     const int lane = threadIdx.x;
     if (lane >= 64) return;
@@ -326,7 +418,7 @@ __device__ __forceinline__ void decay_of(const DeltaArgs& args, const DeltaWhere
         beta = args.beta[at];
         g = g < -1e4f ? -1e4f : g;   // e^-10000 is zero; sums and differences stay finite (a NaN stays)
     }
-    double c = g;
+    double c = g * 1.4426950408889634;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
         const double other = __shfl_up(c, s);
@@ -334,17 +426,29 @@ __device__ __forceinline__ void decay_of(const DeltaArgs& args, const DeltaWhere
     }
     const double last = __shfl(c, 63);
     out.c[lane] = c;
-    out.a[lane] = expf(static_cast<float>(c));
-    out.d[lane] = expf(static_cast<float>(last - c));
+    out.a[lane] = exp2f(static_cast<float>(c));
+    out.d[lane] = exp2f(static_cast<float>(last - c));
     out.beta[lane] = beta;
-    if (lane == 63) out.a_last = expf(static_cast<float>(c));
+}
+
+__device__ __forceinline__ void load_decay(const DeltaArgs& args, const DeltaWhere& w, Decay& out) {
+    static_assert(sizeof(Decay) == 16 * 80, "a Decay is copied in vectors");
+    if (threadIdx.x < sizeof(Decay) / 16)
+        reinterpret_cast<u32x4*>(&out)[threadIdx.x] = reinterpret_cast<const u32x4*>(args.decay + w.at)[threadIdx.x];
 }
 
 __device__ __forceinline__ float gap(const Decay& y, int i, int j) {  // G_ij
-    return expf(static_cast<float>(y.c[i] - y.c[j]));
+    return __builtin_amdgcn_exp2f(static_cast<float>(y.c[i] - y.c[j]));
 }
 
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+
+// Workgroups go to the eight XCDs in turn, each with an L2 of its own: the workgroups of a head, which read the same
+// keys and matrices, are given to one XCD.
+__device__ __forceinline__ int piece_in_l2(int total) {
+    const int per = total / 8, id = blockIdx.x;
+    return id < per * 8 ? (id % 8) * per + id / 8 : id;
+}
 
 // ---- Tm = (I + A)^-1 ----------------------------------------------------------------------------
 
@@ -400,20 +504,29 @@ __device__ __forceinline__ void invert_unit_lower(const Square& a, Square& t, Sq
 template <typename E, int DKP>
 __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
     using M = Mode<E>;
-    __shared__ typename M::template Input<kChunk, DKP> k;
-    __shared__ Square a, t, scratch;
+    union First {   // K is done with when the inversion needs its scratch
+        typename M::template Input<kChunk, DKP> k;
+        Square scratch;
+        __device__ First() {}
+    };
+    __shared__ First u;
+    __shared__ Square a, t;
     __shared__ Decay y;
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
     if (w.rows == 0) return;
-    stage<kChunk, DKP, 256>(k, row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+    Ahead<E, kChunk, DKP, 256> k;
+    k.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
     decay_of(args, w, y);
     for (int i = threadIdx.x; i < kChunk * (kChunk + 4); i += 256) (&t.v[0][0])[i] = 0.f;
+    k.store(u.k);
     __syncthreads();
+    if (threadIdx.x < sizeof(Decay) / 16)
+        reinterpret_cast<u32x4*>(args.decay + w.at)[threadIdx.x] = reinterpret_cast<const u32x4*>(&y)[threadIdx.x];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int block = 0; block <= wave; ++block) {
         f32x4 acc = zero4();
 #pragma unroll
-        for (int s = 0; s < DKP; s += 32) acc = mma(k.rows(wave * 16, s), k.rows(block * 16, s), acc);
+        for (int s = 0; s < DKP; s += 32) acc = mma(u.k.rows(wave * 16, s), u.k.rows(block * 16, s), acc);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = wave * 16 + (lane >> 4) * 4 + e, j = block * 16 + (lane & 15);
@@ -421,238 +534,312 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
         }
     }
     __syncthreads();
-    invert_unit_lower(a, t, scratch);
-    float* out = args.inverse + (static_cast<int64_t>(w.head) * args.chunks + w.chunk) * (kChunk * kChunk);
+    invert_unit_lower(a, t, u.scratch);
+    char* out = args.inverse + w.at * M::square_bytes;
 #pragma unroll
-    for (int i = 0; i < kChunk * kChunk / 4; i += 256) {
-        const int r = (i + threadIdx.x) / 16, c = (i + threadIdx.x) % 16 * 4;
-        *reinterpret_cast<f32x4*>(out + r * kChunk + c) = *reinterpret_cast<const f32x4*>(&t.v[r][c]);
+    for (int i = 0; i < kChunk * kChunk / 8; i += 256) {
+        const int seg = i + threadIdx.x, r = seg / 8, c = seg % 8 * 8;
+        if constexpr (sizeof(E) == 4) {
+            reinterpret_cast<f32x4*>(out)[seg * 2] = *reinterpret_cast<const f32x4*>(&t.v[r][c]);
+            reinterpret_cast<f32x4*>(out)[seg * 2 + 1] = *reinterpret_cast<const f32x4*>(&t.v[r][c + 4]);
+        } else {
+            float x[8];
+            uint32_t words[3][4];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = t.v[r][c + j];
+            split<3, 8>(x, words);
+#pragma unroll
+            for (int part = 0; part < 3; ++part)
+                reinterpret_cast<u32x4*>(out)[part * 512 + seg] = u32x4{words[part][0], words[part][1], words[part][2], words[part][3]};
+        }
     }
 }
 
-// ---- the state, forwards ------------------------------------------------------------------------
+// ---- the state passes ---------------------------------------------------------------------------
+//
+// A workgroup of four wavefronts holds kStateCols columns of a head's state: wavefront w rows 16 w.. of the chunk in
+// the first two products, DKP / 64 tiles of 16 state rows in the last one.  What the next chunk needs is requested
+// before the products of this one and put into LDS after them.
 
-constexpr int kStateThreads = 512;
+constexpr int kStateThreads = 256;
+
+// The 4 x TILES state values of a lane: state rows tile_row(i) .. + 3 of column v0 + lane % 16, kept transposed in LDS.
+template <int DKP>
+struct StateTiles {
+    static constexpr int n = DKP / 64;
+    f32x4 s[n];
+    __device__ __forceinline__ static int row(int i) {
+        return ((threadIdx.x >> 6) + 4 * i) * 16 + ((threadIdx.x & 63) >> 4) * 4;
+    }
+    template <typename Tile>
+    __device__ __forceinline__ void put(Tile& tile) const {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            float v4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v4[e] = s[i][e];
+            tile.put(threadIdx.x & 15, row(i), v4);
+        }
+    }
+    __device__ __forceinline__ void load(const float* state, int64_t head, int Dk, int Dv, int col) {
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                s[i][e] = state != nullptr && row(i) + e < Dk && col < Dv ? state[(head * Dk + row(i) + e) * Dv + col] : 0.f;
+    }
+    __device__ __forceinline__ void save(float* state, int64_t head, int Dk, int Dv, int col) const {
+        if (state == nullptr || col >= Dv) return;
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (row(i) + e < Dk) state[(head * Dk + row(i) + e) * Dv + col] = s[i][e];
+    }
+    __device__ __forceinline__ void keep(float* matrix, int col) const {   // matrix [cols, DKP]
+#pragma unroll
+        for (int i = 0; i < n; ++i) *reinterpret_cast<f32x4*>(matrix + static_cast<int64_t>(col) * DKP + row(i)) = s[i];
+    }
+};
+
+// a, d, beta of a chunk, one value per thread.
+struct FactorsAhead {
+    float x;
+    __device__ __forceinline__ void load(const DeltaArgs& args, int64_t at) {
+        const float* f = reinterpret_cast<const float*>(reinterpret_cast<const char*>(args.decay + at) + offsetof(Decay, a));
+        x = threadIdx.x < 3 * kChunk ? f[threadIdx.x] : 0.f;   // a, d and beta follow each other
+    }
+    __device__ __forceinline__ void store(float (&f)[3 * kChunk]) const {
+        if (threadIdx.x < 3 * kChunk) f[threadIdx.x] = x;
+    }
+};
+static_assert(offsetof(Decay, d) == offsetof(Decay, a) + 4 * kChunk && offsetof(Decay, beta) == offsetof(Decay, d) + 4 * kChunk,
+              "a, d and beta are read as one array");
+
+// Four rows of one column of a strided input, in the layout of a product.
+template <typename E>
+__device__ __forceinline__ void load_column(const DeltaTensor& x, const DeltaWhere& w, int head, int row, int col,
+                                            int valid, E (&out)[4]) {
+    const E* p = row_of<E>(x, w, head);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        out[e] = narrow<E>(0.f);
+        if (row + e < w.rows && col < valid) out[e] = p[(row + e) * x.t + col];
+    }
+}
 
 template <typename E, int DKP>
 __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(DeltaArgs args) {
     using M = Mode<E>;
-    constexpr int NV = kStateCols, TILES = DKP / 16 * (NV / 16) / 8;  // state tiles per wavefront
+    constexpr int NV = kStateCols;
     __shared__ typename M::template Input<kChunk, DKP> k;
-    __shared__ typename M::template Derived<kChunk, kChunk> inverse;
-    __shared__ typename M::template Derived<NV, DKP> state;     // transposed
-    __shared__ typename M::template Derived<NV, kChunk> x, r;   // transposed
-    __shared__ Decay y;
-    const int head = blockIdx.y, v0 = blockIdx.x * NV;
+    __shared__ typename M::template Fine<kChunk, kChunk> inverse;
+    __shared__ typename M::template Fine<NV, DKP> state;     // transposed
+    __shared__ typename M::template Fine<NV, kChunk> x, r;   // transposed
+    __shared__ float factors[3 * kChunk];
+    const float *fa = factors, *fd = factors + kChunk, *fb = factors + 2 * kChunk;
+    const int tiles = args.cols / NV;
+    const int piece = piece_in_l2(args.B * args.Hv * tiles), head = piece / tiles, v0 = (piece - head * tiles) * NV;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lr = (lane >> 4) * 4, lc = lane & 15;
-    const DeltaWhere first = delta_where(args, head, 0);
-    const int chunks = (delta_length(args, first.b) + kChunk - 1) / kChunk;
+    const int lc = lane & 15, row = wave * 16 + (lane >> 4) * 4, col = v0 + lc;
+    DeltaWhere w = delta_where(args, head, 0);
+    const int chunks = (delta_length(args, w.b) + kChunk - 1) / kChunk;
 
-    f32x4 s[TILES];
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-        const int tile = wave + 8 * i, row = tile / 2 * 16 + lr, col = v0 + tile % 2 * 16 + lc;
-        float v4[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v4[e] = 0.f;
-            if (args.state != nullptr && row + e < args.Dk && col < args.Dv)
-                v4[e] = args.state[(static_cast<int64_t>(head) * args.Dk + row + e) * args.Dv + col];
-            s[i][e] = v4[e];
-        }
-        state.put(tile % 2 * 16 + lc, row, v4);
-    }
-    const int rt = wave / 2 * 16, ct = wave % 2 * 16;   // this wavefront's tile of the chunk's rows
+    Ahead<E, kChunk, DKP, kStateThreads> k_next;
+    SquareAhead<E, kStateThreads> inverse_next;
+    FactorsAhead factors_next;
+    E v_next[4], v[4];
+    const auto request = [&](const DeltaWhere& n) {
+        k_next.load(row_of<E>(args.k, n, n.hk), args.k.t, n.rows, args.Dk, args.k.wide != 0);
+        inverse_next.load(args.inverse + n.at * M::square_bytes);
+        factors_next.load(args, n.at);
+        load_column<E>(args.v, n, n.hv, row, col, args.Dv, v_next);
+    };
+    if (chunks > 0) request(w);
+    StateTiles<DKP> s;
+    s.load(args.state, head, args.Dk, args.Dv, col);
+    s.put(state);
     for (int chunk = 0; chunk < chunks; ++chunk) {
-        const DeltaWhere w = delta_where(args, head, chunk);
-        const int64_t at = static_cast<int64_t>(head) * args.chunks + chunk;
+        k_next.store(k);
+        inverse_next.store(inverse);
+        factors_next.store(factors);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = v_next[e];
+        const int64_t at = w.at;
         __syncthreads();
-        stage<kChunk, DKP, kStateThreads>(k, row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
-        stage<kChunk, kChunk, kStateThreads>(inverse, const_cast<const float*>(args.inverse) + at * (kChunk * kChunk),
-                                             kChunk, kChunk, kChunk, true);
-        decay_of(args, w, y);
-        const int col = v0 + ct + lc;
-        float v[4];
-        const E* pv = row_of<E>(args.v, w, w.hv);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[e] = rt + lr + e < w.rows && col < args.Dv ? widen(pv[(rt + lr + e) * args.v.t + col]) : 0.f;
-        float* ps = args.states + at * DKP * args.cols + v0;
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int tile = wave + 8 * i;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ps[(tile / 2 * 16 + lr + e) * static_cast<int64_t>(args.cols) + tile % 2 * 16 + lc] = s[i][e];
+        if (chunk + 1 < chunks) {
+            w = delta_where(args, head, chunk + 1);
+            request(w);
         }
-        __syncthreads();
+        s.keep(args.states + at * DKP * args.cols, col);
         f32x4 acc = zero4();
 #pragma unroll
-        for (int c = 0; c < DKP; c += 32) acc = mma(k.rows(rt, c), state.rows(ct, c), acc);
+        for (int c = 0; c < DKP; c += 32) acc = mma(k.rows(wave * 16, c), state.rows(0, c), acc);
         float out[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = y.beta[rt + lr + e] * (v[e] - y.a[rt + lr + e] * acc[e]);
-        x.put(ct + lc, rt + lr, out);
+        for (int e = 0; e < 4; ++e) out[e] = fb[row + e] * (widen(v[e]) - fa[row + e] * acc[e]);
+        x.put(lc, row, out);
         __syncthreads();
         acc = zero4();
-        for (int c = 0; c < rt + 16; c += 32) acc = mma(inverse.rows(rt, c), x.rows(ct, c), acc);
-        float* pr = args.added + at * kChunk * args.cols + v0;
+        for (int c = 0; c < wave * 16 + 16; c += 32) acc = mma(inverse.rows(wave * 16, c), x.rows(0, c), acc);
+        *reinterpret_cast<f32x4*>(args.added + (at * args.cols + col) * kChunk + row) = acc;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            pr[(rt + lr + e) * static_cast<int64_t>(args.cols) + ct + lc] = acc[e];
-            out[e] = y.d[rt + lr + e] * acc[e];
-        }
-        r.put(ct + lc, rt + lr, out);
+        for (int e = 0; e < 4; ++e) out[e] = fd[row + e] * acc[e];
+        r.put(lc, row, out);
         __syncthreads();
+        const float last = fa[kChunk - 1];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int tile = wave + 8 * i;
+        for (int i = 0; i < s.n; ++i) {
             f32x4 next;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) next[e] = y.a_last * s[i][e];
+            for (int e = 0; e < 4; ++e) next[e] = last * s.s[i][e];
 #pragma unroll
-            for (int c = 0; c < kChunk; c += 32) next = mma(k.cols(tile / 2 * 16, c), r.rows(tile % 2 * 16, c), next);
-            s[i] = next;
-            float v4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v4[e] = next[e];
-            state.put(tile % 2 * 16 + lc, tile / 2 * 16 + lr, v4);
+            for (int c = 0; c < kChunk; c += 32) next = mma(k.cols((wave + 4 * i) * 16, c), r.rows(0, c), next);
+            s.s[i] = next;
         }
+        s.put(state);
+        __syncthreads();
     }
-    if (args.state_out != nullptr) {
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int tile = wave + 8 * i, row = tile / 2 * 16 + lr, col = v0 + tile % 2 * 16 + lc;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (row + e < args.Dk && col < args.Dv)
-                    args.state_out[(static_cast<int64_t>(head) * args.Dk + row + e) * args.Dv + col] = s[i][e];
-        }
-    }
+    s.save(args.state_out, head, args.Dk, args.Dv, col);
 }
 
 // ---- the output ---------------------------------------------------------------------------------
+//
+// The kernels over all chunks have eight wavefronts: wavefront w works on rows 16 (w % 4) .. of the chunk and on half
+// (w / 4) of the columns.
 
-// P of a chunk from staged Q and K, by four wavefronts; blocks above the diagonal are zero.
+constexpr int kPieceThreads = 512;
+
+// P of a chunk from staged Q and K; blocks above the diagonal are zero.
 template <int DKP, typename TQ, typename TK, typename TP>
 __device__ __forceinline__ void scores_of(const TQ& q, const TK& k, const Decay& y, float scale, TP& p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, band = threadIdx.x >> 6 & 3, half = threadIdx.x >> 8;
 #pragma unroll
-    for (int block = 0; block < 4; ++block) {
+    for (int b = 0; b < 2; ++b) {
+        const int block = b * 2 + half;   // both halves get one block of every pair
         f32x4 acc = zero4();
-        if (block <= wave) {
+        if (block <= band) {
 #pragma unroll
-            for (int s = 0; s < DKP; s += 32) acc = mma(q.rows(wave * 16, s), k.rows(block * 16, s), acc);
+            for (int s = 0; s < DKP; s += 32) acc = mma(q.rows(band * 16, s), k.rows(block * 16, s), acc);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = wave * 16 + (lane >> 4) * 4 + e, j = block * 16 + (lane & 15);
+            const int i = band * 16 + (lane >> 4) * 4 + e, j = block * 16 + (lane & 15);
             p.put(i, j, i >= j ? scale * acc[e] * gap(y, i, j) : 0.f);
         }
     }
 }
 
 template <typename E, int DKP>
-__global__ void __launch_bounds__(256) delta_output_kernel(DeltaArgs args) {
+__global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs args) {
     using M = Mode<E>;
-    constexpr int NV = kStateCols;
-    __shared__ typename M::template Input<kChunk, DKP> q;
-    __shared__ typename M::template Derived<kChunk, kChunk> p;
-    __shared__ Decay y;
+    constexpr int NV = kCols;
     struct Columns {
-        typename M::template Derived<DKP, NV> state;
-        typename M::template Derived<kChunk, NV> r;
+        typename M::template Coarse<NV, DKP> state;
+        typename M::template Coarse<NV, kChunk> r;
     };
     union Later {   // K is done with before the columns come
         typename M::template Input<kChunk, DKP> k;
         Columns c;
         __device__ Later() {}
     };
+    __shared__ typename M::template Input<kChunk, DKP> q;
+    __shared__ typename M::template Coarse<kChunk, kChunk> p;
+    __shared__ Decay y;
     __shared__ Later u;
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lr = wave * 16 + (lane >> 4) * 4, lc = lane & 15;
+    const int lane = threadIdx.x & 63, band = threadIdx.x >> 6 & 3, half = threadIdx.x >> 8;
+    const int lr = band * 16 + (lane >> 4) * 4, lc = lane & 15;
     E* out = static_cast<E*>(args.o) + (static_cast<int64_t>(w.t0) * args.B * args.Hv + w.head) * args.Dv;
     const int64_t out_stride = static_cast<int64_t>(args.B) * args.Hv * args.Dv;
     const int present = args.T - w.t0 < kChunk ? args.T - w.t0 : kChunk;
     if (w.rows == 0) {
-        for (int i = threadIdx.x; i < present * args.Dv; i += 256) out[i / args.Dv * out_stride + i % args.Dv] = narrow<E>(0.f);
+        for (int i = threadIdx.x; i < present * args.Dv; i += kPieceThreads)
+            out[i / args.Dv * out_stride + i % args.Dv] = narrow<E>(0.f);
         return;
     }
-    stage<kChunk, DKP, 256>(q, row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-    stage<kChunk, DKP, 256>(u.k, row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
-    decay_of(args, w, y);
+    Ahead<float, NV, DKP, kPieceThreads> state_next;
+    Ahead<float, NV, kChunk, kPieceThreads> r_next;
+    const auto request = [&](int v0) {
+        state_next.load(args.states + (w.at * args.cols + v0) * DKP, DKP, NV, DKP, true);
+        r_next.load(args.added + (w.at * args.cols + v0) * kChunk, kChunk, NV, kChunk, true);
+    };
+    {
+        Ahead<E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+        load_decay(args, w, y);
+        request(0);
+        q_next.store(q);
+        k_next.store(u.k);
+    }
     __syncthreads();
     scores_of<DKP>(q, u.k, y, args.scale, p);
-    const int64_t at = static_cast<int64_t>(w.head) * args.chunks + w.chunk;
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
-        stage<DKP, NV, 256>(u.c.state, const_cast<const float*>(args.states) + at * DKP * args.cols + v0, args.cols, DKP, NV, true);
-        stage<kChunk, NV, 256>(u.c.r, const_cast<const float*>(args.added) + at * kChunk * args.cols + v0, args.cols, kChunk, NV, true);
+        state_next.store_values(u.c.state);
+        r_next.store_values(u.c.r);
         __syncthreads();
-        f32x4 acc[2] = {zero4(), zero4()};
+        if (v0 + NV < args.cols) request(v0 + NV);
+        f32x4 acc = zero4();
 #pragma unroll
-        for (int s = 0; s < DKP; s += 32) {
-            const auto f = q.rows(wave * 16, s);
+        for (int s = 0; s < DKP; s += 32) acc = mma(q.rows(band * 16, s), u.c.state.rows(half * 16, s), acc);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) acc[c] = mma(f, u.c.state.cols(c * 16, s), acc[c]);
-        }
+        for (int e = 0; e < 4; ++e) acc[e] *= args.scale * y.a[lr + e];
+        for (int s = 0; s < band * 16 + 16; s += 32) acc = mma(p.rows(band * 16, s), u.c.r.rows(half * 16, s), acc);
+        const int col = v0 + half * 16 + lc;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c][e] *= args.scale * y.a[lr + e];
-        for (int s = 0; s < wave * 16 + 16; s += 32) {
-            const auto f = p.rows(wave * 16, s);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) acc[c] = mma(f, u.c.r.cols(c * 16, s), acc[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = v0 + c * 16 + lc;
-                if (lr + e < present && col < args.Dv)
-                    out[(lr + e) * out_stride + col] = narrow<E>(lr + e < w.rows ? acc[c][e] : 0.f);
-            }
+        for (int e = 0; e < 4; ++e)
+            if (lr + e < present && col < args.Dv)
+                out[(lr + e) * out_stride + col] = narrow<E>(lr + e < w.rows ? acc[e] : 0.f);
     }
 }
 
 // ---- backward: P^T dO ---------------------------------------------------------------------------
 
 template <typename E, int DKP>
-__global__ void __launch_bounds__(256) delta_inner_grad_kernel(DeltaArgs args) {
+__global__ void __launch_bounds__(kPieceThreads) delta_inner_grad_kernel(DeltaArgs args) {
     using M = Mode<E>;
-    constexpr int NV = kStateCols;
-    __shared__ typename M::template Input<kChunk, DKP> q, k;
-    __shared__ typename M::template Derived<kChunk, kChunk> p;
-    __shared__ typename M::template Input<kChunk, NV> go;
+    constexpr int NV = kCols;
+    struct Scores {
+        typename M::template Input<kChunk, DKP> q, k;
+    };
+    union Later {   // Q and K are done with before dO comes
+        Scores s;
+        typename M::template Input<kChunk, NV> go;
+        __device__ Later() {}
+    };
+    __shared__ Later u;
+    __shared__ typename M::template Fine<kChunk, kChunk> p;
     __shared__ Decay y;
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
     if (w.rows == 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lr = wave * 16 + (lane >> 4) * 4, lc = lane & 15;
-    stage<kChunk, DKP, 256>(q, row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-    stage<kChunk, DKP, 256>(k, row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
-    decay_of(args, w, y);
-    __syncthreads();
-    scores_of<DKP>(q, k, y, args.scale, p);
-    const int64_t at = static_cast<int64_t>(w.head) * args.chunks + w.chunk;
+    const int lane = threadIdx.x & 63, band = threadIdx.x >> 6 & 3, half = threadIdx.x >> 8;
+    const int lr = band * 16 + (lane >> 4) * 4, lc = lane & 15;
+    Ahead<E, kChunk, NV, kPieceThreads> go_next;
     const E* pg = row_of<E>(args.grad_o, w, w.hv);
+    const auto request = [&](int v0) {
+        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0, args.grad_o.wide != 0);
+    };
+    {
+        Ahead<E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+        load_decay(args, w, y);
+        request(0);
+        q_next.store(u.s.q);
+        k_next.store(u.s.k);
+    }
+    __syncthreads();
+    scores_of<DKP>(u.s.q, u.s.k, y, args.scale, p);
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
-        stage<kChunk, NV, 256>(go, pg + v0, args.grad_o.t, w.rows, args.Dv - v0, args.grad_o.wide != 0);
+        go_next.store(u.go);
         __syncthreads();
-        f32x4 acc[2] = {zero4(), zero4()};
-        for (int s = wave * 16 / 32 * 32; s < kChunk; s += 32) {
-            const auto f = p.cols(wave * 16, s);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) acc[c] = mma(f, go.cols(c * 16, s), acc[c]);
-        }
-        float* out = args.inner + at * kChunk * args.cols + v0;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) out[static_cast<int64_t>(lr + e) * args.cols + c * 16 + lc] = acc[c][e];
+        if (v0 + NV < args.cols) request(v0 + NV);
+        f32x4 acc = zero4();
+        for (int s = band * 16 / 32 * 32; s < kChunk; s += 32) acc = mma(p.cols(band * 16, s), u.go.cols(half * 16, s), acc);
+        *reinterpret_cast<f32x4*>(args.inner + (w.at * args.cols + v0 + half * 16 + lc) * kChunk + lr) = acc;
     }
 }
 
@@ -661,110 +848,92 @@ __global__ void __launch_bounds__(256) delta_inner_grad_kernel(DeltaArgs args) {
 template <typename E, int DKP>
 __global__ void __launch_bounds__(kStateThreads) delta_state_grad_kernel(DeltaArgs args) {
     using M = Mode<E>;
-    constexpr int NV = kStateCols, TILES = DKP / 16 * (NV / 16) / 8;
+    constexpr int NV = kStateCols;
     __shared__ typename M::template Input<kChunk, DKP> q, k;
-    __shared__ typename M::template Derived<kChunk, kChunk> inverse;
-    __shared__ typename M::template Derived<NV, DKP> state;       // gradient of the state, transposed
-    __shared__ typename M::template Derived<NV, kChunk> r, x, go; // dR, beta a dX, scale a dO, transposed
-    __shared__ Decay y;
-    const int head = blockIdx.y, v0 = blockIdx.x * NV;
+    __shared__ typename M::template Fine<kChunk, kChunk> inverse;
+    __shared__ typename M::template Fine<NV, DKP> state;       // gradient of the state, transposed
+    __shared__ typename M::template Fine<NV, kChunk> r, x, go; // dR, -beta a dX, scale a dO, transposed
+    __shared__ float factors[3 * kChunk];
+    const float *fa = factors, *fd = factors + kChunk, *fb = factors + 2 * kChunk;
+    const int tiles = args.cols / NV;
+    const int piece = piece_in_l2(args.B * args.Hv * tiles), head = piece / tiles, v0 = (piece - head * tiles) * NV;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lr = (lane >> 4) * 4, lc = lane & 15;
-    const DeltaWhere first = delta_where(args, head, 0);
-    const int chunks = (delta_length(args, first.b) + kChunk - 1) / kChunk;
+    const int lc = lane & 15, row = wave * 16 + (lane >> 4) * 4, col = v0 + lc;
+    DeltaWhere w = delta_where(args, head, 0);
+    const int chunks = (delta_length(args, w.b) + kChunk - 1) / kChunk;
 
-    f32x4 s[TILES];
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-        const int tile = wave + 8 * i, row = tile / 2 * 16 + lr, col = v0 + tile % 2 * 16 + lc;
-        float v4[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v4[e] = 0.f;
-            if (args.grad_state != nullptr && row + e < args.Dk && col < args.Dv)
-                v4[e] = args.grad_state[(static_cast<int64_t>(head) * args.Dk + row + e) * args.Dv + col];
-            s[i][e] = v4[e];
-        }
-        state.put(tile % 2 * 16 + lc, row, v4);
+    Ahead<E, kChunk, DKP, kStateThreads> q_next, k_next;
+    SquareAhead<E, kStateThreads> inverse_next;
+    FactorsAhead factors_next;
+    E g_next[4], g[4];
+    f32x4 inner_next, inner;
+    const auto request = [&](const DeltaWhere& n) {
+        q_next.load(row_of<E>(args.q, n, n.hk), args.q.t, n.rows, args.Dk, args.q.wide != 0);
+        k_next.load(row_of<E>(args.k, n, n.hk), args.k.t, n.rows, args.Dk, args.k.wide != 0);
+        inverse_next.load(args.inverse + n.at * M::square_bytes);
+        factors_next.load(args, n.at);
+        load_column<E>(args.grad_o, n, n.hv, row, col, args.Dv, g_next);
+        inner_next = *reinterpret_cast<const f32x4*>(args.inner + (n.at * args.cols + col) * kChunk + row);
+    };
+    if (chunks > 0) {
+        w = delta_where(args, head, chunks - 1);
+        request(w);
     }
-    const int rt = wave / 2 * 16, ct = wave % 2 * 16;
+    StateTiles<DKP> s;
+    s.load(args.grad_state, head, args.Dk, args.Dv, col);
+    s.put(state);
     for (int chunk = chunks - 1; chunk >= 0; --chunk) {
-        const DeltaWhere w = delta_where(args, head, chunk);
-        const int64_t at = static_cast<int64_t>(head) * args.chunks + chunk;
+        q_next.store(q);
+        k_next.store(k);
+        inverse_next.store(inverse);
+        factors_next.store(factors);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = g_next[e];
+        inner = inner_next;
+        const int64_t at = w.at;
         __syncthreads();
-        stage<kChunk, DKP, kStateThreads>(q, row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-        stage<kChunk, DKP, kStateThreads>(k, row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
-        stage<kChunk, kChunk, kStateThreads>(inverse, const_cast<const float*>(args.inverse) + at * (kChunk * kChunk),
-                                             kChunk, kChunk, kChunk, true);
-        decay_of(args, w, y);
-        const int col = v0 + ct + lc;
-        float g[4], out[4];
-        const E* pg = row_of<E>(args.grad_o, w, w.hv);
-        float* px = args.inner + at * kChunk * args.cols + v0;
-        f32x4 acc;
+        if (chunk > 0) {
+            w = delta_where(args, head, chunk - 1);
+            request(w);
+        }
+        s.keep(args.state_grads + at * DKP * args.cols, col);
+        f32x4 acc = zero4();
+#pragma unroll
+        for (int c = 0; c < DKP; c += 32) acc = mma(k.rows(wave * 16, c), state.rows(0, c), acc);
+        float out[4], scaled[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            g[e] = rt + lr + e < w.rows && col < args.Dv ? widen(pg[(rt + lr + e) * args.grad_o.t + col]) : 0.f;
-            acc[e] = px[(rt + lr + e) * static_cast<int64_t>(args.cols) + ct + lc];
+            out[e] = inner[e] + fd[row + e] * acc[e];
+            scaled[e] = args.scale * fa[row + e] * widen(g[e]);
         }
-        float* ps = args.state_grads + at * DKP * args.cols + v0;
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int tile = wave + 8 * i;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ps[(tile / 2 * 16 + lr + e) * static_cast<int64_t>(args.cols) + tile % 2 * 16 + lc] = s[i][e];
-        }
-        __syncthreads();
-        f32x4 from_state = zero4();
-#pragma unroll
-        for (int c = 0; c < DKP; c += 32) from_state = mma(k.rows(rt, c), state.rows(ct, c), from_state);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = rt + lr + e;
-            out[e] = acc[e] + y.d[i] * from_state[e];
-            g[e] *= args.scale * y.a[i];
-        }
-        r.put(ct + lc, rt + lr, out);
-        go.put(ct + lc, rt + lr, g);
+        r.put(lc, row, out);
+        go.put(lc, row, scaled);
         __syncthreads();
         acc = zero4();
-        for (int c = rt / 32 * 32; c < kChunk; c += 32) acc = mma(inverse.cols(rt, c), r.rows(ct, c), acc);
+        for (int c = wave * 16 / 32 * 32; c < kChunk; c += 32) acc = mma(inverse.cols(wave * 16, c), r.rows(0, c), acc);
+        *reinterpret_cast<f32x4*>(args.inner + (at * args.cols + col) * kChunk + row) = acc;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = rt + lr + e;
-            px[i * static_cast<int64_t>(args.cols) + ct + lc] = acc[e];
-            out[e] = -y.beta[i] * y.a[i] * acc[e];
-        }
-        x.put(ct + lc, rt + lr, out);
-        __syncthreads();
+        for (int e = 0; e < 4; ++e) out[e] = -fb[row + e] * fa[row + e] * acc[e];
+        x.put(lc, row, out);
+        const float last = fa[kChunk - 1];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int tile = wave + 8 * i;
+        for (int i = 0; i < s.n; ++i) {   // what does not wait for dX
             f32x4 next;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) next[e] = y.a_last * s[i][e];
+            for (int e = 0; e < 4; ++e) next[e] = last * s.s[i][e];
 #pragma unroll
-            for (int c = 0; c < kChunk; c += 32) {
-                next = mma(q.cols(tile / 2 * 16, c), go.rows(tile % 2 * 16, c), next);
-                next = mma(k.cols(tile / 2 * 16, c), x.rows(tile % 2 * 16, c), next);
-            }
-            s[i] = next;
-            float v4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v4[e] = next[e];
-            state.put(tile % 2 * 16 + lc, tile / 2 * 16 + lr, v4);
+            for (int c = 0; c < kChunk; c += 32) next = mma(q.cols((wave + 4 * i) * 16, c), go.rows(0, c), next);
+            s.s[i] = next;
         }
-    }
-    if (args.grad_initial != nullptr) {
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            const int tile = wave + 8 * i, row = tile / 2 * 16 + lr, col = v0 + tile % 2 * 16 + lc;
+        for (int i = 0; i < s.n; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (row + e < args.Dk && col < args.Dv)
-                    args.grad_initial[(static_cast<int64_t>(head) * args.Dk + row + e) * args.Dv + col] = s[i][e];
-        }
+            for (int c = 0; c < kChunk; c += 32) s.s[i] = mma(k.cols((wave + 4 * i) * 16, c), x.rows(0, c), s.s[i]);
+        s.put(state);
+        __syncthreads();
     }
+    s.save(args.grad_initial, head, args.Dk, args.Dv, col);
 }
 
 // ---- backward: the gradients of the inputs ------------------------------------------------------
@@ -779,17 +948,17 @@ __device__ __forceinline__ float row_sum16(float v) {  // over the 16 lanes that
 
 // QO: type of grad_q and grad_k (the storage type, or float partial gradients where value heads share a key head).
 template <typename E, typename QO, int DKP>
-__global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
+__global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaArgs args) {
     using M = Mode<E>;
-    constexpr int NV = kStateCols, KT = DKP / 16;
+    constexpr int NV = kCols, KT = DKP / 32;   // tiles of 16 key columns per wavefront
     struct Columns {
-        typename M::template Derived<kChunk, NV> x, r;
+        typename M::template Fine<NV, kChunk> x, r;   // transposed, like s and ds
         typename M::template Input<kChunk, NV> go;
-        typename M::template Derived<DKP, NV> s, ds;
+        typename M::template Fine<NV, DKP> s, ds;
     };
     struct Rows {
         typename M::template Input<kChunk, DKP> q, k;
-        typename M::template Derived<kChunk, kChunk> m, n;
+        typename M::template Coarse<kChunk, kChunk> m, n;
     };
     union Shared {
         Columns c;
@@ -798,10 +967,11 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
     };
     __shared__ Shared u;
     __shared__ Decay y;
-    __shared__ float row_beta[kChunk], row_c[kChunk], row_e[kChunk], col_c[4][kChunk], dot_v[kChunk], inner[4];
+    // sums of a row from both halves of the workgroup, of a column from every band
+    __shared__ float row_beta[2][kChunk], row_c[2][kChunk], row_e[2][kChunk], col_c[4][kChunk], dot_v[kChunk], inner[8];
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lr = wave * 16 + (lane >> 4) * 4, lc = lane & 15;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, band = wave & 3, half = wave >> 2;
+    const int lr = band * 16 + (lane >> 4) * 4, lc = lane & 15;
     const int present = args.T - w.t0 < kChunk ? args.T - w.t0 : kChunk;
     // rows of the dense outputs: (t, b, head) of Hv heads; grad_q / grad_k per value head or, unshared, per key head
     const int64_t row0 = static_cast<int64_t>(w.t0) * args.B * args.Hv + w.head, row_step = static_cast<int64_t>(args.B) * args.Hv;
@@ -809,101 +979,119 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
     QO* gq = static_cast<QO*>(args.grad_q) + row0 * args.Dk;
     QO* gk = static_cast<QO*>(args.grad_k) + row0 * args.Dk;
     if (w.rows == 0) {
-        for (int i = threadIdx.x; i < present * args.Dv; i += 256)
+        for (int i = threadIdx.x; i < present * args.Dv; i += kPieceThreads)
             gv[i / args.Dv * row_step * args.Dv + i % args.Dv] = narrow<E>(0.f);
-        for (int i = threadIdx.x; i < present * args.Dk; i += 256) {
+        for (int i = threadIdx.x; i < present * args.Dk; i += kPieceThreads) {
             gq[i / args.Dk * row_step * args.Dk + i % args.Dk] = narrow<QO>(0.f);
             gk[i / args.Dk * row_step * args.Dk + i % args.Dk] = narrow<QO>(0.f);
         }
-        for (int i = threadIdx.x; i < present; i += 256) {
+        for (int i = threadIdx.x; i < present; i += kPieceThreads) {
             args.grad_g[row0 + i * row_step] = 0.f;
             args.grad_beta[row0 + i * row_step] = 0.f;
         }
         return;
     }
-    decay_of(args, w, y);
-    const int64_t at = static_cast<int64_t>(w.head) * args.chunks + w.chunk;
     const E* pv = row_of<E>(args.v, w, w.hv);
     const E* pg = row_of<E>(args.grad_o, w, w.hv);
+    Ahead<float, NV, kChunk, kPieceThreads> x_next, r_next;
+    Ahead<float, NV, DKP, kPieceThreads> s_next, ds_next;
+    Ahead<E, kChunk, NV, kPieceThreads> go_next;
+    const auto request = [&](int v0) {
+        x_next.load(args.inner + (w.at * args.cols + v0) * kChunk, kChunk, NV, kChunk, true);
+        r_next.load(args.added + (w.at * args.cols + v0) * kChunk, kChunk, NV, kChunk, true);
+        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0, args.grad_o.wide != 0);
+        s_next.load(args.states + (w.at * args.cols + v0) * DKP, DKP, NV, DKP, true);
+        ds_next.load(args.state_grads + (w.at * args.cols + v0) * DKP, DKP, NV, DKP, true);
+    };
+    load_decay(args, w, y);
+    request(0);
 
-    f32x4 y1[KT], y2[KT], y3[KT], da[4], dp[4];
+    f32x4 y1[KT], y2[KT], y3[KT], da[2], dp[2];
 #pragma unroll
     for (int i = 0; i < KT; ++i) y1[i] = y2[i] = y3[i] = zero4();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) da[i] = dp[i] = zero4();
+    for (int i = 0; i < 2; ++i) da[i] = dp[i] = zero4();
     float v_dot = 0.f, s_dot = 0.f;
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
-        {   // dX: 64 rows of 4 times 8 columns, one each; with it dV and v . dX
-            const int i = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
-            float x[8], v[8];
-            load8<float>(args.inner + (at * kChunk + i) * args.cols, v0 + c, args.cols, true, x);
-            u.c.x.put(i, c, x);
-            load8<E>(pv + (i < w.rows ? i : 0) * args.v.t, v0 + c, i < w.rows ? args.Dv : 0, args.v.wide != 0, v);
+        x_next.store_values(u.c.x);
+        r_next.store_values(u.c.r);
+        go_next.store(u.c.go);
+        s_next.store_values(u.c.s);
+        ds_next.store_values(u.c.ds);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v_dot += v[j] * x[j];
-            if (i < present) {
-                const float beta = i < w.rows ? y.beta[i] : 0.f;
+        for (int i = 0; i < s_next.n; ++i) {
+            float a[8], b[8];
+            values_of(s_next.x[i], a);
+            values_of(ds_next.x[i], b);
+            if ((s_next.total % kPieceThreads == 0) || i * kPieceThreads + static_cast<int>(threadIdx.x) < s_next.total) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (v0 + c + j < args.Dv) gv[i * row_step * args.Dv + v0 + c + j] = narrow<E>(i < w.rows ? beta * x[j] : 0.f);
+                for (int j = 0; j < 8; ++j) s_dot += a[j] * b[j];
             }
-        }
-        stage<kChunk, NV, 256>(u.c.r, const_cast<const float*>(args.added) + at * kChunk * args.cols + v0, args.cols, kChunk, NV, true);
-        stage<kChunk, NV, 256>(u.c.go, pg + v0, args.grad_o.t, w.rows, args.Dv - v0, args.grad_o.wide != 0);
-#pragma unroll
-        for (int i = 0; i < DKP * NV / 8; i += 256) {
-            const int seg = i + threadIdx.x, row = seg / (NV / 8), c = seg % (NV / 8) * 8;
-            float s[8], ds[8];
-            load8<float>(args.states + (at * DKP + row) * args.cols, v0 + c, args.cols, true, s);
-            load8<float>(args.state_grads + (at * DKP + row) * args.cols, v0 + c, args.cols, true, ds);
-            u.c.s.put(row, c, s);
-            u.c.ds.put(row, c, ds);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s_dot += s[j] * ds[j];
         }
         __syncthreads();
-        const auto fx = u.c.x.rows(wave * 16, 0);
-        const auto fg = u.c.go.rows(wave * 16, 0);
-        const auto fr = u.c.r.rows(wave * 16, 0);
+        if (v0 + NV < args.cols) request(v0 + NV);
+        {   // dV and v . dX: eight threads with four columns each share a row
+            const int i = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+            if (i < present) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = v0 + c + j;
+                    if (at >= args.Dv) continue;
+                    const float dx = u.c.x.get(c + j, i);
+                    if (i < w.rows) v_dot += widen(pv[i * args.v.t + at]) * dx;
+                    gv[i * row_step * args.Dv + at] = narrow<E>(i < w.rows ? y.beta[i] * dx : 0.f);
+                }
+            }
+        }
+        const auto fx = u.c.x.cols(band * 16, 0);
+        const auto fg = u.c.go.rows(band * 16, 0);
+        const auto fr = u.c.r.cols(band * 16, 0);
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
-            const auto fs = u.c.s.rows(i * 16, 0);
+            const auto fs = u.c.s.cols((half * KT + i) * 16, 0);
             y1[i] = mma(fx, fs, y1[i]);
             y2[i] = mma(fg, fs, y2[i]);
-            y3[i] = mma(fr, u.c.ds.rows(i * 16, 0), y3[i]);
+            y3[i] = mma(fr, u.c.ds.cols((half * KT + i) * 16, 0), y3[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i <= wave) {
-                const auto f = u.c.r.rows(i * 16, 0);
-                da[i] = mma(fx, f, da[i]);
-                dp[i] = mma(fg, f, dp[i]);
+        for (int b = 0; b < 2; ++b)
+            if (b * 2 + half <= band) {
+                const auto f = u.c.r.cols((b * 2 + half) * 16, 0);
+                da[b] = mma(fx, f, da[b]);
+                dp[b] = mma(fg, f, dp[b]);
             }
     }
-    // v . dX: four threads share a row;  <S, dS'>: the whole workgroup
+    // v . dX over the eight threads of a row;  <S, dS'> over the workgroup
     v_dot += __shfl_xor(v_dot, 1);
     v_dot += __shfl_xor(v_dot, 2);
+    v_dot += __shfl_xor(v_dot, 4);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s_dot += __shfl_xor(s_dot, d);
-    __syncthreads();
-    if ((threadIdx.x & 3) == 0) dot_v[threadIdx.x >> 2] = v_dot;
-    if (lane == 0) inner[wave] = s_dot;
-    stage<kChunk, DKP, 256>(u.w.q, row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-    stage<kChunk, DKP, 256>(u.w.k, row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+    {
+        Ahead<E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+        __syncthreads();
+        if ((threadIdx.x & 7) == 0) dot_v[threadIdx.x >> 3] = v_dot;
+        if (lane == 0) inner[wave] = s_dot;
+        q_next.store(u.w.q);
+        k_next.store(u.w.k);
+    }
     __syncthreads();
 
     // M, N and the sums over their products with A and P
     float sum_beta[4] = {}, sum_c[4] = {};
 #pragma unroll
-    for (int block = 0; block < 4; ++block) {
+    for (int b = 0; b < 2; ++b) {
+        const int block = b * 2 + half;
         f32x4 kk = zero4(), qk = zero4();
-        if (block <= wave) {
+        if (block <= band) {
 #pragma unroll
             for (int s = 0; s < DKP; s += 32) {
                 const auto f = u.w.k.rows(block * 16, s);
-                kk = mma(u.w.k.rows(wave * 16, s), f, kk);
-                qk = mma(u.w.q.rows(wave * 16, s), f, qk);
+                kk = mma(u.w.k.rows(band * 16, s), f, kk);
+                qk = mma(u.w.q.rows(band * 16, s), f, qk);
             }
         }
         float col = 0.f;
@@ -911,8 +1099,8 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
         for (int e = 0; e < 4; ++e) {
             const int i = lr + e, j = block * 16 + lc;
             const float decay = i >= j ? gap(y, i, j) : 0.f;
-            const float a_grad = i > j ? -da[block][e] * decay : 0.f;
-            const float p_grad = i >= j ? dp[block][e] * decay * args.scale : 0.f;
+            const float a_grad = i > j ? -da[b][e] * decay : 0.f;
+            const float p_grad = i >= j ? dp[b][e] * decay * args.scale : 0.f;
             const float m = a_grad * y.beta[i];
             const float both = m * kk[e] + p_grad * qk[e];
             sum_beta[e] += a_grad * kk[e];
@@ -923,7 +1111,7 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
         }
         col += __shfl_xor(col, 16);
         col += __shfl_xor(col, 32);
-        if (lane < 16) col_c[wave][block * 16 + lc] = col;
+        if (lane < 16) col_c[band][block * 16 + lc] = col;
     }
     // k . Y1, q . Y2, k . Y3 by row
 #pragma unroll
@@ -931,7 +1119,8 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
         float d1 = 0.f, d2 = 0.f, d3 = 0.f;
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
-            const float kv = u.w.k.get(lr + e, i * 16 + lc), qv = u.w.q.get(lr + e, i * 16 + lc);
+            const int c = (half * KT + i) * 16 + lc;
+            const float kv = u.w.k.get(lr + e, c), qv = u.w.q.get(lr + e, c);
             d1 += kv * y1[i][e];
             d2 += qv * y2[i][e];
             d3 += kv * y3[i][e];
@@ -941,23 +1130,27 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
         const float e_row = y.d[lr + e] * row_sum16(d3);
         const float b_row = row_sum16(sum_beta[e] - a * d1);
         if (lc == 0) {
-            row_c[lr + e] = rest - e_row;
-            row_e[lr + e] = e_row;
-            row_beta[lr + e] = b_row;
+            row_c[half][lr + e] = rest - e_row;
+            row_e[half][lr + e] = e_row;
+            row_beta[half][lr + e] = b_row;
         }
     }
     __syncthreads();
     if (wave == 0) {
         const int i = lane;
         const bool here = i < w.rows;
-        double e_sum = here ? row_e[i] : 0.0;
-        double dc = row_c[i];
+        double e_sum = here ? static_cast<double>(row_e[0][i]) + row_e[1][i] : 0.0;
+        double dc = static_cast<double>(row_c[0][i]) + row_c[1][i];
 #pragma unroll
         for (int o = 0; o < 4; ++o) dc -= col_c[o][i];
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) e_sum += __shfl_xor(e_sum, d);
-        if (i == 63)
-            dc += e_sum + static_cast<double>(y.a_last) * (static_cast<double>(inner[0]) + inner[1] + inner[2] + inner[3]);
+        if (i == 63) {
+            double dot = 0.0;
+#pragma unroll
+            for (int o = 0; o < 8; ++o) dot += inner[o];
+            dc += e_sum + static_cast<double>(y.a[kChunk - 1]) * dot;
+        }
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {   // sums from the row to the end
             const double other = __shfl_down(dc, d);
@@ -965,11 +1158,12 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
         }
         if (i < present) {
             args.grad_g[row0 + i * row_step] = here ? static_cast<float>(dc) : 0.f;
-            args.grad_beta[row0 + i * row_step] = here ? row_beta[i] + dot_v[i] : 0.f;
+            args.grad_beta[row0 + i * row_step] = here ? row_beta[0][i] + row_beta[1][i] + dot_v[i] : 0.f;
         }
     }
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
+        const int c0 = (half * KT + i) * 16;
         f32x4 q, k;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -979,19 +1173,19 @@ __global__ void __launch_bounds__(256) delta_input_grad_kernel(DeltaArgs args) {
         }
 #pragma unroll
         for (int s = 0; s < kChunk; s += 32) {
-            const auto fk = u.w.k.cols(i * 16, s);
-            if (s <= wave * 16) {   // rows of this wavefront against columns up to the diagonal
-                q = mma(u.w.n.rows(wave * 16, s), fk, q);
-                k = mma(u.w.m.rows(wave * 16, s), fk, k);
+            const auto fk = u.w.k.cols(c0, s);
+            if (s <= band * 16) {   // rows of this wavefront against columns up to the diagonal
+                q = mma(u.w.n.rows(band * 16, s), fk, q);
+                k = mma(u.w.m.rows(band * 16, s), fk, k);
             }
-            if (s + 32 > wave * 16) {
-                k = mma(u.w.m.cols(wave * 16, s), fk, k);
-                k = mma(u.w.n.cols(wave * 16, s), u.w.q.cols(i * 16, s), k);
+            if (s + 32 > band * 16) {
+                k = mma(u.w.m.cols(band * 16, s), fk, k);
+                k = mma(u.w.n.cols(band * 16, s), u.w.q.cols(c0, s), k);
             }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int col = i * 16 + lc;
+            const int col = c0 + lc;
             if (lr + e < present && col < args.Dk) {
                 const bool here = lr + e < w.rows;
                 gq[(lr + e) * row_step * args.Dk + col] = narrow<QO>(here ? q[e] : 0.f);
@@ -1028,11 +1222,11 @@ hipError_t delta_backward_bf16(const DeltaArgs& a, void* grad_q, void* grad_k, h
 template <typename E, int DKP>
 hipError_t delta_forward_as(const DeltaArgs& a, hipStream_t st) {
     const dim3 pieces(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.Hv));
-    const dim3 columns(static_cast<unsigned>(a.cols / kStateCols), static_cast<unsigned>(a.B * a.Hv));
+    const dim3 columns(static_cast<unsigned>(a.cols / kStateCols * a.B * a.Hv));
     hipError_t err = hipSuccess;
     if (a.chunks > 0) err = launch(delta_inverse_kernel<E, DKP>, pieces, dim3(256), st, a);
     if (err == hipSuccess) err = launch(delta_state_kernel<E, DKP>, columns, dim3(kStateThreads), st, a);
-    if (err == hipSuccess && a.chunks > 0) err = launch(delta_output_kernel<E, DKP>, pieces, dim3(256), st, a);
+    if (err == hipSuccess && a.chunks > 0) err = launch(delta_output_kernel<E, DKP>, pieces, dim3(kPieceThreads), st, a);
     return err;
 }
 
@@ -1040,13 +1234,13 @@ hipError_t delta_forward_as(const DeltaArgs& a, hipStream_t st) {
 template <typename E, int DKP>
 hipError_t delta_backward_as(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st) {
     const dim3 pieces(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.Hv));
-    const dim3 columns(static_cast<unsigned>(a.cols / kStateCols), static_cast<unsigned>(a.B * a.Hv));
+    const dim3 columns(static_cast<unsigned>(a.cols / kStateCols * a.B * a.Hv));
     hipError_t err = hipSuccess;
-    if (a.chunks > 0) err = launch(delta_inner_grad_kernel<E, DKP>, pieces, dim3(256), st, a);
+    if (a.chunks > 0) err = launch(delta_inner_grad_kernel<E, DKP>, pieces, dim3(kPieceThreads), st, a);
     if (err == hipSuccess) err = launch(delta_state_grad_kernel<E, DKP>, columns, dim3(kStateThreads), st, a);
     if (err != hipSuccess || a.chunks == 0) return err;
-    if (a.Hv == a.Hk) return launch(delta_input_grad_kernel<E, E, DKP>, pieces, dim3(256), st, a);
-    err = launch(delta_input_grad_kernel<E, float, DKP>, pieces, dim3(256), st, a);
+    if (a.Hv == a.Hk) return launch(delta_input_grad_kernel<E, E, DKP>, pieces, dim3(kPieceThreads), st, a);
+    err = launch(delta_input_grad_kernel<E, float, DKP>, pieces, dim3(kPieceThreads), st, a);
     if (err != hipSuccess) return err;
     const int64_t rows = static_cast<int64_t>(a.T) * a.B * a.Hk;
     const int64_t blocks = ceil_div(rows * a.Dk, 256);

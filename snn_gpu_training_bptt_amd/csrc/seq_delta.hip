@@ -174,7 +174,7 @@ DeltaTensor tensor_of(const void* p, const int64_t* strides, int64_t D, size_t e
 
 struct Sizes {
     int64_t pieces, heads, chunks, cols, dkp;
-    size_t inverse, added, states;               // bytes of the forward's matrices
+    size_t decay, inverse, added, states;        // bytes of what the forward leaves behind
     size_t inner, state_grads, partial;          // of the backward's
 };
 
@@ -183,10 +183,12 @@ Sizes sizes_of(const snnseq_delta* c) {
     s.chunks = ceil_div(c->T, kChunk);
     s.heads = c->B * c->Hv;
     s.pieces = s.chunks * s.heads;
-    s.cols = ceil_div(c->Dv, kStateCols) * kStateCols;
+    s.cols = ceil_div(c->Dv, kCols) * kCols;
     s.dkp = c->Dk <= 64 ? 64 : 128;
     const size_t n = static_cast<size_t>(s.pieces) * sizeof(float);
-    s.inverse = n * kChunk * kChunk;
+    s.decay = static_cast<size_t>(s.pieces) * sizeof(Decay);
+    s.inverse = static_cast<size_t>(s.pieces) *
+                (c->dtype == SNNLIF_DTYPE_F32 ? Mode<float>::square_bytes : Mode<bf16_t>::square_bytes);
     s.added = s.inner = n * kChunk * static_cast<size_t>(s.cols);
     s.states = s.state_grads = n * static_cast<size_t>(s.dkp * s.cols);
     s.partial = c->Hv == c->Hk ? 0 : round_up(static_cast<size_t>(c->T * s.heads * c->Dk) * sizeof(float), 16);
@@ -207,9 +209,10 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved) {
     a.v = tensor_of(c->v, c->v_strides, c->Dv, es);
     a.g = c->g; a.beta = c->beta; a.state = c->state;
     char* p = static_cast<char*>(saved);
-    a.inverse = reinterpret_cast<float*>(p);
-    a.added = reinterpret_cast<float*>(p + s.inverse);
-    a.states = reinterpret_cast<float*>(p + s.inverse + s.added);
+    a.decay = reinterpret_cast<Decay*>(p);
+    a.inverse = p + s.decay;
+    a.added = reinterpret_cast<float*>(p + s.decay + s.inverse);
+    a.states = reinterpret_cast<float*>(p + s.decay + s.inverse + s.added);
     return a;
 }
 
@@ -221,7 +224,7 @@ using namespace snnseq;
 extern "C" size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call) {
     if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
     const Sizes s = sizes_of(call);
-    return s.inverse + s.added + s.states;
+    return s.decay + s.inverse + s.added + s.states;
 }
 
 extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved,
@@ -235,7 +238,7 @@ extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* s
     if (!aligned_to(o, element_size(call->dtype)) || !aligned_to(state_out, 4) || !aligned_to(saved, 16))
         return SNNLIF_ERR_ALIGN;
     const Sizes s = sizes_of(call);
-    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.inverse + s.added + s.states)) return SNNLIF_ERR_WORKSPACE;
+    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.decay + s.inverse + s.added + s.states)) return SNNLIF_ERR_WORKSPACE;
     DeltaArgs a = args_of(call, s, saved);
     a.o = o;
     a.state_out = state_out;
@@ -268,7 +271,7 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
         !aligned_to(grad_state_out, 4) || !aligned_to(saved, 16) || !aligned_to(workspace, 16))
         return SNNLIF_ERR_ALIGN;
     const Sizes s = sizes_of(call);
-    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.inverse + s.added + s.states || workspace == nullptr ||
+    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.decay + s.inverse + s.added + s.states || workspace == nullptr ||
                          workspace_bytes < s.inner + s.state_grads + 2 * s.partial))
         return SNNLIF_ERR_WORKSPACE;
     DeltaArgs a = args_of(call, s, const_cast<void*>(saved));
