@@ -33,9 +33,12 @@ EXT_LIB = os.path.join(LIB_DIR, "snnlib.so")
 
 # -ffp-contract=off: products and sums stay separately rounded (bit parity with per-op fp32).
 # -packed-fp32-ops off: keep the compiler from forming packed fp32 VALU instructions.
+# -amdgpu-mfma-vgpr-form: matrix instructions add to ordinary registers; with accumulation registers every result
+#   is moved twice, a tenth of the instructions in the gated delta rule's chains.
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    "-mllvm", "-amdgpu-mfma-vgpr-form=1",
     "-Wno-unused-command-line-argument",
 ]
 KERNEL_SOURCES = ["lif_abi.hip", "lif_f32.hip", "lif_f64.hip", "lif_bf16.hip", "lif_bn_f32.hip",

@@ -57,6 +57,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // ---- operands of the matrix instructions --------------------------------------------------------
 //
@@ -104,11 +106,12 @@ __device__ __forceinline__ void split(const float (&x)[n], uint32_t (&words)[N][
     for (int part = 0; part < N; ++part)
 #pragma unroll
         for (int j = 0; j < n; j += 2) {
-            const uint16_t lo = bits_of(rest[j]), hi = bits_of(rest[j + 1]);
-            words[part][j / 2] = lo | static_cast<uint32_t>(hi) << 16;
+            const bf16x2 pair = __builtin_convertvector(f32x2{rest[j], rest[j + 1]}, bf16x2);   // one instruction
+            const uint32_t word = __builtin_bit_cast(uint32_t, pair);
+            words[part][j / 2] = word;
             if (part + 1 < N) {
-                rest[j] -= value_of(lo);
-                rest[j + 1] -= value_of(hi);
+                rest[j] -= __builtin_bit_cast(float, word << 16);
+                rest[j + 1] -= __builtin_bit_cast(float, word & 0xffff0000u);
             }
         }
 }
@@ -217,21 +220,62 @@ struct TileF {
     }
 };
 
+// Fragments in memory: 64 lanes times 16 bytes are one run, so that a wavefront reads an operand of its products
+// straight into registers, one access of 1 KiB per part, without LDS and with one address.
+template <typename F> constexpr int frag_bytes() { return static_cast<int>(sizeof(F)) * 64; }
+
+template <typename F>
+__device__ __forceinline__ F load_frag(const char* base, int index) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(base + index * frag_bytes<F>()) + (threadIdx.x & 63);
+    struct Words { u32x4 x[sizeof(F) / 16]; } w;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(F) / 16); ++i) w.x[i] = p[i * 64];
+    return __builtin_bit_cast(F, w);
+}
+
+template <typename F>
+__device__ __forceinline__ void store_frag(char* base, int index, const F& f) {
+    u32x4* p = reinterpret_cast<u32x4*>(base + index * frag_bytes<F>()) + (threadIdx.x & 63);
+    struct Words { u32x4 x[sizeof(F) / 16]; };
+    const Words w = __builtin_bit_cast(Words, f);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(F) / 16); ++i) p[i * 64] = w.x[i];
+}
+
+// Eight fp32 values as a fragment's values.
+__device__ __forceinline__ void frag_of(const float (&x)[8], FragH<3>& f) {
+    uint32_t words[3][4];
+    split<3, 8>(x, words);
+#pragma unroll
+    for (int part = 0; part < 3; ++part)
+        f.p[part] = __builtin_bit_cast(bf16x8, u32x4{words[part][0], words[part][1], words[part][2], words[part][3]});
+}
+__device__ __forceinline__ void frag_of(const float (&x)[8], FragF& f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = x[j];
+}
+
 // What a storage type computes with: tiles of inputs, and of derived values on the way to fp32 results (Fine) or to
-// results of the storage type (Coarse).  kSquareParts: how a 64 x 64 matrix is handed from kernel to kernel.
+// results of the storage type (Coarse).
 template <typename E> struct Mode;
 template <> struct Mode<bf16_t> {
     template <int R, int C> using Input = TileH<1, R, C>;
     template <int R, int C> using Fine = TileH<3, R, C>;
     template <int R, int C> using Coarse = TileH<2, R, C>;
-    static constexpr int square_bytes = 3 * 2 * kChunk * kChunk;
+    using InputFrag = FragH<1>;
+    using FineFrag = FragH<3>;
 };
 template <> struct Mode<float> {
     template <int R, int C> using Input = TileF<R, C>;
     template <int R, int C> using Fine = TileF<R, C>;
     template <int R, int C> using Coarse = TileF<R, C>;
-    static constexpr int square_bytes = 4 * kChunk * kChunk;
+    using InputFrag = FragF;
+    using FineFrag = FragF;
 };
+
+// Bytes of a chunk's operands in this form: keys (or queries) by rows or transposed, and a 64 x 64 matrix.
+template <typename E> constexpr int keys_bytes(int dkp) { return dkp / 8 * frag_bytes<typename Mode<E>::InputFrag>(); }
+template <typename E> constexpr int square_bytes() { return 8 * frag_bytes<typename Mode<E>::FineFrag>(); }
 
 // ---- arguments ----------------------------------------------------------------------------------
 
@@ -263,10 +307,12 @@ struct DeltaArgs {
     // per (batch entry, value head, chunk); matrices with a column of the state are transposed, as the state passes
     // hold them: each column of theirs is one run of memory
     Decay* decay;
-    char* inverse;              // Tm [64, 64], Mode::square_bytes
+    char *inverse, *inverse_t;  // Tm and its transpose, fragments (band of 16 rows, 32 columns of it); the latter or nullptr
+    char *keys, *keys_t;        // per (batch entry, key head, chunk): K by rows, and transposed, fragments
     float* added;               // R, [cols, 64]
     float* states;              // state before the chunk, [cols, DKP]
     // backward
+    char* queries_t;            // as keys_t
     float* inner;               // P^T dO, then dX, [cols, 64]
     float* state_grads;         // gradient of the state after the chunk, [cols, DKP]
     void *grad_q, *grad_k;      // [T, B, Hk, Dk] of the storage type, or fp32 [T, B, Hv, Dk] where heads share keys
@@ -278,7 +324,8 @@ struct DeltaArgs {
 struct DeltaWhere {  // the chunk (or head) a workgroup works on
     int b, hv, hk, chunk, head;
     int t0, rows;    // first step and how many of its 64 rows exist
-    int64_t at;      // its place among the matrices
+    int64_t at;      // its place among the matrices of the value heads
+    int64_t key_at;  // and of the key heads
 };
 
 __device__ __forceinline__ int delta_length(const DeltaArgs& a, int b) {
@@ -287,7 +334,8 @@ __device__ __forceinline__ int delta_length(const DeltaArgs& a, int b) {
     return n < 0 ? 0 : n > a.T ? a.T : n;
 }
 
-__device__ __forceinline__ DeltaWhere delta_where(const DeltaArgs& a, int head, int chunk) {
+// `length` of the head's sequence, where it is known already
+__device__ __forceinline__ DeltaWhere delta_where(const DeltaArgs& a, int head, int chunk, int length = -1) {
     DeltaWhere w;
     w.head = head;
     w.b = head / a.Hv;
@@ -295,32 +343,58 @@ __device__ __forceinline__ DeltaWhere delta_where(const DeltaArgs& a, int head, 
     w.hk = w.hv / (a.Hv / a.Hk);
     w.chunk = chunk;
     w.t0 = chunk * kChunk;
-    const int left = delta_length(a, w.b) - w.t0;
+    const int left = (length < 0 ? delta_length(a, w.b) : length) - w.t0;
     w.rows = left < 0 ? 0 : left > kChunk ? kChunk : left;
     w.at = static_cast<int64_t>(head) * a.chunks + chunk;
+    w.key_at = (static_cast<int64_t>(w.b) * a.Hk + w.hk) * a.chunks + chunk;
     return w;
 }
 
 // ---- staging ------------------------------------------------------------------------------------
 
-// Eight consecutive values of a row, zero behind `valid`.
-template <typename E>
-__device__ __forceinline__ Raw8<E> load_raw8(const E* row, int c, int valid, bool wide) {
+// Eight consecutive values of a row.  Without a branch and without a look at the values, so that all loads of a thread
+// are under way together: what lies behind `valid` is read at the row's beginning, and keep_valid takes it out later.
+template <bool WIDE, typename E>
+__device__ __forceinline__ Raw8<E> load_raw8(const E* row, int c, int valid) {
     Raw8<E> x;
+    if constexpr (WIDE) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(row + (c < valid ? c : 0));
 #pragma unroll
-    for (u32x4& part : x.r) part = u32x4{0, 0, 0, 0};
-    if (wide) {
-        if (c < valid) {
-#pragma unroll
-            for (int h = 0; h < static_cast<int>(sizeof(E) / 2); ++h) x.r[h] = reinterpret_cast<const u32x4*>(row + c)[h];
-        }
+        for (int h = 0; h < static_cast<int>(sizeof(E) / 2); ++h) x.r[h] = p[h];
     } else {
+        uint32_t bits[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (c + j < valid) {
-                if constexpr (sizeof(E) == 4) x.r[j / 4][j % 4] = __builtin_bit_cast(uint32_t, row[c + j]);
-                else x.r[0][j / 2] |= static_cast<uint32_t>(row[c + j].bits) << (j % 2 * 16);
-            }
+        for (int j = 0; j < 8; ++j) {
+            const E v = row[c + j < valid ? c + j : 0];
+            if constexpr (sizeof(E) == 4) bits[j] = __builtin_bit_cast(uint32_t, v);
+            else bits[j] = v.bits;
+        }
+        if constexpr (sizeof(E) == 4) {
+            x.r[0] = u32x4{bits[0], bits[1], bits[2], bits[3]};
+            x.r[1] = u32x4{bits[4], bits[5], bits[6], bits[7]};
+        } else {
+            x.r[0] = u32x4{bits[0] | bits[1] << 16, bits[2] | bits[3] << 16, bits[4] | bits[5] << 16, bits[6] | bits[7] << 16};
+        }
+    }
+    return x;
+}
+
+// Zero at and behind `valid` (wide rows end at a multiple of eight).
+template <bool WIDE, typename E>
+__device__ __forceinline__ Raw8<E> keep_valid(Raw8<E> x, int c, int valid) {
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int h = 0; h < static_cast<int>(sizeof(E) / 2); ++h) x.r[h] = c < valid ? x.r[h] : u32x4{0, 0, 0, 0};
+    } else {
+        constexpr int per = 4 / static_cast<int>(sizeof(E));   // values per word
+#pragma unroll
+        for (int j = 0; j < 8 / per; ++j) {
+            const int left = valid - c - j * per;
+            uint32_t word = x.r[j / 4][j % 4];
+            if constexpr (per == 2) word = left > 1 ? word : left == 1 ? word & 0xffffu : 0u;
+            else word = left > 0 ? word : 0u;
+            x.r[j / 4][j % 4] = word;
+        }
     }
     return x;
 }
@@ -342,17 +416,24 @@ __device__ __forceinline__ void values_of(const Raw8<float>& x, float (&v)[8]) {
 
 // ROWS x COLS of a tensor, eight values of a row per access, requested now (load) and put into LDS later (store), so
 // that a product can run in between.
-template <typename E, int ROWS, int COLS, int THREADS>
+template <bool WIDE, typename E, int ROWS, int COLS, int THREADS>
 struct Ahead {
     static constexpr int total = ROWS * COLS / 8, n = (total + THREADS - 1) / THREADS;
     Raw8<E> x[n];
-    // rows `stride` values apart, of which `rows` x `valid` exist
-    __device__ __forceinline__ void load(const E* base, int64_t stride, int rows, int valid, bool wide) {
+    int rows, valid;
+    // rows `stride` values apart, of which `rows_` x `valid_` exist (one at least of each)
+    __device__ __forceinline__ void load(const E* base, int64_t stride, int rows_, int valid_) {
+        rows = rows_;
+        valid = valid_;
 #pragma unroll
         for (int i = 0; i < n; ++i) {
             const int seg = i * THREADS + threadIdx.x, r = seg / (COLS / 8), c = seg % (COLS / 8) * 8;
-            x[i] = load_raw8<E>(base + (r < rows ? r : 0) * stride, c, r < rows ? valid : 0, wide);
+            x[i] = load_raw8<WIDE, E>(base + (r < rows ? r : 0) * stride, c, valid);
         }
+    }
+    __device__ __forceinline__ Raw8<E> get(int i) const {
+        const int seg = i * THREADS + threadIdx.x, r = seg / (COLS / 8), c = seg % (COLS / 8) * 8;
+        return keep_valid<WIDE, E>(x[i], c, r < rows ? valid : 0);
     }
     template <typename Tile>
     __device__ __forceinline__ void store(Tile& tile) const {
@@ -360,44 +441,35 @@ struct Ahead {
         for (int i = 0; i < n; ++i) {
             const int seg = i * THREADS + threadIdx.x;
             if (total % THREADS != 0 && seg >= total) break;
-            tile.put(seg / (COLS / 8), seg % (COLS / 8) * 8, x[i]);
-        }
-    }
-    // through fp32 values, for tiles of several parts
-    template <typename Tile>
-    __device__ __forceinline__ void store_values(Tile& tile) const {
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const int seg = i * THREADS + threadIdx.x;
-            if (total % THREADS != 0 && seg >= total) break;
-            float v[8];
-            values_of(x[i], v);
-            tile.put(seg / (COLS / 8), seg % (COLS / 8) * 8, v);
+            tile.put(seg / (COLS / 8), seg % (COLS / 8) * 8, get(i));
         }
     }
 };
 
-// A 64 x 64 matrix in the form kernels hand to each other: its parts, without padding.
-template <typename E, int THREADS>
-struct SquareAhead {
-    static constexpr int n = Mode<E>::square_bytes / 16 / THREADS;
-    u32x4 x[n];
-    __device__ __forceinline__ void load(const char* p) {
-#pragma unroll
-        for (int i = 0; i < n; ++i) x[i] = reinterpret_cast<const u32x4*>(p)[i * THREADS + threadIdx.x];
+// ROWS x COLS of an fp32 matrix without gaps, stored as the parts a tile keeps.
+template <int ROWS, int COLS, int THREADS>
+struct MatrixAhead {
+    static constexpr int total = ROWS * COLS / 8, n = (total + THREADS - 1) / THREADS;
+    Raw8<float> x[n];
+    __device__ __forceinline__ static bool mine(int i) {
+        return total % THREADS == 0 || i * THREADS + static_cast<int>(threadIdx.x) < total;
     }
-    __device__ __forceinline__ void store(TileH<3, kChunk, kChunk>& tile) const {
+    __device__ __forceinline__ void load(const float* base) {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int seg = i * THREADS + threadIdx.x, part = seg / 512, r = seg % 512 / 8, c = seg % 8 * 8;
-            *reinterpret_cast<u32x4*>(&tile.v[part][r * tile.ld + c]) = x[i];
+            const int seg = mine(i) ? i * THREADS + threadIdx.x : 0;
+            x[i] = load_raw8<true, float>(base, seg * 8, total * 8);
         }
     }
-    __device__ __forceinline__ void store(TileF<kChunk, kChunk>& tile) const {
+    template <typename Tile>
+    __device__ __forceinline__ void store(Tile& tile) const {
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const int seg = i * THREADS + threadIdx.x, r = seg / 16, c = seg % 16 * 4;
-            *reinterpret_cast<u32x4*>(&tile.v[r * tile.ld + c]) = x[i];
+            const int seg = i * THREADS + threadIdx.x;
+            if (!mine(i)) break;
+            float v[8];
+            values_of(x[i], v);
+            tile.put(seg / (COLS / 8), seg % (COLS / 8) * 8, v);
         }
     }
 };
@@ -431,11 +503,17 @@ __device__ __forceinline__ void decay_of(const DeltaArgs& args, const DeltaWhere
     out.beta[lane] = beta;
 }
 
-__device__ __forceinline__ void load_decay(const DeltaArgs& args, const DeltaWhere& w, Decay& out) {
-    static_assert(sizeof(Decay) == 16 * 80, "a Decay is copied in vectors");
-    if (threadIdx.x < sizeof(Decay) / 16)
-        reinterpret_cast<u32x4*>(&out)[threadIdx.x] = reinterpret_cast<const u32x4*>(args.decay + w.at)[threadIdx.x];
-}
+struct DecayAhead {
+    static constexpr unsigned n = sizeof(Decay) / 16;
+    u32x4 x;
+    __device__ __forceinline__ void load(const DeltaArgs& args, int64_t at) {
+        x = reinterpret_cast<const u32x4*>(args.decay + at)[threadIdx.x < n ? threadIdx.x : 0];
+    }
+    __device__ __forceinline__ void store(Decay& out) const {
+        if (threadIdx.x < n) reinterpret_cast<u32x4*>(&out)[threadIdx.x] = x;
+    }
+};
+static_assert(sizeof(Decay) % 16 == 0, "a Decay is copied in vectors");
 
 __device__ __forceinline__ float gap(const Decay& y, int i, int j) {  // G_ij
     return __builtin_amdgcn_exp2f(static_cast<float>(y.c[i] - y.c[j]));
@@ -448,6 +526,18 @@ __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 __device__ __forceinline__ int piece_in_l2(int total) {
     const int per = total / 8, id = blockIdx.x;
     return id < per * 8 ? (id % 8) * per + id / 8 : id;
+}
+
+// The transpose of staged keys or queries, as fragments (16 key columns, half of the rows), by WAVES wavefronts.
+template <typename E, int DKP, int WAVES, typename Tile>
+__device__ __forceinline__ void store_transposed(const Tile& tile, char* out) {
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < DKP / 8; i += WAVES) {
+        const int index = i + wave;
+        if (DKP / 8 % WAVES != 0 && index >= DKP / 8) break;
+        store_frag(out, index, tile.cols(index / 2 * 16, index % 2 * 32));
+    }
 }
 
 // ---- Tm = (I + A)^-1 ----------------------------------------------------------------------------
@@ -501,7 +591,7 @@ __device__ __forceinline__ void invert_unit_lower(const Square& a, Square& t, Sq
     }
 }
 
-template <typename E, int DKP>
+template <typename E, bool WIDE, int DKP>
 __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
     using M = Mode<E>;
     union First {   // K is done with when the inversion needs its scratch
@@ -514,8 +604,8 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
     __shared__ Decay y;
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
     if (w.rows == 0) return;
-    Ahead<E, kChunk, DKP, 256> k;
-    k.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+    Ahead<WIDE, E, kChunk, DKP, 256> k;
+    k.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
     decay_of(args, w, y);
     for (int i = threadIdx.x; i < kChunk * (kChunk + 4); i += 256) (&t.v[0][0])[i] = 0.f;
     k.store(u.k);
@@ -523,6 +613,12 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
     if (threadIdx.x < sizeof(Decay) / 16)
         reinterpret_cast<u32x4*>(args.decay + w.at)[threadIdx.x] = reinterpret_cast<const u32x4*>(&y)[threadIdx.x];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (w.hv % (args.Hv / args.Hk) == 0) {   // the first of the value heads that share these keys
+#pragma unroll
+        for (int s = 0; s < DKP / 32; ++s)
+            store_frag(args.keys + w.key_at * keys_bytes<E>(DKP), wave * (DKP / 32) + s, u.k.rows(wave * 16, s * 32));
+        store_transposed<E, DKP, 4>(u.k, args.keys_t + w.key_at * keys_bytes<E>(DKP));
+    }
     for (int block = 0; block <= wave; ++block) {
         f32x4 acc = zero4();
 #pragma unroll
@@ -535,22 +631,21 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
     }
     __syncthreads();
     invert_unit_lower(a, t, u.scratch);
-    char* out = args.inverse + w.at * M::square_bytes;
+    // fragment (band of rows or columns, half of the contraction): a wavefront writes both halves of its band
 #pragma unroll
-    for (int i = 0; i < kChunk * kChunk / 8; i += 256) {
-        const int seg = i + threadIdx.x, r = seg / 8, c = seg % 8 * 8;
-        if constexpr (sizeof(E) == 4) {
-            reinterpret_cast<f32x4*>(out)[seg * 2] = *reinterpret_cast<const f32x4*>(&t.v[r][c]);
-            reinterpret_cast<f32x4*>(out)[seg * 2 + 1] = *reinterpret_cast<const f32x4*>(&t.v[r][c + 4]);
-        } else {
-            float x[8];
-            uint32_t words[3][4];
+    for (int s = 0; s < 2; ++s) {
+        const int r = wave * 16 + (lane & 15), c = s * 32 + (lane >> 4) * 8;
+        float x[8];
+        typename M::FineFrag f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = t.v[r][c + j];
-            split<3, 8>(x, words);
+        for (int j = 0; j < 8; ++j) x[j] = t.v[r][c + j];
+        frag_of(x, f);
+        store_frag(args.inverse + w.at * square_bytes<E>(), wave * 2 + s, f);
+        if (args.inverse_t != nullptr) {
 #pragma unroll
-            for (int part = 0; part < 3; ++part)
-                reinterpret_cast<u32x4*>(out)[part * 512 + seg] = u32x4{words[part][0], words[part][1], words[part][2], words[part][3]};
+            for (int j = 0; j < 8; ++j) x[j] = t.v[c + j][r];
+            frag_of(x, f);
+            store_frag(args.inverse_t + w.at * square_bytes<E>(), wave * 2 + s, f);
         }
     }
 }
@@ -558,8 +653,10 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
 // ---- the state passes ---------------------------------------------------------------------------
 //
 // A workgroup of four wavefronts holds kStateCols columns of a head's state: wavefront w rows 16 w.. of the chunk in
-// the first two products, DKP / 64 tiles of 16 state rows in the last one.  What the next chunk needs is requested
-// before the products of this one and put into LDS after them.
+// the first two products, DKP / 64 tiles of 16 state rows in the last one.  The chain from chunk to chunk -- three
+// products, each through LDS to the next -- is all that counts, so nothing else is on it: keys and matrices come as
+// fragments, straight into registers, a chunk ahead (two sets of registers take turns), and LDS holds only what the
+// wavefronts exchange.
 
 constexpr int kStateThreads = 256;
 
@@ -602,103 +699,133 @@ struct StateTiles {
     }
 };
 
-// a, d, beta of a chunk, one value per thread.
-struct FactorsAhead {
-    float x;
-    __device__ __forceinline__ void load(const DeltaArgs& args, int64_t at) {
-        const float* f = reinterpret_cast<const float*>(reinterpret_cast<const char*>(args.decay + at) + offsetof(Decay, a));
-        x = threadIdx.x < 3 * kChunk ? f[threadIdx.x] : 0.f;   // a, d and beta follow each other
+// Four rows of one column of a strided input, in the layout of a product; requested and looked at apart, as above.
+template <typename E>
+struct ColumnAhead {
+    E x[4];
+    int rows;
+    __device__ __forceinline__ void load(const DeltaTensor& t, const DeltaWhere& w, int head, int row, int col, int valid) {
+        rows = col < valid ? w.rows - row : 0;
+        const E* p = row_of<E>(t, w, head) + (rows > 0 ? row * t.t + col : 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = p[min(e, max(rows - 1, 0)) * t.t];
     }
-    __device__ __forceinline__ void store(float (&f)[3 * kChunk]) const {
-        if (threadIdx.x < 3 * kChunk) f[threadIdx.x] = x;
+    __device__ __forceinline__ float get(int e) const { return e < rows ? widen(x[e]) : 0.f; }
+};
+
+// What the forward pass takes from memory for a chunk.
+template <typename E, int DKP>
+struct StateOperands {
+    using M = Mode<E>;
+    typename M::InputFrag k[DKP / 32], kt[DKP / 64][2];
+    typename M::FineFrag inverse[2];
+    f32x4 a, d, beta;
+    float a_last;
+    ColumnAhead<E> v;
+    DeltaWhere w;
+    // in three parts, each requested while a product waits for LDS: a vector access of a wavefront occupies the
+    // memory path of the CU for 16 cycles, and all of them in a row would stand in the way of the chain
+    __device__ __forceinline__ void load_keys(const DeltaArgs& args, int head, int chunk, int length, int row, int col) {
+        w = delta_where(args, head, chunk, length);
+        const char* keys = args.keys + w.key_at * keys_bytes<E>(DKP);
+#pragma unroll
+        for (int s = 0; s < DKP / 32; ++s) k[s] = load_frag<typename M::InputFrag>(keys, (threadIdx.x >> 6) * (DKP / 32) + s);
+        const Decay* y = args.decay + w.at;
+        a = *reinterpret_cast<const f32x4*>(y->a + row);
+        d = *reinterpret_cast<const f32x4*>(y->d + row);
+        beta = *reinterpret_cast<const f32x4*>(y->beta + row);
+        a_last = y->a[kChunk - 1];
+        v.load(args.v, w, w.hv, row, col, args.Dv);
+    }
+    __device__ __forceinline__ void load_inverse(const DeltaArgs& args) {
+        const char* matrix = args.inverse + w.at * square_bytes<E>();
+        inverse[0] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2);
+        inverse[1] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2 + 1);
+    }
+    __device__ __forceinline__ void load_transposed(const DeltaArgs& args) {
+        const char* keys_t = args.keys_t + w.key_at * keys_bytes<E>(DKP);
+#pragma unroll
+        for (int i = 0; i < DKP / 64; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                kt[i][s] = load_frag<typename M::InputFrag>(keys_t, ((threadIdx.x >> 6) + 4 * i) * 2 + s);
     }
 };
-static_assert(offsetof(Decay, d) == offsetof(Decay, a) + 4 * kChunk && offsetof(Decay, beta) == offsetof(Decay, d) + 4 * kChunk,
-              "a, d and beta are read as one array");
-
-// Four rows of one column of a strided input, in the layout of a product.
-template <typename E>
-__device__ __forceinline__ void load_column(const DeltaTensor& x, const DeltaWhere& w, int head, int row, int col,
-                                            int valid, E (&out)[4]) {
-    const E* p = row_of<E>(x, w, head);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        out[e] = narrow<E>(0.f);
-        if (row + e < w.rows && col < valid) out[e] = p[(row + e) * x.t + col];
-    }
-}
 
 template <typename E, int DKP>
 __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(DeltaArgs args) {
     using M = Mode<E>;
     constexpr int NV = kStateCols;
-    __shared__ typename M::template Input<kChunk, DKP> k;
-    __shared__ typename M::template Fine<kChunk, kChunk> inverse;
     __shared__ typename M::template Fine<NV, DKP> state;     // transposed
     __shared__ typename M::template Fine<NV, kChunk> x, r;   // transposed
-    __shared__ float factors[3 * kChunk];
-    const float *fa = factors, *fd = factors + kChunk, *fb = factors + 2 * kChunk;
     const int tiles = args.cols / NV;
     const int piece = piece_in_l2(args.B * args.Hv * tiles), head = piece / tiles, v0 = (piece - head * tiles) * NV;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int lc = lane & 15, row = wave * 16 + (lane >> 4) * 4, col = v0 + lc;
-    DeltaWhere w = delta_where(args, head, 0);
-    const int chunks = (delta_length(args, w.b) + kChunk - 1) / kChunk;
+    const int length = delta_length(args, head / args.Hv), chunks = (length + kChunk - 1) / kChunk;
 
-    Ahead<E, kChunk, DKP, kStateThreads> k_next;
-    SquareAhead<E, kStateThreads> inverse_next;
-    FactorsAhead factors_next;
-    E v_next[4], v[4];
-    const auto request = [&](const DeltaWhere& n) {
-        k_next.load(row_of<E>(args.k, n, n.hk), args.k.t, n.rows, args.Dk, args.k.wide != 0);
-        inverse_next.load(args.inverse + n.at * M::square_bytes);
-        factors_next.load(args, n.at);
-        load_column<E>(args.v, n, n.hv, row, col, args.Dv, v_next);
-    };
-    if (chunks > 0) request(w);
+    StateOperands<E, DKP> even, odd;
+    if (chunks > 0) {
+        even.load_keys(args, head, 0, length, row, col);
+        even.load_inverse(args);
+        even.load_transposed(args);
+    }
     StateTiles<DKP> s;
     s.load(args.state, head, args.Dk, args.Dv, col);
     s.put(state);
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        k_next.store(k);
-        inverse_next.store(inverse);
-        factors_next.store(factors);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = v_next[e];
-        const int64_t at = w.at;
+    const auto step = [&](int chunk, const StateOperands<E, DKP>& now, StateOperands<E, DKP>& next) {
+        // behind the last chunk: the same once more.  Loads under a condition would make every wait one for all of them
+        const int ahead = chunk + 1 < chunks ? chunk + 1 : chunk;
         __syncthreads();
-        if (chunk + 1 < chunks) {
-            w = delta_where(args, head, chunk + 1);
-            request(w);
-        }
-        s.keep(args.states + at * DKP * args.cols, col);
-        f32x4 acc = zero4();
+        f32x4 acc[2] = {zero4(), zero4()};
+        typename M::FineFrag f[DKP / 32];
 #pragma unroll
-        for (int c = 0; c < DKP; c += 32) acc = mma(k.rows(wave * 16, c), state.rows(0, c), acc);
+        for (int c = 0; c < DKP / 32; ++c) f[c] = state.rows(0, c * 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_keys(args, head, ahead, length, row, col);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < DKP / 32; ++c) acc[c % 2] = mma(now.k[c], f[c], acc[c % 2]);
         float out[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = fb[row + e] * (widen(v[e]) - fa[row + e] * acc[e]);
+        for (int e = 0; e < 4; ++e) out[e] = now.beta[e] * (now.v.get(e) - now.a[e] * (acc[0][e] + acc[1][e]));
         x.put(lc, row, out);
+        s.keep(args.states + now.w.at * DKP * args.cols, col);
         __syncthreads();
-        acc = zero4();
-        for (int c = 0; c < wave * 16 + 16; c += 32) acc = mma(inverse.rows(wave * 16, c), x.rows(0, c), acc);
-        *reinterpret_cast<f32x4*>(args.added + (at * args.cols + col) * kChunk + row) = acc;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = fd[row + e] * acc[e];
-        r.put(lc, row, out);
-        __syncthreads();
-        const float last = fa[kChunk - 1];
-#pragma unroll
-        for (int i = 0; i < s.n; ++i) {
-            f32x4 next;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) next[e] = last * s.s[i][e];
-#pragma unroll
-            for (int c = 0; c < kChunk; c += 32) next = mma(k.cols((wave + 4 * i) * 16, c), r.rows(0, c), next);
-            s.s[i] = next;
+        f[0] = x.rows(0, 0);
+        f[1] = x.rows(0, 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_inverse(args);
+        __builtin_amdgcn_sched_barrier(0);
+        acc[0] = mma(now.inverse[0], f[0], zero4());
+        if (wave >= 2) {   // rows below 32 have nothing right of column 32
+            acc[1] = mma(now.inverse[1], f[1], zero4());
+            acc[0] += acc[1];
         }
-        s.put(state);
+        f32x4 next_s[s.n];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = now.d[e] * acc[0][e];
+        r.put(lc, row, out);
+        *reinterpret_cast<f32x4*>(args.added + (now.w.at * args.cols + col) * kChunk + row) = acc[0];
+#pragma unroll
+        for (int i = 0; i < s.n; ++i) next_s[i] = now.a_last * s.s[i];
         __syncthreads();
+        f[0] = r.rows(0, 0);
+        f[1] = r.rows(0, 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_transposed(args);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < s.n; ++i) next_s[i] = mma(now.kt[i][c], f[c], next_s[i]);
+#pragma unroll
+        for (int i = 0; i < s.n; ++i) s.s[i] = next_s[i];
+        s.put(state);
+    };
+    for (int chunk = 0; chunk < chunks; chunk += 2) {
+        step(chunk, even, odd);
+        if (chunk + 1 < chunks) step(chunk + 1, odd, even);
     }
     s.save(args.state_out, head, args.Dk, args.Dv, col);
 }
@@ -730,7 +857,7 @@ __device__ __forceinline__ void scores_of(const TQ& q, const TK& k, const Decay&
     }
 }
 
-template <typename E, int DKP>
+template <typename E, bool WIDE, int DKP>
 __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs args) {
     using M = Mode<E>;
     constexpr int NV = kCols;
@@ -758,18 +885,20 @@ __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs a
             out[i / args.Dv * out_stride + i % args.Dv] = narrow<E>(0.f);
         return;
     }
-    Ahead<float, NV, DKP, kPieceThreads> state_next;
-    Ahead<float, NV, kChunk, kPieceThreads> r_next;
+    MatrixAhead<NV, DKP, kPieceThreads> state_next;
+    MatrixAhead<NV, kChunk, kPieceThreads> r_next;
     const auto request = [&](int v0) {
-        state_next.load(args.states + (w.at * args.cols + v0) * DKP, DKP, NV, DKP, true);
-        r_next.load(args.added + (w.at * args.cols + v0) * kChunk, kChunk, NV, kChunk, true);
+        state_next.load(args.states + (w.at * args.cols + v0) * DKP);
+        r_next.load(args.added + (w.at * args.cols + v0) * kChunk);
     };
     {
-        Ahead<E, kChunk, DKP, kPieceThreads> q_next, k_next;
-        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
-        load_decay(args, w, y);
+        Ahead<WIDE, E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
+        DecayAhead y_next;
+        y_next.load(args, w.at);
         request(0);
+        y_next.store(y);
         q_next.store(q);
         k_next.store(u.k);
     }
@@ -777,8 +906,8 @@ __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs a
     scores_of<DKP>(q, u.k, y, args.scale, p);
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
-        state_next.store_values(u.c.state);
-        r_next.store_values(u.c.r);
+        state_next.store(u.c.state);
+        r_next.store(u.c.r);
         __syncthreads();
         if (v0 + NV < args.cols) request(v0 + NV);
         f32x4 acc = zero4();
@@ -797,7 +926,7 @@ __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs a
 
 // ---- backward: P^T dO ---------------------------------------------------------------------------
 
-template <typename E, int DKP>
+template <typename E, bool WIDE, int DKP>
 __global__ void __launch_bounds__(kPieceThreads) delta_inner_grad_kernel(DeltaArgs args) {
     using M = Mode<E>;
     constexpr int NV = kCols;
@@ -816,21 +945,25 @@ __global__ void __launch_bounds__(kPieceThreads) delta_inner_grad_kernel(DeltaAr
     if (w.rows == 0) return;
     const int lane = threadIdx.x & 63, band = threadIdx.x >> 6 & 3, half = threadIdx.x >> 8;
     const int lr = band * 16 + (lane >> 4) * 4, lc = lane & 15;
-    Ahead<E, kChunk, NV, kPieceThreads> go_next;
+    Ahead<WIDE, E, kChunk, NV, kPieceThreads> go_next;
     const E* pg = row_of<E>(args.grad_o, w, w.hv);
     const auto request = [&](int v0) {
-        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0, args.grad_o.wide != 0);
+        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0);
     };
     {
-        Ahead<E, kChunk, DKP, kPieceThreads> q_next, k_next;
-        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
-        load_decay(args, w, y);
+        Ahead<WIDE, E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
+        DecayAhead y_next;
+        y_next.load(args, w.at);
         request(0);
+        y_next.store(y);
         q_next.store(u.s.q);
         k_next.store(u.s.k);
     }
     __syncthreads();
+    if (w.hv % (args.Hv / args.Hk) == 0)
+        store_transposed<E, DKP, kPieceThreads / 64>(u.s.q, args.queries_t + w.key_at * keys_bytes<E>(DKP));
     scores_of<DKP>(u.s.q, u.s.k, y, args.scale, p);
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
@@ -846,92 +979,128 @@ __global__ void __launch_bounds__(kPieceThreads) delta_inner_grad_kernel(DeltaAr
 // ---- the state, backwards -----------------------------------------------------------------------
 
 template <typename E, int DKP>
+struct StateGradOperands {
+    using M = Mode<E>;
+    typename M::InputFrag k[DKP / 32], kt[DKP / 64][2], qt[DKP / 64][2];
+    typename M::FineFrag inverse[2];   // transposed
+    f32x4 a, d, beta, inner;
+    float a_last;
+    ColumnAhead<E> go;
+    DeltaWhere w;
+    // in parts, as in the forward pass
+    __device__ __forceinline__ void load_keys(const DeltaArgs& args, int head, int chunk, int length, int row, int col) {
+        w = delta_where(args, head, chunk, length);
+        const char* keys = args.keys + w.key_at * keys_bytes<E>(DKP);
+#pragma unroll
+        for (int s = 0; s < DKP / 32; ++s) k[s] = load_frag<typename M::InputFrag>(keys, (threadIdx.x >> 6) * (DKP / 32) + s);
+        inner = *reinterpret_cast<const f32x4*>(args.inner + (w.at * args.cols + col) * kChunk + row);
+        go.load(args.grad_o, w, w.hv, row, col, args.Dv);
+        const Decay* y = args.decay + w.at;
+        a = *reinterpret_cast<const f32x4*>(y->a + row);
+        d = *reinterpret_cast<const f32x4*>(y->d + row);
+        beta = *reinterpret_cast<const f32x4*>(y->beta + row);
+        a_last = y->a[kChunk - 1];
+    }
+    __device__ __forceinline__ void load_inverse(const DeltaArgs& args) {
+        const char* matrix = args.inverse_t + w.at * square_bytes<E>();
+        inverse[1] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2 + 1);
+        inverse[0] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2);
+    }
+    __device__ __forceinline__ void load_transposed(typename M::InputFrag (&x)[DKP / 64][2], const char* matrix) {
+#pragma unroll
+        for (int i = 0; i < DKP / 64; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                x[i][s] = load_frag<typename M::InputFrag>(matrix + w.key_at * keys_bytes<E>(DKP), ((threadIdx.x >> 6) + 4 * i) * 2 + s);
+    }
+};
+
+template <typename E, int DKP>
 __global__ void __launch_bounds__(kStateThreads) delta_state_grad_kernel(DeltaArgs args) {
     using M = Mode<E>;
     constexpr int NV = kStateCols;
-    __shared__ typename M::template Input<kChunk, DKP> q, k;
-    __shared__ typename M::template Fine<kChunk, kChunk> inverse;
     __shared__ typename M::template Fine<NV, DKP> state;       // gradient of the state, transposed
     __shared__ typename M::template Fine<NV, kChunk> r, x, go; // dR, -beta a dX, scale a dO, transposed
-    __shared__ float factors[3 * kChunk];
-    const float *fa = factors, *fd = factors + kChunk, *fb = factors + 2 * kChunk;
     const int tiles = args.cols / NV;
     const int piece = piece_in_l2(args.B * args.Hv * tiles), head = piece / tiles, v0 = (piece - head * tiles) * NV;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int lc = lane & 15, row = wave * 16 + (lane >> 4) * 4, col = v0 + lc;
-    DeltaWhere w = delta_where(args, head, 0);
-    const int chunks = (delta_length(args, w.b) + kChunk - 1) / kChunk;
+    const int length = delta_length(args, head / args.Hv), chunks = (length + kChunk - 1) / kChunk;
 
-    Ahead<E, kChunk, DKP, kStateThreads> q_next, k_next;
-    SquareAhead<E, kStateThreads> inverse_next;
-    FactorsAhead factors_next;
-    E g_next[4], g[4];
-    f32x4 inner_next, inner;
-    const auto request = [&](const DeltaWhere& n) {
-        q_next.load(row_of<E>(args.q, n, n.hk), args.q.t, n.rows, args.Dk, args.q.wide != 0);
-        k_next.load(row_of<E>(args.k, n, n.hk), args.k.t, n.rows, args.Dk, args.k.wide != 0);
-        inverse_next.load(args.inverse + n.at * M::square_bytes);
-        factors_next.load(args, n.at);
-        load_column<E>(args.grad_o, n, n.hv, row, col, args.Dv, g_next);
-        inner_next = *reinterpret_cast<const f32x4*>(args.inner + (n.at * args.cols + col) * kChunk + row);
-    };
+    StateGradOperands<E, DKP> even, odd;
     if (chunks > 0) {
-        w = delta_where(args, head, chunks - 1);
-        request(w);
+        even.load_keys(args, head, chunks - 1, length, row, col);
+        even.load_transposed(even.qt, args.queries_t);
+        even.load_inverse(args);
+        even.load_transposed(even.kt, args.keys_t);
     }
     StateTiles<DKP> s;
     s.load(args.grad_state, head, args.Dk, args.Dv, col);
     s.put(state);
-    for (int chunk = chunks - 1; chunk >= 0; --chunk) {
-        q_next.store(q);
-        k_next.store(k);
-        inverse_next.store(inverse);
-        factors_next.store(factors);
+    const auto step = [&](int chunk, const StateGradOperands<E, DKP>& now, StateGradOperands<E, DKP>& next) {
+        float out[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = g_next[e];
-        inner = inner_next;
-        const int64_t at = w.at;
+        for (int e = 0; e < 4; ++e) out[e] = args.scale * now.a[e] * now.go.get(e);
+        go.put(lc, row, out);   // its readers of the chunk before are behind a barrier
+        const int ahead = chunk > 0 ? chunk - 1 : 0;   // as above
         __syncthreads();
-        if (chunk > 0) {
-            w = delta_where(args, head, chunk - 1);
-            request(w);
-        }
-        s.keep(args.state_grads + at * DKP * args.cols, col);
-        f32x4 acc = zero4();
+        f32x4 acc[2] = {zero4(), zero4()};
+        typename M::FineFrag f[DKP / 32];
 #pragma unroll
-        for (int c = 0; c < DKP; c += 32) acc = mma(k.rows(wave * 16, c), state.rows(0, c), acc);
-        float out[4], scaled[4];
+        for (int c = 0; c < DKP / 32; ++c) f[c] = state.rows(0, c * 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_keys(args, head, ahead, length, row, col);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            out[e] = inner[e] + fd[row + e] * acc[e];
-            scaled[e] = args.scale * fa[row + e] * widen(g[e]);
-        }
+        for (int c = 0; c < DKP / 32; ++c) acc[c % 2] = mma(now.k[c], f[c], acc[c % 2]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = now.inner[e] + now.d[e] * (acc[0][e] + acc[1][e]);
         r.put(lc, row, out);
-        go.put(lc, row, scaled);
+        s.keep(args.state_grads + now.w.at * DKP * args.cols, col);
         __syncthreads();
-        acc = zero4();
-        for (int c = wave * 16 / 32 * 32; c < kChunk; c += 32) acc = mma(inverse.cols(wave * 16, c), r.rows(0, c), acc);
-        *reinterpret_cast<f32x4*>(args.inner + (at * args.cols + col) * kChunk + row) = acc;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = -fb[row + e] * fa[row + e] * acc[e];
-        x.put(lc, row, out);
-        const float last = fa[kChunk - 1];
-#pragma unroll
-        for (int i = 0; i < s.n; ++i) {   // what does not wait for dX
-            f32x4 next;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) next[e] = last * s.s[i][e];
-#pragma unroll
-            for (int c = 0; c < kChunk; c += 32) next = mma(q.cols((wave + 4 * i) * 16, c), go.rows(0, c), next);
-            s.s[i] = next;
+        f[0] = r.rows(0, 0);
+        f[1] = r.rows(0, 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_inverse(args);
+        __builtin_amdgcn_sched_barrier(0);
+        acc[1] = mma(now.inverse[1], f[1], zero4());
+        if (wave < 2) {   // columns from 32 on have nothing above row 32
+            acc[0] = mma(now.inverse[0], f[0], zero4());
+            acc[1] += acc[0];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = -now.beta[e] * now.a[e] * acc[1][e];
+        x.put(lc, row, out);
+        *reinterpret_cast<f32x4*>(args.inner + (now.w.at * args.cols + col) * kChunk + row) = acc[1];
+        f[0] = go.rows(0, 0);   // does not wait for dX
+        f[1] = go.rows(0, 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_transposed(next.qt, args.queries_t);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 next_s[s.n];
+#pragma unroll
+        for (int i = 0; i < s.n; ++i) next_s[i] = now.a_last * s.s[i];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < s.n; ++i) next_s[i] = mma(now.qt[i][c], f[c], next_s[i]);
         __syncthreads();
+        f[0] = x.rows(0, 0);
+        f[1] = x.rows(0, 32);
+        __builtin_amdgcn_sched_barrier(0);
+        next.load_transposed(next.kt, args.keys_t);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < s.n; ++i)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int c = 0; c < kChunk; c += 32) s.s[i] = mma(k.cols((wave + 4 * i) * 16, c), x.rows(0, c), s.s[i]);
+            for (int i = 0; i < s.n; ++i) next_s[i] = mma(now.kt[i][c], f[c], next_s[i]);
+#pragma unroll
+        for (int i = 0; i < s.n; ++i) s.s[i] = next_s[i];
         s.put(state);
-        __syncthreads();
+    };
+    for (int chunk = chunks - 1; chunk >= 0; chunk -= 2) {
+        step(chunk, even, odd);
+        if (chunk > 0) step(chunk - 1, odd, even);
     }
     s.save(args.grad_initial, head, args.Dk, args.Dv, col);
 }
@@ -947,7 +1116,7 @@ __device__ __forceinline__ float row_sum16(float v) {  // over the 16 lanes that
 }
 
 // QO: type of grad_q and grad_k (the storage type, or float partial gradients where value heads share a key head).
-template <typename E, typename QO, int DKP>
+template <typename E, bool WIDE, typename QO, int DKP>
 __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaArgs args) {
     using M = Mode<E>;
     constexpr int NV = kCols, KT = DKP / 32;   // tiles of 16 key columns per wavefront
@@ -993,18 +1162,20 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
     }
     const E* pv = row_of<E>(args.v, w, w.hv);
     const E* pg = row_of<E>(args.grad_o, w, w.hv);
-    Ahead<float, NV, kChunk, kPieceThreads> x_next, r_next;
-    Ahead<float, NV, DKP, kPieceThreads> s_next, ds_next;
-    Ahead<E, kChunk, NV, kPieceThreads> go_next;
+    MatrixAhead<NV, kChunk, kPieceThreads> x_next, r_next;
+    MatrixAhead<NV, DKP, kPieceThreads> s_next, ds_next;
+    Ahead<WIDE, E, kChunk, NV, kPieceThreads> go_next;
     const auto request = [&](int v0) {
-        x_next.load(args.inner + (w.at * args.cols + v0) * kChunk, kChunk, NV, kChunk, true);
-        r_next.load(args.added + (w.at * args.cols + v0) * kChunk, kChunk, NV, kChunk, true);
-        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0, args.grad_o.wide != 0);
-        s_next.load(args.states + (w.at * args.cols + v0) * DKP, DKP, NV, DKP, true);
-        ds_next.load(args.state_grads + (w.at * args.cols + v0) * DKP, DKP, NV, DKP, true);
+        x_next.load(args.inner + (w.at * args.cols + v0) * kChunk);
+        r_next.load(args.added + (w.at * args.cols + v0) * kChunk);
+        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0);
+        s_next.load(args.states + (w.at * args.cols + v0) * DKP);
+        ds_next.load(args.state_grads + (w.at * args.cols + v0) * DKP);
     };
-    load_decay(args, w, y);
+    DecayAhead y_next;
+    y_next.load(args, w.at);
     request(0);
+    y_next.store(y);
 
     f32x4 y1[KT], y2[KT], y3[KT], da[2], dp[2];
 #pragma unroll
@@ -1014,17 +1185,17 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
     float v_dot = 0.f, s_dot = 0.f;
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
-        x_next.store_values(u.c.x);
-        r_next.store_values(u.c.r);
+        x_next.store(u.c.x);
+        r_next.store(u.c.r);
         go_next.store(u.c.go);
-        s_next.store_values(u.c.s);
-        ds_next.store_values(u.c.ds);
+        s_next.store(u.c.s);
+        ds_next.store(u.c.ds);
 #pragma unroll
         for (int i = 0; i < s_next.n; ++i) {
             float a[8], b[8];
             values_of(s_next.x[i], a);
             values_of(ds_next.x[i], b);
-            if ((s_next.total % kPieceThreads == 0) || i * kPieceThreads + static_cast<int>(threadIdx.x) < s_next.total) {
+            if (s_next.mine(i)) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s_dot += a[j] * b[j];
             }
@@ -1069,9 +1240,9 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s_dot += __shfl_xor(s_dot, d);
     {
-        Ahead<E, kChunk, DKP, kPieceThreads> q_next, k_next;
-        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk, args.q.wide != 0);
-        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk, args.k.wide != 0);
+        Ahead<WIDE, E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
         __syncthreads();
         if ((threadIdx.x & 7) == 0) dot_v[threadIdx.x >> 3] = v_dot;
         if (lane == 0) inner[wave] = s_dot;
@@ -1219,28 +1390,28 @@ hipError_t delta_forward_bf16(const DeltaArgs& a, hipStream_t st);
 hipError_t delta_backward_f32(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st);
 hipError_t delta_backward_bf16(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st);
 
-template <typename E, int DKP>
+template <typename E, bool WIDE, int DKP>
 hipError_t delta_forward_as(const DeltaArgs& a, hipStream_t st) {
     const dim3 pieces(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.Hv));
     const dim3 columns(static_cast<unsigned>(a.cols / kStateCols * a.B * a.Hv));
     hipError_t err = hipSuccess;
-    if (a.chunks > 0) err = launch(delta_inverse_kernel<E, DKP>, pieces, dim3(256), st, a);
+    if (a.chunks > 0) err = launch(delta_inverse_kernel<E, WIDE, DKP>, pieces, dim3(256), st, a);
     if (err == hipSuccess) err = launch(delta_state_kernel<E, DKP>, columns, dim3(kStateThreads), st, a);
-    if (err == hipSuccess && a.chunks > 0) err = launch(delta_output_kernel<E, DKP>, pieces, dim3(kPieceThreads), st, a);
+    if (err == hipSuccess && a.chunks > 0) err = launch(delta_output_kernel<E, WIDE, DKP>, pieces, dim3(kPieceThreads), st, a);
     return err;
 }
 
 // grad_q, grad_k: where the gradients go in the end (a.grad_q and a.grad_k are partial ones where heads share keys)
-template <typename E, int DKP>
+template <typename E, bool WIDE, int DKP>
 hipError_t delta_backward_as(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st) {
     const dim3 pieces(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.Hv));
     const dim3 columns(static_cast<unsigned>(a.cols / kStateCols * a.B * a.Hv));
     hipError_t err = hipSuccess;
-    if (a.chunks > 0) err = launch(delta_inner_grad_kernel<E, DKP>, pieces, dim3(kPieceThreads), st, a);
+    if (a.chunks > 0) err = launch(delta_inner_grad_kernel<E, WIDE, DKP>, pieces, dim3(kPieceThreads), st, a);
     if (err == hipSuccess) err = launch(delta_state_grad_kernel<E, DKP>, columns, dim3(kStateThreads), st, a);
     if (err != hipSuccess || a.chunks == 0) return err;
-    if (a.Hv == a.Hk) return launch(delta_input_grad_kernel<E, E, DKP>, pieces, dim3(kPieceThreads), st, a);
-    err = launch(delta_input_grad_kernel<E, float, DKP>, pieces, dim3(kPieceThreads), st, a);
+    if (a.Hv == a.Hk) return launch(delta_input_grad_kernel<E, WIDE, E, DKP>, pieces, dim3(kPieceThreads), st, a);
+    err = launch(delta_input_grad_kernel<E, WIDE, float, DKP>, pieces, dim3(kPieceThreads), st, a);
     if (err != hipSuccess) return err;
     const int64_t rows = static_cast<int64_t>(a.T) * a.B * a.Hk;
     const int64_t blocks = ceil_div(rows * a.Dk, 256);
@@ -1249,14 +1420,21 @@ hipError_t delta_backward_as(const DeltaArgs& a, void* grad_q, void* grad_k, hip
                   static_cast<E*>(grad_k), rows, a.Dk, a.Hv / a.Hk);
 }
 
-// Keys of up to 64 values, and of up to 128.
-#define SNNSEQ_DEFINE_DELTA(NAME, E)                                                                         \
-    hipError_t delta_forward_##NAME(const DeltaArgs& a, hipStream_t st) {                                    \
-        return a.Dk <= 64 ? delta_forward_as<E, 64>(a, st) : delta_forward_as<E, 128>(a, st);                \
-    }                                                                                                        \
-    hipError_t delta_backward_##NAME(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st) {       \
-        return a.Dk <= 64 ? delta_backward_as<E, 64>(a, grad_q, grad_k, st)                                  \
-                          : delta_backward_as<E, 128>(a, grad_q, grad_k, st);                                \
+// Keys of up to 64 values and of up to 128; rows that can be read in vectors of 16 bytes, and any others.
+#define SNNSEQ_DEFINE_DELTA(NAME, E)                                                                           \
+    hipError_t delta_forward_##NAME(const DeltaArgs& a, hipStream_t st) {                                      \
+        const bool wide = a.q.wide && a.k.wide;                                                                \
+        if (a.Dk <= 64)                                                                                        \
+            return wide ? delta_forward_as<E, true, 64>(a, st) : delta_forward_as<E, false, 64>(a, st);        \
+        return wide ? delta_forward_as<E, true, 128>(a, st) : delta_forward_as<E, false, 128>(a, st);          \
+    }                                                                                                          \
+    hipError_t delta_backward_##NAME(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st) {         \
+        const bool wide = a.q.wide && a.k.wide && a.grad_o.wide;                                               \
+        if (a.Dk <= 64)                                                                                        \
+            return wide ? delta_backward_as<E, true, 64>(a, grad_q, grad_k, st)                                \
+                        : delta_backward_as<E, false, 64>(a, grad_q, grad_k, st);                              \
+        return wide ? delta_backward_as<E, true, 128>(a, grad_q, grad_k, st)                                   \
+                    : delta_backward_as<E, false, 128>(a, grad_q, grad_k, st);                                 \
     }
 
 }  // namespace snnseq

@@ -174,8 +174,9 @@ DeltaTensor tensor_of(const void* p, const int64_t* strides, int64_t D, size_t e
 
 struct Sizes {
     int64_t pieces, heads, chunks, cols, dkp;
-    size_t decay, inverse, added, states;        // bytes of what the forward leaves behind
-    size_t inner, state_grads, partial;          // of the backward's
+    size_t decay, inverse, keys, added, states;  // bytes of what the forward leaves behind (inverse and keys: twice)
+    size_t inner, state_grads, queries, partial; // of the backward's
+    size_t saved, workspace;                     // in all
 };
 
 Sizes sizes_of(const snnseq_delta* c) {
@@ -187,11 +188,15 @@ Sizes sizes_of(const snnseq_delta* c) {
     s.dkp = c->Dk <= 64 ? 64 : 128;
     const size_t n = static_cast<size_t>(s.pieces) * sizeof(float);
     s.decay = static_cast<size_t>(s.pieces) * sizeof(Decay);
-    s.inverse = static_cast<size_t>(s.pieces) *
-                (c->dtype == SNNLIF_DTYPE_F32 ? Mode<float>::square_bytes : Mode<bf16_t>::square_bytes);
+    const bool f32 = c->dtype == SNNLIF_DTYPE_F32;
+    s.inverse = static_cast<size_t>(s.pieces) * (f32 ? square_bytes<float>() : square_bytes<bf16_t>());
+    s.keys = s.queries = static_cast<size_t>(c->B * c->Hk * s.chunks) *
+                         (f32 ? keys_bytes<float>(static_cast<int>(s.dkp)) : keys_bytes<bf16_t>(static_cast<int>(s.dkp)));
     s.added = s.inner = n * kChunk * static_cast<size_t>(s.cols);
     s.states = s.state_grads = n * static_cast<size_t>(s.dkp * s.cols);
     s.partial = c->Hv == c->Hk ? 0 : round_up(static_cast<size_t>(c->T * s.heads * c->Dk) * sizeof(float), 16);
+    s.saved = s.decay + 2 * s.inverse + 2 * s.keys + s.added + s.states;
+    s.workspace = s.inner + s.state_grads + s.queries + 2 * s.partial;
     return s;
 }
 
@@ -211,8 +216,11 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved) {
     char* p = static_cast<char*>(saved);
     a.decay = reinterpret_cast<Decay*>(p);
     a.inverse = p + s.decay;
-    a.added = reinterpret_cast<float*>(p + s.decay + s.inverse);
-    a.states = reinterpret_cast<float*>(p + s.decay + s.inverse + s.added);
+    a.inverse_t = a.inverse + s.inverse;
+    a.keys = a.inverse_t + s.inverse;
+    a.keys_t = a.keys + s.keys;
+    a.added = reinterpret_cast<float*>(a.keys_t + s.keys);
+    a.states = reinterpret_cast<float*>(a.keys_t + s.keys + s.added);
     return a;
 }
 
@@ -224,7 +232,7 @@ using namespace snnseq;
 extern "C" size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call) {
     if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
     const Sizes s = sizes_of(call);
-    return s.decay + s.inverse + s.added + s.states;
+    return s.saved;
 }
 
 extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved,
@@ -238,7 +246,7 @@ extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* s
     if (!aligned_to(o, element_size(call->dtype)) || !aligned_to(state_out, 4) || !aligned_to(saved, 16))
         return SNNLIF_ERR_ALIGN;
     const Sizes s = sizes_of(call);
-    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.decay + s.inverse + s.added + s.states)) return SNNLIF_ERR_WORKSPACE;
+    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.saved)) return SNNLIF_ERR_WORKSPACE;
     DeltaArgs a = args_of(call, s, saved);
     a.o = o;
     a.state_out = state_out;
@@ -249,7 +257,7 @@ extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* s
 extern "C" size_t snnseq_gated_delta_bp_workspace_bytes(const snnseq_delta* call) {
     if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
     const Sizes s = sizes_of(call);
-    return s.inner + s.state_grads + 2 * s.partial;
+    return s.workspace;
 }
 
 extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved, size_t saved_bytes,
@@ -271,8 +279,8 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
         !aligned_to(grad_state_out, 4) || !aligned_to(saved, 16) || !aligned_to(workspace, 16))
         return SNNLIF_ERR_ALIGN;
     const Sizes s = sizes_of(call);
-    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.decay + s.inverse + s.added + s.states || workspace == nullptr ||
-                         workspace_bytes < s.inner + s.state_grads + 2 * s.partial))
+    if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.saved || workspace == nullptr ||
+                         workspace_bytes < s.workspace))
         return SNNLIF_ERR_WORKSPACE;
     DeltaArgs a = args_of(call, s, const_cast<void*>(saved));
     char* p = static_cast<char*>(workspace);
@@ -280,8 +288,9 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
     a.grad_state = grad_state_out;
     a.inner = reinterpret_cast<float*>(p);
     a.state_grads = reinterpret_cast<float*>(p + s.inner);
-    a.grad_q = s.partial ? p + s.inner + s.state_grads : grad_q;
-    a.grad_k = s.partial ? p + s.inner + s.state_grads + s.partial : grad_k;
+    a.queries_t = p + s.inner + s.state_grads;
+    a.grad_q = s.partial ? a.queries_t + s.queries : grad_q;
+    a.grad_k = s.partial ? a.queries_t + s.queries + s.partial : grad_k;
     a.grad_v = grad_v;
     a.grad_g = grad_g;
     a.grad_beta = grad_beta;
