@@ -317,6 +317,7 @@ struct DeltaArgs {
     float* state_grads;         // gradient of the state after the chunk, [cols, DKP]
     void *grad_q, *grad_k;      // [T, B, Hk, Dk] of the storage type, or fp32 [T, B, Hv, Dk] where heads share keys
     void* grad_v;               // [T, B, Hv, Dv]
+    int wide_grad_v;            // four of its values in one access
     float *grad_g, *grad_beta;  // [T, B, Hv]
     float* grad_initial;        // [B, Hv, Dk, Dv] or nullptr
 };
@@ -519,6 +520,10 @@ __device__ __forceinline__ float gap(const Decay& y, int i, int j) {  // G_ij
     return __builtin_amdgcn_exp2f(static_cast<float>(y.c[i] - y.c[j]));
 }
 
+// What a later kernel reads: the non-temporal hint.  A load waits for the stores before it, and without the hint the
+// state pass over 8192 steps of 16 heads (350 MB of matrices) took 259 us instead of 228.
+__device__ __forceinline__ void store_later(float* p, f32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(p)); }
+
 __device__ __forceinline__ f32x4 zero4() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 
 // Workgroups go to the eight XCDs in turn, each with an L2 of its own: the workgroups of a head, which read the same
@@ -695,7 +700,7 @@ struct StateTiles {
     }
     __device__ __forceinline__ void keep(float* matrix, int col) const {   // matrix [cols, DKP]
 #pragma unroll
-        for (int i = 0; i < n; ++i) *reinterpret_cast<f32x4*>(matrix + static_cast<int64_t>(col) * DKP + row(i)) = s[i];
+        for (int i = 0; i < n; ++i) store_later(matrix + static_cast<int64_t>(col) * DKP + row(i), s[i]);
     }
 };
 
@@ -806,7 +811,7 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(DeltaArgs ar
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = now.d[e] * acc[0][e];
         r.put(lc, row, out);
-        *reinterpret_cast<f32x4*>(args.added + (now.w.at * args.cols + col) * kChunk + row) = acc[0];
+        store_later(args.added + (now.w.at * args.cols + col) * kChunk + row, acc[0]);
 #pragma unroll
         for (int i = 0; i < s.n; ++i) next_s[i] = now.a_last * s.s[i];
         __syncthreads();
@@ -1071,7 +1076,7 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_grad_kernel(DeltaAr
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = -now.beta[e] * now.a[e] * acc[1][e];
         x.put(lc, row, out);
-        *reinterpret_cast<f32x4*>(args.inner + (now.w.at * args.cols + col) * kChunk + row) = acc[1];
+        store_later(args.inner + (now.w.at * args.cols + col) * kChunk + row, acc[1]);
         f[0] = go.rows(0, 0);   // does not wait for dX
         f[1] = go.rows(0, 32);
         __builtin_amdgcn_sched_barrier(0);
@@ -1122,18 +1127,18 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
     constexpr int NV = kCols, KT = DKP / 32;   // tiles of 16 key columns per wavefront
     struct Columns {
         typename M::template Fine<NV, kChunk> x, r;   // transposed, like s and ds
-        typename M::template Input<kChunk, NV> go;
+        typename M::template Input<kChunk, NV> go, v;
         typename M::template Fine<NV, DKP> s, ds;
     };
-    struct Rows {
-        typename M::template Input<kChunk, DKP> q, k;
+    struct Squares {
         typename M::template Coarse<kChunk, kChunk> m, n;
     };
-    union Shared {
+    union Shared {   // the columns are done with when M and N come
         Columns c;
-        Rows w;
+        Squares w;
         __device__ Shared() {}
     };
+    __shared__ typename M::template Input<kChunk, DKP> q_rows, k_rows;
     __shared__ Shared u;
     __shared__ Decay y;
     // sums of a row from both halves of the workgroup, of a column from every band
@@ -1164,30 +1169,39 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
     const E* pg = row_of<E>(args.grad_o, w, w.hv);
     MatrixAhead<NV, kChunk, kPieceThreads> x_next, r_next;
     MatrixAhead<NV, DKP, kPieceThreads> s_next, ds_next;
-    Ahead<WIDE, E, kChunk, NV, kPieceThreads> go_next;
+    Ahead<WIDE, E, kChunk, NV, kPieceThreads> go_next, v_next;
     const auto request = [&](int v0) {
         x_next.load(args.inner + (w.at * args.cols + v0) * kChunk);
         r_next.load(args.added + (w.at * args.cols + v0) * kChunk);
         go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0);
+        v_next.load(pv + v0, args.v.t, w.rows, args.Dv - v0);
         s_next.load(args.states + (w.at * args.cols + v0) * DKP);
         ds_next.load(args.state_grads + (w.at * args.cols + v0) * DKP);
     };
-    DecayAhead y_next;
-    y_next.load(args, w.at);
-    request(0);
-    y_next.store(y);
+    {
+        Ahead<WIDE, E, kChunk, DKP, kPieceThreads> q_next, k_next;
+        DecayAhead y_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
+        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
+        y_next.load(args, w.at);
+        request(0);
+        q_next.store(q_rows);
+        k_next.store(k_rows);
+        y_next.store(y);
+    }
 
-    f32x4 y1[KT], y2[KT], y3[KT], da[2], dp[2];
+    f32x4 y1[KT], y2[KT], y3[KT], da[2], dp[2], v_dx = zero4();
 #pragma unroll
     for (int i = 0; i < KT; ++i) y1[i] = y2[i] = y3[i] = zero4();
 #pragma unroll
     for (int i = 0; i < 2; ++i) da[i] = dp[i] = zero4();
-    float v_dot = 0.f, s_dot = 0.f;
+    float s_dot = 0.f;
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
         x_next.store(u.c.x);
         r_next.store(u.c.r);
         go_next.store(u.c.go);
+        v_next.store(u.c.v);
         s_next.store(u.c.s);
         ds_next.store(u.c.ds);
 #pragma unroll
@@ -1202,22 +1216,27 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
         }
         __syncthreads();
         if (v0 + NV < args.cols) request(v0 + NV);
-        {   // dV and v . dX: eight threads with four columns each share a row
-            const int i = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
-            if (i < present) {
+        {   // dV: eight threads with four columns each share a row
+            const int i = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4, at = v0 + c;
+            if (i < present && at < args.Dv) {
+                E* p = gv + i * row_step * args.Dv + at;
+                const float beta = y.beta[i];
+                Vec<E, 4 * sizeof(E)> out;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = v0 + c + j;
-                    if (at >= args.Dv) continue;
-                    const float dx = u.c.x.get(c + j, i);
-                    if (i < w.rows) v_dot += widen(pv[i * args.v.t + at]) * dx;
-                    gv[i * row_step * args.Dv + at] = narrow<E>(i < w.rows ? y.beta[i] * dx : 0.f);
+                for (int j = 0; j < 4; ++j) out.e[j] = narrow<E>(i < w.rows ? beta * u.c.x.get(c + j, i) : 0.f);
+                if (args.wide_grad_v) {
+                    store_vec<E, 4 * sizeof(E)>(p, out);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (at + j < args.Dv) p[j] = out.e[j];
                 }
             }
         }
         const auto fx = u.c.x.cols(band * 16, 0);
         const auto fg = u.c.go.rows(band * 16, 0);
         const auto fr = u.c.r.cols(band * 16, 0);
+        if (half == 0) v_dx = mma(u.c.v.rows(band * 16, 0), fx, v_dx);   // v . dX is its diagonal
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
             const auto fs = u.c.s.cols((half * KT + i) * 16, 0);
@@ -1233,23 +1252,15 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
                 dp[b] = mma(fg, f, dp[b]);
             }
     }
-    // v . dX over the eight threads of a row;  <S, dS'> over the workgroup
-    v_dot += __shfl_xor(v_dot, 1);
-    v_dot += __shfl_xor(v_dot, 2);
-    v_dot += __shfl_xor(v_dot, 4);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s_dot += __shfl_xor(s_dot, d);
-    {
-        Ahead<WIDE, E, kChunk, DKP, kPieceThreads> q_next, k_next;
-        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
-        k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
-        __syncthreads();
-        if ((threadIdx.x & 7) == 0) dot_v[threadIdx.x >> 3] = v_dot;
-        if (lane == 0) inner[wave] = s_dot;
-        q_next.store(u.w.q);
-        k_next.store(u.w.k);
-    }
+    for (int d = 1; d < 64; d <<= 1) s_dot += __shfl_xor(s_dot, d);   // <S, dS'>
     __syncthreads();
+    if (lane == 0) inner[wave] = s_dot;
+    if (half == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if ((lane >> 4) * 4 + e == lc) dot_v[lr + e] = v_dx[e];
+    }
 
     // M, N and the sums over their products with A and P
     float sum_beta[4] = {}, sum_c[4] = {};
@@ -1260,9 +1271,9 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
         if (block <= band) {
 #pragma unroll
             for (int s = 0; s < DKP; s += 32) {
-                const auto f = u.w.k.rows(block * 16, s);
-                kk = mma(u.w.k.rows(band * 16, s), f, kk);
-                qk = mma(u.w.q.rows(band * 16, s), f, qk);
+                const auto f = k_rows.rows(block * 16, s);
+                kk = mma(k_rows.rows(band * 16, s), f, kk);
+                qk = mma(q_rows.rows(band * 16, s), f, qk);
             }
         }
         float col = 0.f;
@@ -1291,7 +1302,7 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
             const int c = (half * KT + i) * 16 + lc;
-            const float kv = u.w.k.get(lr + e, c), qv = u.w.q.get(lr + e, c);
+            const float kv = k_rows.get(lr + e, c), qv = q_rows.get(lr + e, c);
             d1 += kv * y1[i][e];
             d2 += qv * y2[i][e];
             d3 += kv * y3[i][e];
@@ -1344,14 +1355,14 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
         }
 #pragma unroll
         for (int s = 0; s < kChunk; s += 32) {
-            const auto fk = u.w.k.cols(c0, s);
+            const auto fk = k_rows.cols(c0, s);
             if (s <= band * 16) {   // rows of this wavefront against columns up to the diagonal
                 q = mma(u.w.n.rows(band * 16, s), fk, q);
                 k = mma(u.w.m.rows(band * 16, s), fk, k);
             }
             if (s + 32 > band * 16) {
                 k = mma(u.w.m.cols(band * 16, s), fk, k);
-                k = mma(u.w.n.cols(band * 16, s), u.w.q.cols(c0, s), k);
+                k = mma(u.w.n.cols(band * 16, s), q_rows.cols(c0, s), k);
             }
         }
 #pragma unroll
@@ -1429,7 +1440,7 @@ hipError_t delta_backward_as(const DeltaArgs& a, void* grad_q, void* grad_k, hip
         return wide ? delta_forward_as<E, true, 128>(a, st) : delta_forward_as<E, false, 128>(a, st);          \
     }                                                                                                          \
     hipError_t delta_backward_##NAME(const DeltaArgs& a, void* grad_q, void* grad_k, hipStream_t st) {         \
-        const bool wide = a.q.wide && a.k.wide && a.grad_o.wide;                                               \
+        const bool wide = a.q.wide && a.k.wide && a.v.wide && a.grad_o.wide;                                   \
         if (a.Dk <= 64)                                                                                        \
             return wide ? delta_backward_as<E, true, 64>(a, grad_q, grad_k, st)                                \
                         : delta_backward_as<E, false, 64>(a, grad_q, grad_k, st);                              \
