@@ -146,10 +146,21 @@ struct TileH {
         static_assert(N == 1, "what lies in memory is one part");
         *reinterpret_cast<u32x4*>(&v[0][r * ld + c]) = x.r[0];
     }
-    __device__ __forceinline__ float get(int r, int c) const {
-        float x = value_of(v[N - 1][r * ld + c]);
+    // rows r0 + (l / 16) * 4 .. + 3 of column c0 + l % 16, the layout of a 16 x 16 product; by the transposing read
+    __device__ __forceinline__ f32x4 block(int r0, int c0) const {
+        const int lane = threadIdx.x & 63;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int part = N - 2; part >= 0; --part) x += value_of(v[part][r * ld + c]);
+        for (int part = N - 1; part >= 0; --part) {
+            const uint16_t* p = &v[part][(r0 + (lane >> 2)) * ld + c0 + (lane & 3) * 4];
+            const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(const_cast<uint16_t*>(p)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const short bits = w[e];
+                x[e] += value_of(static_cast<uint16_t>(bits));
+            }
+        }
         return x;
     }
     // operand indexed by rows r0 .., contracted over columns k0 ..
@@ -198,7 +209,13 @@ struct TileF {
         *reinterpret_cast<u32x4*>(&v[r * ld + c]) = x.r[0];
         *reinterpret_cast<u32x4*>(&v[r * ld + c + 4]) = x.r[1];
     }
-    __device__ __forceinline__ float get(int r, int c) const { return v[r * ld + c]; }
+    __device__ __forceinline__ f32x4 block(int r0, int c0) const {
+        const int lane = threadIdx.x & 63;
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = v[(r0 + (lane >> 4) * 4 + e) * ld + c0 + (lane & 15)];
+        return x;
+    }
     __device__ __forceinline__ FragF rows(int r0, int k0) const {
         const int lane = threadIdx.x & 63;
         const float* p = &v[(r0 + (lane & 15)) * ld + k0 + (lane >> 4) * 8];
@@ -1131,7 +1148,7 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
         typename M::template Fine<NV, DKP> s, ds;
     };
     struct Squares {
-        typename M::template Coarse<kChunk, kChunk> m, n;
+        typename M::template Coarse<kChunk, kChunk> m, n;   // transposed
     };
     union Shared {   // the columns are done with when M and N come
         Columns c;
@@ -1143,12 +1160,26 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
     __shared__ Decay y;
     // sums of a row from both halves of the workgroup, of a column from every band
     __shared__ float row_beta[2][kChunk], row_c[2][kChunk], row_e[2][kChunk], col_c[4][kChunk], dot_v[kChunk], inner[8];
-    const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, band = wave & 3, half = wave >> 2;
     const int lr = band * 16 + (lane >> 4) * 4, lc = lane & 15;
-    const int present = args.T - w.t0 < kChunk ? args.T - w.t0 : kChunk;
     // rows of the dense outputs: (t, b, head) of Hv heads; grad_q / grad_k per value head or, unshared, per key head
-    const int64_t row0 = static_cast<int64_t>(w.t0) * args.B * args.Hv + w.head, row_step = static_cast<int64_t>(args.B) * args.Hv;
+    const int64_t row_step = static_cast<int64_t>(args.B) * args.Hv;
+
+    MatrixAhead<NV, kChunk, kPieceThreads> x_next, r_next;
+    MatrixAhead<NV, DKP, kPieceThreads> s_next, ds_next;
+    Ahead<WIDE, E, kChunk, NV, kPieceThreads> go_next, v_next;
+    DecayAhead y_next;
+    const auto request = [&](const DeltaWhere& w, int v0) {
+        x_next.load(args.inner + (w.at * args.cols + v0) * kChunk);
+        r_next.load(args.added + (w.at * args.cols + v0) * kChunk);
+        go_next.load(row_of<E>(args.grad_o, w, w.hv) + v0, args.grad_o.t, w.rows, args.Dv - v0);
+        v_next.load(row_of<E>(args.v, w, w.hv) + v0, args.v.t, w.rows, args.Dv - v0);
+        s_next.load(args.states + (w.at * args.cols + v0) * DKP);
+        ds_next.load(args.state_grads + (w.at * args.cols + v0) * DKP);
+    };
+    const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
+    const int present = args.T - w.t0 < kChunk ? args.T - w.t0 : kChunk;
+    const int64_t row0 = static_cast<int64_t>(w.t0) * args.B * args.Hv + w.head;
     E* gv = static_cast<E*>(args.grad_v) + row0 * args.Dv;
     QO* gq = static_cast<QO*>(args.grad_q) + row0 * args.Dk;
     QO* gk = static_cast<QO*>(args.grad_k) + row0 * args.Dk;
@@ -1165,26 +1196,12 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
         }
         return;
     }
-    const E* pv = row_of<E>(args.v, w, w.hv);
-    const E* pg = row_of<E>(args.grad_o, w, w.hv);
-    MatrixAhead<NV, kChunk, kPieceThreads> x_next, r_next;
-    MatrixAhead<NV, DKP, kPieceThreads> s_next, ds_next;
-    Ahead<WIDE, E, kChunk, NV, kPieceThreads> go_next, v_next;
-    const auto request = [&](int v0) {
-        x_next.load(args.inner + (w.at * args.cols + v0) * kChunk);
-        r_next.load(args.added + (w.at * args.cols + v0) * kChunk);
-        go_next.load(pg + v0, args.grad_o.t, w.rows, args.Dv - v0);
-        v_next.load(pv + v0, args.v.t, w.rows, args.Dv - v0);
-        s_next.load(args.states + (w.at * args.cols + v0) * DKP);
-        ds_next.load(args.state_grads + (w.at * args.cols + v0) * DKP);
-    };
     {
         Ahead<WIDE, E, kChunk, DKP, kPieceThreads> q_next, k_next;
-        DecayAhead y_next;
         q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
         k_next.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
         y_next.load(args, w.at);
-        request(0);
+        request(w, 0);
         q_next.store(q_rows);
         k_next.store(k_rows);
         y_next.store(y);
@@ -1215,15 +1232,16 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
             }
         }
         __syncthreads();
-        if (v0 + NV < args.cols) request(v0 + NV);
-        {   // dV: eight threads with four columns each share a row
-            const int i = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4, at = v0 + c;
+        if (v0 + NV < args.cols) request(w, v0 + NV);
+        {   // dV: 16 rows times 16 columns per wavefront, four columns of a row per lane
+            const f32x4 dx = u.c.x.block(half * 16, band * 16);
+            const int i = band * 16 + lc, at = v0 + half * 16 + (lane >> 4) * 4;
+            const float beta = y.beta[i];
+            Vec<E, 4 * sizeof(E)> out;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out.e[j] = narrow<E>(i < w.rows ? beta * dx[j] : 0.f);
             if (i < present && at < args.Dv) {
                 E* p = gv + i * row_step * args.Dv + at;
-                const float beta = y.beta[i];
-                Vec<E, 4 * sizeof(E)> out;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) out.e[j] = narrow<E>(i < w.rows ? beta * u.c.x.get(c + j, i) : 0.f);
                 if (args.wide_grad_v) {
                     store_vec<E, 4 * sizeof(E)>(p, out);
                 } else {
@@ -1254,19 +1272,18 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) s_dot += __shfl_xor(s_dot, d);   // <S, dS'>
-    __syncthreads();
     if (lane == 0) inner[wave] = s_dot;
     if (half == 0) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if ((lane >> 4) * 4 + e == lc) dot_v[lr + e] = v_dx[e];
     }
-
+    __syncthreads();
     // M, N and the sums over their products with A and P
-    float sum_beta[4] = {}, sum_c[4] = {};
+    f32x4 sum_beta = zero4(), sum_c = zero4();
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const int block = b * 2 + half;
+        const int block = b * 2 + half, j = block * 16 + lc;
         f32x4 kk = zero4(), qk = zero4();
         if (block <= band) {
 #pragma unroll
@@ -1276,41 +1293,40 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
                 qk = mma(q_rows.rows(band * 16, s), f, qk);
             }
         }
-        float col = 0.f;
+        float col = 0.f, m4[4], n4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = lr + e, j = block * 16 + lc;
+            const int i = lr + e;
             const float decay = i >= j ? gap(y, i, j) : 0.f;
             const float a_grad = i > j ? -da[b][e] * decay : 0.f;
-            const float p_grad = i >= j ? dp[b][e] * decay * args.scale : 0.f;
-            const float m = a_grad * y.beta[i];
-            const float both = m * kk[e] + p_grad * qk[e];
+            n4[e] = i >= j ? dp[b][e] * decay * args.scale : 0.f;
+            m4[e] = a_grad * y.beta[i];
+            const float both = m4[e] * kk[e] + n4[e] * qk[e];
             sum_beta[e] += a_grad * kk[e];
             sum_c[e] += both;
             col += both;
-            u.w.m.put(i, j, m);
-            u.w.n.put(i, j, p_grad);
         }
+        u.w.m.put(j, lr, m4);
+        u.w.n.put(j, lr, n4);
         col += __shfl_xor(col, 16);
         col += __shfl_xor(col, 32);
-        if (lane < 16) col_c[band][block * 16 + lc] = col;
+        if (lane < 16) col_c[band][j] = col;
     }
     // k . Y1, q . Y2, k . Y3 by row
+    f32x4 d1 = zero4(), d2 = zero4(), d3 = zero4();
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+        const f32x4 kv = k_rows.block(band * 16, (half * KT + i) * 16), qv = q_rows.block(band * 16, (half * KT + i) * 16);
+        d1 += kv * y1[i];
+        d2 += qv * y2[i];
+        d3 += kv * y3[i];
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float d1 = 0.f, d2 = 0.f, d3 = 0.f;
-#pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            const int c = (half * KT + i) * 16 + lc;
-            const float kv = k_rows.get(lr + e, c), qv = q_rows.get(lr + e, c);
-            d1 += kv * y1[i][e];
-            d2 += qv * y2[i][e];
-            d3 += kv * y3[i][e];
-        }
         const float a = y.a[lr + e], beta = y.beta[lr + e];
-        const float rest = row_sum16(sum_c[e] - beta * a * d1 + args.scale * a * d2);
-        const float e_row = y.d[lr + e] * row_sum16(d3);
-        const float b_row = row_sum16(sum_beta[e] - a * d1);
+        const float rest = row_sum16(sum_c[e] - beta * a * d1[e] + args.scale * a * d2[e]);
+        const float e_row = y.d[lr + e] * row_sum16(d3[e]);
+        const float b_row = row_sum16(sum_beta[e] - a * d1[e]);
         if (lc == 0) {
             row_c[half][lr + e] = rest - e_row;
             row_e[half][lr + e] = e_row;
@@ -1343,37 +1359,50 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
             args.grad_beta[row0 + i * row_step] = here ? row_beta[0][i] + row_beta[1][i] + dot_v[i] : 0.f;
         }
     }
+    f32x4 a4, ad, ab;
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-        const int c0 = (half * KT + i) * 16;
-        f32x4 q, k;
+    for (int e = 0; e < 4; ++e) {
+        a4[e] = args.scale * y.a[lr + e];
+        ad[e] = y.d[lr + e];
+        ab[e] = y.beta[lr + e] * y.a[lr + e];
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = y.a[lr + e];
-            q[e] = args.scale * a * y2[i][e];
-            k[e] = y.d[lr + e] * y3[i][e] - y.beta[lr + e] * a * y1[i][e];
-        }
+    for (int i = 0; i < KT; ++i) {   // from here y2 is dQ and y1 dK
+        y2[i] = a4 * y2[i];
+        y1[i] = ad * y3[i] - ab * y1[i];
+    }
 #pragma unroll
-        for (int s = 0; s < kChunk; s += 32) {
-            const auto fk = k_rows.cols(c0, s);
-            if (s <= band * 16) {   // rows of this wavefront against columns up to the diagonal
-                q = mma(u.w.n.rows(band * 16, s), fk, q);
-                k = mma(u.w.m.rows(band * 16, s), fk, k);
-            }
-            if (s + 32 > band * 16) {
-                k = mma(u.w.m.cols(band * 16, s), fk, k);
-                k = mma(u.w.n.cols(band * 16, s), q_rows.cols(c0, s), k);
-            }
-        }
+    for (int s = 0; s < kChunk; s += 32) {
+        const bool left = s <= band * 16, below = s + 32 > band * 16;   // rows of the band end at the diagonal
+        if (left) {
+            const auto fn = u.w.n.cols(band * 16, s), fm = u.w.m.cols(band * 16, s);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int col = c0 + lc;
-            if (lr + e < present && col < args.Dk) {
-                const bool here = lr + e < w.rows;
-                gq[(lr + e) * row_step * args.Dk + col] = narrow<QO>(here ? q[e] : 0.f);
-                gk[(lr + e) * row_step * args.Dk + col] = narrow<QO>(here ? k[e] : 0.f);
+            for (int i = 0; i < KT; ++i) {
+                const auto fk = k_rows.cols((half * KT + i) * 16, s);
+                y2[i] = mma(fn, fk, y2[i]);
+                y1[i] = mma(fm, fk, y1[i]);
             }
         }
+        if (below) {
+            const auto fn = u.w.n.rows(band * 16, s), fm = u.w.m.rows(band * 16, s);
+#pragma unroll
+            for (int i = 0; i < KT; ++i) {
+                y1[i] = mma(fm, k_rows.cols((half * KT + i) * 16, s), y1[i]);
+                y1[i] = mma(fn, q_rows.cols((half * KT + i) * 16, s), y1[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (lr + e >= present) continue;
+        QO *pq = gq + (lr + e) * row_step * args.Dk + half * KT * 16 + lc, *pk = gk + (lr + e) * row_step * args.Dk + half * KT * 16 + lc;
+        const bool here = lr + e < w.rows;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+            if ((half * KT + i) * 16 + lc < args.Dk) {
+                pq[i * 16] = narrow<QO>(here ? y2[i][e] : 0.f);
+                pk[i * 16] = narrow<QO>(here ? y1[i][e] : 0.f);
+            }
     }
 }
 
