@@ -114,13 +114,15 @@ typedef struct snnseq_delta {
     int dtype;
 } snnseq_delta;
 
-/* Bytes the forward writes for the backward: per chunk of 64 steps and value head the fp32 state before it, the rows
- * added to it and a 64 x 64 matrix.  A caller that wants no backward passes the same memory as scratch.  0 for invalid arguments. */
-size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call);
+/* Bytes of device memory (`saved`) the forward works in.  for_backward != 0: and leaves behind for the backward, per
+ * chunk of 64 steps and value head the fp32 state before it, the rows added to it and 64 x 64 matrices, per key head the
+ * keys.  for_backward == 0: scratch, smaller.  0 for invalid arguments. */
+size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call, int for_backward);
 
-/* o dense [T, B, Hv, Dv]; state_out [B, Hv, Dk, Dv] (may be NULL): the state after the last step. */
+/* o dense [T, B, Hv, Dv]; state_out [B, Hv, Dk, Dv] (may be NULL): the state after the last step.  o and state_out do not
+ * depend on for_backward by a bit. */
 int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved, size_t saved_bytes,
-                          void* stream);
+                          int for_backward, void* stream);
 
 size_t snnseq_gated_delta_bp_workspace_bytes(const snnseq_delta* call);
 

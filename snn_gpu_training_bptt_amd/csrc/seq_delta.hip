@@ -179,7 +179,7 @@ struct Sizes {
     size_t saved, workspace;                     // in all
 };
 
-Sizes sizes_of(const snnseq_delta* c) {
+Sizes sizes_of(const snnseq_delta* c, bool for_backward) {
     Sizes s;
     s.chunks = ceil_div(c->T, kChunk);
     s.heads = c->B * c->Hv;
@@ -195,12 +195,12 @@ Sizes sizes_of(const snnseq_delta* c) {
     s.added = s.inner = n * kChunk * static_cast<size_t>(s.cols);
     s.states = s.state_grads = n * static_cast<size_t>(s.dkp * s.cols);
     s.partial = c->Hv == c->Hk ? 0 : round_up(static_cast<size_t>(c->T * s.heads * c->Dk) * sizeof(float), 16);
-    s.saved = s.decay + 2 * s.inverse + 2 * s.keys + s.added + s.states;
+    s.saved = s.decay + (for_backward ? 2 : 1) * s.inverse + 2 * s.keys + s.added + s.states;
     s.workspace = s.inner + s.state_grads + s.queries + 2 * s.partial;
     return s;
 }
 
-DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved) {
+DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved, bool for_backward) {
     const size_t es = element_size(c->dtype);
     DeltaArgs a{};
     a.T = static_cast<int>(c->T); a.B = static_cast<int>(c->B);
@@ -216,8 +216,8 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved) {
     char* p = static_cast<char*>(saved);
     a.decay = reinterpret_cast<Decay*>(p);
     a.inverse = p + s.decay;
-    a.inverse_t = a.inverse + s.inverse;
-    a.keys = a.inverse_t + s.inverse;
+    a.inverse_t = for_backward ? a.inverse + s.inverse : nullptr;
+    a.keys = a.inverse + (for_backward ? 2 : 1) * s.inverse;
     a.keys_t = a.keys + s.keys;
     a.added = reinterpret_cast<float*>(a.keys_t + s.keys);
     a.states = reinterpret_cast<float*>(a.keys_t + s.keys + s.added);
@@ -229,14 +229,13 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved) {
 
 using namespace snnseq;
 
-extern "C" size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call) {
+extern "C" size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call, int for_backward) {
     if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
-    const Sizes s = sizes_of(call);
-    return s.saved;
+    return sizes_of(call, for_backward != 0).saved;
 }
 
 extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved,
-                                     size_t saved_bytes, void* stream) {
+                                     size_t saved_bytes, int for_backward, void* stream) {
     const int bad = delta_error(call);
     if (bad != SNNLIF_OK) return bad;
     if (empty(call)) return SNNLIF_OK;
@@ -245,9 +244,9 @@ extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* s
     if (call->T > 0 && o == nullptr) return SNNLIF_ERR_ARG;
     if (!aligned_to(o, element_size(call->dtype)) || !aligned_to(state_out, 4) || !aligned_to(saved, 16))
         return SNNLIF_ERR_ALIGN;
-    const Sizes s = sizes_of(call);
+    const Sizes s = sizes_of(call, for_backward != 0);
     if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.saved)) return SNNLIF_ERR_WORKSPACE;
-    DeltaArgs a = args_of(call, s, saved);
+    DeltaArgs a = args_of(call, s, saved, for_backward != 0);
     a.o = o;
     a.state_out = state_out;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -256,8 +255,7 @@ extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* s
 
 extern "C" size_t snnseq_gated_delta_bp_workspace_bytes(const snnseq_delta* call) {
     if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
-    const Sizes s = sizes_of(call);
-    return s.workspace;
+    return sizes_of(call, true).workspace;
 }
 
 extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved, size_t saved_bytes,
@@ -278,11 +276,11 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
         !aligned_to(grad_g, 4) || !aligned_to(grad_beta, 4) || !aligned_to(grad_state, 4) ||
         !aligned_to(grad_state_out, 4) || !aligned_to(saved, 16) || !aligned_to(workspace, 16))
         return SNNLIF_ERR_ALIGN;
-    const Sizes s = sizes_of(call);
+    const Sizes s = sizes_of(call, true);
     if (s.pieces > 0 && (saved == nullptr || saved_bytes < s.saved || workspace == nullptr ||
                          workspace_bytes < s.workspace))
         return SNNLIF_ERR_WORKSPACE;
-    DeltaArgs a = args_of(call, s, const_cast<void*>(saved));
+    DeltaArgs a = args_of(call, s, const_cast<void*>(saved), true);
     char* p = static_cast<char*>(workspace);
     a.grad_o = tensor_of(grad_o, grad_o_strides, call->Dv, es);
     a.grad_state = grad_state_out;

@@ -4,7 +4,7 @@
 //   embed_bp(tokens, grad_out, vocab, scale) -> grad_weight
 //   gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act) -> [mean, rstd, y]
 //   gn_act_bp(x, weight_gn, bias_gn, mean, rstd, groups, act, grad_y) -> [grad_x, grad_weight_gn, grad_bias_gn]
-//   gated_delta_fp(q, k, v, g, beta, state, lengths, scale) -> [o, state_out, saved]
+//   gated_delta_fp(q, k, v, g, beta, state, lengths, scale, for_backward) -> [o, state_out, saved]
 //   gated_delta_bp(q, k, v, g, beta, state, lengths, scale, saved, grad_o, grad_state_out)
 //                  -> [grad_q, grad_k, grad_v, grad_g, grad_beta, grad_state]
 //   gated_delta_step(q, k, v, g, beta, state, scale, state_out) -> o
@@ -308,18 +308,19 @@ DeltaOperands delta_operands(const Tensor& q, const Tensor& k, const Tensor& v, 
 }
 
 std::vector<Tensor> gated_delta_fp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, MaybeTensor state,
-                                   MaybeTensor lengths, double scale) {
+                                   MaybeTensor lengths, double scale, bool for_backward) {
     const char* op = "gated_delta_fp";
     check_on_gpu(q, op, "q");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
     Tensor o = torch::empty(v.sizes(), v.options());
     Tensor state_out = torch::empty({d.call.B, d.call.Hv, d.call.Dk, d.call.Dv}, d.g.options());
-    const size_t bytes = snnseq_gated_delta_saved_bytes(&d.call);
+    const size_t bytes = snnseq_gated_delta_saved_bytes(&d.call, for_backward);
     Tensor saved = workspace_of(bytes, o);
     check_rc(snnseq_gated_delta_fp(&d.call, o.data_ptr(), state_out.data_ptr<float>(), saved.data_ptr(), bytes,
-                                   current_stream()),
+                                   for_backward, current_stream()),
              op);
+    if (!for_backward) saved = Tensor();
     return {o, state_out, saved};
 }
 
@@ -333,9 +334,9 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
     check_like(grad_o, q, op, "grad_o", "q");
     TORCH_CHECK(grad_o.sizes() == v.sizes(), "snnlib.", op, ": grad_o ", grad_o.sizes(), " and v ", v.sizes(),
                 " must have the same shape");
-    TORCH_CHECK(saved.is_cuda() && saved.device() == q.device() && saved.scalar_type() == at::kByte &&
+    TORCH_CHECK(saved.defined() && saved.is_cuda() && saved.device() == q.device() && saved.scalar_type() == at::kByte &&
                     saved.is_contiguous() &&
-                    static_cast<size_t>(saved.numel()) == snnseq_gated_delta_saved_bytes(&d.call),
+                    static_cast<size_t>(saved.numel()) == snnseq_gated_delta_saved_bytes(&d.call, 1),
                 "snnlib.", op, ": saved must be what gated_delta_fp returned for these operands");
     Tensor go = dense_rows(grad_o), gs;
     if (grad_state_out.has_value() && grad_state_out->defined()) {
@@ -395,7 +396,9 @@ void bind_token_layers(pybind11::module_& m) {
     m.def("embed_bp", &embed_bp, "gradient of the embedding table, by sorted tokens");
     m.def("gn_act_fp", &gn_act_fp, "group norm with an activation, channels last: [mean, rstd, y]");
     m.def("gn_act_bp", &gn_act_bp, "its backward: [grad_x, grad_weight_gn, grad_bias_gn]");
-    m.def("gated_delta_fp", &gated_delta_fp, "gated delta rule over a sequence: [o, state_out, saved]");
+    m.def("gated_delta_fp", &gated_delta_fp, "gated delta rule over a sequence: [o, state_out, saved]",
+          pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("g"), pybind11::arg("beta"),
+          pybind11::arg("state"), pybind11::arg("lengths"), pybind11::arg("scale"), pybind11::arg("for_backward") = true);
     m.def("gated_delta_bp", &gated_delta_bp, "its backward: [grad_q, grad_k, grad_v, grad_g, grad_beta, grad_state]");
     m.def("gated_delta_step", &gated_delta_step, "gated delta rule, one time step: o, the state updated");
 }

@@ -8,6 +8,10 @@ Same surface as the reference's ``snnlib_func.py`` for every single-GPU layer
 ``BnFireFcDistFunc`` :297-327, ``BnFireConvDistFunc`` :336-377, whose backward runs the native op in
 two halves with ``torch.distributed.all_reduce`` of two ``[C]`` vectors between them.
 
+The token layers -- ``EmbedFunc``, ``GnActFunc``, ``GatedDeltaFunc`` with ``embed_func``, ``gn_act_func``,
+``gated_delta_func`` and ``gated_delta_step`` -- extend the set to networks over token sequences on the same
+time axis; the reference has no counterpart.
+
 Contract shared by all of them, as in the reference: a forward saves only its *inputs* (plus the
 per-channel inverse standard deviation a batch-norm forward returns) -- never spikes or membrane
 potentials -- and calls the native ``snnlib.<op>_fp``; the backward calls ``snnlib.<op>_bp``, which
@@ -383,7 +387,7 @@ def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
         scale = q.shape[-1] ** -0.5
     if _records(q, k, v, g, beta, state):
         return GatedDeltaFunc.apply(q, k, v, g, beta, state, lengths, scale)
-    return tuple(snnlib.gated_delta_fp(q, k, v, g, beta, state, lengths, scale)[:2])
+    return tuple(snnlib.gated_delta_fp(q, k, v, g, beta, state, lengths, scale, False)[:2])
 
 
 def gated_delta_step(q, k, v, g, beta, state, scale=None, state_out=None):

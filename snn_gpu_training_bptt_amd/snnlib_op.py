@@ -15,6 +15,9 @@ reference takes from ``torch.var_mean(..., unbiased=False)`` and this build from
 kernel, ``snnlib.bn_stats``) or the running ones; the running statistics are ``nn.Parameter`` objects that are
 *replaced* on every training-mode call (momentum 0.1, variance corrected by n/(n-1), n = elements
 per channel of the first input seen).
+
+``Embed``, ``GnAct`` and ``GatedDelta`` are layers over token sequences, ``[T, B, ...]`` like the others; the reference
+has no counterpart.
 """
 import math
 
@@ -267,3 +270,45 @@ class BnFireConvDist(_ShardedBatchStatistics):
         return sf.bn_fire_conv_dist_func(x, self.weight_bn, self.bias_bn, var, mean, self.eps_bn,
                                          self.weight_conv, self.bias_conv, self.stride, self.padding,
                                          self.if_bias_conv, self._reduce_op())
+
+
+class Embed(nn.Module):
+    """``[T, B]`` integer tokens to ``[T, B, cout]``: rows of a table times ``scale``.  A token outside the table (-1,
+    say, behind the end of a sequence) gives a row of zeros and no gradient."""
+
+    def __init__(self, vocab, cout, scale=1.0):
+        super(Embed, self).__init__()
+        self.scale = scale
+        self.weight_embed = nn.Parameter(nn.init.normal_(torch.zeros(vocab, cout), 0, 1 / math.sqrt(cout)))
+
+    def forward(self, tokens):
+        return sf.embed_func(tokens, self.weight_embed, self.scale)
+
+
+class GnAct(nn.Module):
+    """Group norm over the ``cin`` channels of the last axis, per time step and batch entry (no statistics of
+    the batch, so nothing to all-reduce and nothing to keep running), then ``act``: "none", "relu", "silu" or "gelu"."""
+
+    def __init__(self, groups, cin, eps_gn=1e-5, act="silu"):
+        super(GnAct, self).__init__()
+        self.groups, self.eps_gn, self.act = groups, eps_gn, act
+        self.weight_gn = nn.Parameter(torch.ones(cin))
+        self.bias_gn = nn.Parameter(torch.zeros(cin))
+
+    def forward(self, x):
+        return sf.gn_act_func(x, self.weight_gn, self.bias_gn, self.groups, self.eps_gn, self.act)
+
+
+class GatedDelta(nn.Module):
+    """The gated delta rule: a leaky memory over time like ``Fire``'s membrane, but a matrix that is written by keys and
+    read by queries (``sf.gated_delta_func``).  ``forward`` takes a whole sequence, ``step`` one time step of generation."""
+
+    def __init__(self, scale=None):
+        super(GatedDelta, self).__init__()
+        self.scale = scale
+
+    def forward(self, q, k, v, g, beta, state=None, lengths=None):
+        return sf.gated_delta_func(q, k, v, g, beta, state, lengths, self.scale)
+
+    def step(self, q, k, v, g, beta, state, state_out=None):
+        return sf.gated_delta_step(q, k, v, g, beta, state, self.scale, state_out)
