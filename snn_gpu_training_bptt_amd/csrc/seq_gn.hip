@@ -22,7 +22,9 @@
 namespace snnseq {
 namespace {
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
+// Two instructions, off by a unit in the last place and |v| * 2^-24: that of v's own rounding.  The library's exponential,
+// four times as many, made the norm of bf16 tokens bound by arithmetic.
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 __device__ __forceinline__ float erf_of(float v) { return erff(v); }
 __device__ __forceinline__ double erf_of(double v) { return erf(v); }
@@ -68,60 +70,75 @@ __device__ __forceinline__ A lanes_sum(A v, int lanes) {
 
 constexpr int kRowsBlock = 256;
 
-template <typename E, int BYTES, int K>
+// U items (sample, group), `step` apart, per group of L lanes: all of them requested before the first is looked at.
+// `step` is a multiple of G, so that they share their channels' weights.
+template <typename E, int BYTES, int K, int U>
 __global__ void __launch_bounds__(kRowsBlock)
 gn_rows_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                        E* __restrict__ y, arith_t<E>* __restrict__ mean, arith_t<E>* __restrict__ rstd, int64_t items,
-                       int G, int cpg, arith_t<E> eps, int act, int lanes_log2) {
+                       int64_t step, int G, int cpg, arith_t<E> eps, int act, int lanes_log2) {
     using A = arith_t<E>;
     constexpr int n = Vec<E, BYTES>::n;
     const int L = 1 << lanes_log2;
     const int lane = threadIdx.x & (L - 1);
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * (kRowsBlock >> lanes_log2) + (threadIdx.x >> lanes_log2);
-    if (item >= items) return;  // whole groups of lanes
-    const int g = static_cast<int>(item % G);
-    const E* px = x + item * cpg;
-    Vec<E, BYTES> v[K], w[K], b[K];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kRowsBlock >> lanes_log2) + (threadIdx.x >> lanes_log2);
+    if (first >= step) return;  // whole groups of lanes
+    const int g = static_cast<int>(first % G);
+    Vec<E, BYTES> v[U][K], w[K], b[K];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * L + lane) * n;
+            const int64_t item = first + u * step;
+            v[u][k].raw = typename Vec<E, BYTES>::raw_t(0);
+            if (c < cpg && item < items) v[u][k] = load_vec_once<E, BYTES>(x + item * cpg + c);
+        }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * L + lane) * n;
-        v[k].raw = w[k].raw = b[k].raw = typename Vec<E, BYTES>::raw_t(0);
+        w[k].raw = b[k].raw = typename Vec<E, BYTES>::raw_t(0);
         if (c < cpg) {
-            v[k] = load_vec_once<E, BYTES>(px + c);
             w[k] = load_vec<E, BYTES>(weight + g * cpg + c);
             b[k] = load_vec<E, BYTES>(bias + g * cpg + c);
         }
     }
-    A sum = A(0);
+    const A per = A(1) / A(cpg);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int u = 0; u < U; ++u) {
+        const int64_t item = first + u * step;
+        if (item >= items) return;
+        A sum = A(0);
 #pragma unroll
-        for (int j = 0; j < n; ++j) sum += widen(v[k].e[j]);  // absent values are zero
-    const A m = lanes_sum(sum, L) / A(cpg);
-    A sq = A(0);
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-        if ((k * L + lane) * n < cpg) {
+            for (int j = 0; j < n; ++j) sum += widen(v[u][k].e[j]);  // absent values are zero
+        const A m = lanes_sum(sum, L) * per;
+        A sq = A(0);
 #pragma unroll
-            for (int j = 0; j < n; ++j) {
-                const A d = widen(v[k].e[j]) - m;
-                sq += d * d;
+        for (int k = 0; k < K; ++k)
+            if ((k * L + lane) * n < cpg) {
+#pragma unroll
+                for (int j = 0; j < n; ++j) {
+                    const A d = widen(v[u][k].e[j]) - m;
+                    sq += d * d;
+                }
             }
+        const A r = inverse_root(lanes_sum(sq, L) * per + eps);
+        if (lane == 0) {
+            mean[item] = m;
+            rstd[item] = r;
         }
-    const A r = inverse_root(lanes_sum(sq, L) / A(cpg) + eps);
-    if (lane == 0) {
-        mean[item] = m;
-        rstd[item] = r;
-    }
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int c = (k * L + lane) * n;
-        if (c >= cpg) continue;
-        Vec<E, BYTES> o;
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * L + lane) * n;
+            if (c >= cpg) continue;
+            Vec<E, BYTES> o;
 #pragma unroll
-        for (int j = 0; j < n; ++j)
-            o.e[j] = narrow<E>(act_value((widen(v[k].e[j]) - m) * r * widen(w[k].e[j]) + widen(b[k].e[j]), act));
-        store_vec<E, BYTES>(y + item * cpg + c, o);
+            for (int j = 0; j < n; ++j)
+                o.e[j] = narrow<E>(act_value((widen(v[u][k].e[j]) - m) * r * widen(w[k].e[j]) + widen(b[k].e[j]), act));
+            store_vec<E, BYTES>(y + item * cpg + c, o);
+        }
     }
 }
 
@@ -154,20 +171,35 @@ gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
                 b[k] = load_vec<E, BYTES>(bias + g * cpg + c);
             }
         }
-        for (int64_t s = static_cast<int64_t>(blockIdx.x) * spb + sample; s < S;
-             s += static_cast<int64_t>(gridDim.x) * spb) {
+        const int64_t hop = static_cast<int64_t>(gridDim.x) * spb;
+        int64_t s = static_cast<int64_t>(blockIdx.x) * spb + sample;
+        Vec<E, BYTES> v_next[K], d_next[K];
+        A m_next = A(0), r_next = A(0);
+        const auto request = [&](int64_t at) {   // the sample after this one is under way while this one is worked on
+            const int64_t item = (at < S ? at : s) * G + g;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * L + lane) * n;
+                v_next[k].raw = d_next[k].raw = typename Vec<E, BYTES>::raw_t(0);
+                if (c < cpg) {
+                    v_next[k] = load_vec_once<E, BYTES>(x + item * cpg + c);
+                    d_next[k] = load_vec_once<E, BYTES>(grad + item * cpg + c);
+                }
+            }
+            m_next = mean[item];
+            r_next = rstd[item];
+        };
+        if (s < S) request(s);
+        for (; s < S; s += hop) {
             const int64_t item = s * G + g;
             Vec<E, BYTES> v[K], d[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (k * L + lane) * n;
-                v[k].raw = d[k].raw = typename Vec<E, BYTES>::raw_t(0);
-                if (c < cpg) {
-                    v[k] = load_vec_once<E, BYTES>(x + item * cpg + c);
-                    d[k] = load_vec_once<E, BYTES>(grad + item * cpg + c);
-                }
+                v[k] = v_next[k];
+                d[k] = d_next[k];
             }
-            const A m = mean[item], r = rstd[item];
+            const A m = m_next, r = r_next;
+            request(s + hop);
             A gz[K * n], c1 = A(0), c2 = A(0);
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -245,11 +277,13 @@ gn_parameters_kernel(const arith_t<E>* __restrict__ part, E* __restrict__ grad_w
 // ---- slab ---------------------------------------------------------------------------------------
 
 // Values a thread holds of each input: 32 (64 registers of x and grad_y), half as many where a thread of a
-// 1024-thread workgroup, limited to 128 registers, holds both inputs, and half as many doubles; in at most 16 vectors.
+// 1024-thread workgroup, limited to 128 registers, holds both inputs, and half as many doubles; in at most 16 vectors
+// (8 there), each of which costs an address.
 constexpr int held_vectors(int element_bytes, int vector_values, int block, bool backward) {
-    const int values = (element_bytes == 8 ? 16 : 32) / (backward && block == 1024 ? 2 : 1);
+    const bool tight = backward && block == 1024;
+    const int values = (element_bytes == 8 ? 16 : 32) / (tight ? 2 : 1), most = tight ? 8 : 16;
     const int k = values / vector_values;
-    return k > 16 ? 16 : k;
+    return k > most ? most : k;
 }
 
 // Workgroups go to the eight XCDs in turn, each with an L2 of its own: consecutive pieces of work are given to one
@@ -392,23 +426,29 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
         b = load_vec<E, BYTES>(bias + c);
     }
     A total_a[n] = {}, total_b[n] = {};
-    for (int64_t s = slice; s < S; s += slices) {
+    Vec<E, BYTES> v[K], d[K];
+    A m_next = A(0), r_next = A(0);
+    // The one workgroup of 1024 threads that a CU holds requests a sample while the one before is summed up and stored
+    // ([8 64 32 32 128] fp32: 267 us, 301 without); smaller ones overlap each other, and the registers are theirs.
+    // What does not exist is read at the slab's beginning and left out below.
+    constexpr bool kRequestAhead = BT == 1024 && sizeof(E) == 4;
+    const auto request = [&](int64_t s) {
         const E *px = x + s * P * C, *pg = grad + s * P * C;
-        Vec<E, BYTES> v[K], d[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int p = t.row + k * t.rows;
-            v[k].raw = d[k].raw = typename Vec<E, BYTES>::raw_t(0);
-            if (t.here && p < P) {
-                v[k] = load_vec_once<E, BYTES>(px + static_cast<uint32_t>(p * C + c));
-                d[k] = load_vec_once<E, BYTES>(pg + static_cast<uint32_t>(p * C + c));
-            }
+            const uint32_t at = t.here && p < P ? static_cast<uint32_t>(p * C + c) : 0u;
+            v[k] = load_vec<E, BYTES>(px + at);
+            d[k] = load_vec<E, BYTES>(pg + at);
         }
-        A m = A(0), r = A(0);
-        if (t.here) {
-            m = mean[s * G + t.first_group + t.group];
-            r = rstd[s * G + t.first_group + t.group];
-        }
+        const int64_t item = s * G + (t.here ? t.first_group + t.group : 0);
+        m_next = mean[item];
+        r_next = rstd[item];
+    };
+    if (kRequestAhead && slice < S) request(slice);
+    for (int64_t s = slice; s < S; s += slices) {
+        if (!kRequestAhead) request(s);
+        const A m = m_next, r = r_next;
         // xhat and gz take the registers of x and grad_y: 64 at most, within the 128 of a 1024-thread workgroup
         A xh[K * n], gz[K * n], acc_a[n] = {}, acc_b[n] = {};
 #pragma unroll
@@ -425,6 +465,7 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
                 acc_b[j] += valid ? q : A(0);
             }
         }
+        if (kRequestAhead) request(s + slices < S ? s + slices : s);
         __syncthreads();  // the sums of the sample before have been read
 #pragma unroll
         for (int j = 0; j < n; ++j) {
@@ -734,9 +775,10 @@ Plan plan_of(int dtype, int vec_bytes, int64_t S, int64_t P, int64_t C, int64_t 
         p.part_rows = wanted < most ? wanted : most;
     } else {
         p.way = Way::split;
-        // 1024 threads only where 256 cannot hold the slab: more workgroups per CU overlap loads with stores
-        for (int64_t segment = 128; segment >= 64 && p.way == Way::split && P * C * es < (int64_t(1) << 31);
-             segment >>= 1) {
+        // 1024 threads only where 256 cannot hold the slab: more workgroups per CU overlap loads with stores.  Segments
+        // of 32 bytes, which 256 threads could hold, cost twice the time ([8 64 32 32 128] fp32: backward 475 us against 276)
+        const bool small_sample = P * C * es < (int64_t(1) << 31);
+        for (int64_t segment = 128; segment >= 64 && p.way == Way::split && small_sample; segment >>= 1) {
             int64_t gpb = ceil_div(segment, cpg * es);
             gpb = gpb < G ? gpb : G;
             const int64_t cols = gpb * vpg;
@@ -750,7 +792,6 @@ Plan plan_of(int dtype, int vec_bytes, int64_t S, int64_t P, int64_t C, int64_t 
                 p.bundles = static_cast<int>(ceil_div(G, gpb));
                 break;
             }
-            if (gpb == G && cpg * es * G < segment) break;
         }
         if (p.way == Way::slab) {
             const int64_t wanted = ceil_div(p.block == 256 ? 2048 : 512, p.bundles);
@@ -788,15 +829,23 @@ struct Call {
     hipStream_t stream;
 };
 
+template <typename E, int BYTES, int K, int U>
+hipError_t rows_forward_by(const Call& a, const Plan& p) {
+    using A = arith_t<E>;
+    const int64_t items = a.S * a.G, step = ceil_div(a.S, U) * a.G;
+    return launch(gn_rows_forward_kernel<E, BYTES, K, U>,
+                  dim3(static_cast<unsigned>(ceil_div(step, kRowsBlock >> p.lanes_log2))), dim3(kRowsBlock), a.stream,
+                  static_cast<const E*>(a.x), static_cast<const E*>(a.weight), static_cast<const E*>(a.bias),
+                  static_cast<E*>(a.out), static_cast<A*>(a.mean_out), static_cast<A*>(a.rstd_out), items, step,
+                  static_cast<int>(a.G), static_cast<int>(a.C / a.G), static_cast<A>(a.eps), a.act, p.lanes_log2);
+}
+
 template <typename E, int BYTES, int K>
 hipError_t rows_forward(const Call& a, const Plan& p) {
-    using A = arith_t<E>;
-    const int64_t items = a.S * a.G;
-    return launch(gn_rows_forward_kernel<E, BYTES, K>,
-                  dim3(static_cast<unsigned>(ceil_div(items, kRowsBlock >> p.lanes_log2))), dim3(kRowsBlock), a.stream,
-                  static_cast<const E*>(a.x), static_cast<const E*>(a.weight), static_cast<const E*>(a.bias),
-                  static_cast<E*>(a.out), static_cast<A*>(a.mean_out), static_cast<A*>(a.rstd_out), items,
-                  static_cast<int>(a.G), static_cast<int>(a.C / a.G), static_cast<A>(a.eps), a.act, p.lanes_log2);
+    // four samples per group of lanes where that leaves eight workgroups for every CU: more requests in flight
+    // ([16384, 8 groups of 128] bf16 silu: 21.5 us); fewer samples want the workgroups
+    if (K == 1 && a.S * a.G >= int64_t(4) * 8 * 256 * (kRowsBlock >> p.lanes_log2)) return rows_forward_by<E, BYTES, K, 4>(a, p);
+    return rows_forward_by<E, BYTES, K, 1>(a, p);
 }
 
 template <typename E, int BYTES, int K>
