@@ -9,10 +9,16 @@
 //                  -> [grad_q, grad_k, grad_v, grad_g, grad_beta, grad_state]
 //   gated_delta_step(q, k, v, g, beta, state, scale, state_out) -> o
 //
+// and, differentiable, embed(tokens, weight, scale), gn_act(x, weight_gn, bias_gn, groups, eps_gn, act) and
+// gated_delta(q, k, v, g, beta, state, lengths, scale) -> (o, state_out).  Their autograd functions are here and not in
+// Python, unlike the fire layers': on a few thousand tokens the kernels of a forward and backward are over in 20 us, and
+// two Python frames and the wait for the interpreter in the backward's thread took 30 us more than these do.
+//
 // As in snnlib_ext.cpp: this file validates tensors, allocates outputs and workspaces and forwards raw device
 // pointers to the C ABI (include/snnlib_seq.h) on the current stream of the tensors' device; it holds no device
 // code and no fallback.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -216,6 +222,8 @@ std::vector<Tensor> gn_act_bp(Tensor x, Tensor weight_gn, Tensor bias_gn, Tensor
     return {grad_x, grad_weight, grad_bias};
 }
 
+bool records(std::initializer_list<const Tensor*> tensors);   // whether autograd would record an operator on these
+
 // ---- gated delta rule ---------------------------------------------------------------------------
 
 using MaybeTensor = c10::optional<Tensor>;
@@ -369,6 +377,8 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
 Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor state, double scale,
                         MaybeTensor state_out) {
     const char* op = "gated_delta_step";
+    TORCH_CHECK(!records({&q, &k, &v, &g, &beta, &state}), "snnlib.", op, ": a step is not differentiable: call it with "
+                "gradients off, or use gated_delta");
     check_on_gpu(q, op, "q");
     check_on_gpu(state, op, "state");
     const DeviceGuard guard(q.device());
@@ -388,10 +398,122 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Ten
     return o;
 }
 
+// ---- autograd -----------------------------------------------------------------------------------
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool records(std::initializer_list<const Tensor*> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// Gradients come from kernels autograd knows nothing of: differentiating them in turn is an error, not a zero.
+variable_list differentiable_once(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list defined;
+    for (const Tensor& g : grads)
+        if (g.defined()) {
+            defined.push_back(g.detach());
+            defined.back().set_requires_grad(true);
+        }
+    const auto error = std::make_shared<torch::autograd::DelayedError>(
+        "the gradients of the token layers cannot be differentiated again", static_cast<int64_t>(defined.size()));
+    const variable_list out = (*error)(std::move(defined));
+    size_t next = 0;
+    for (Tensor& g : grads)
+        if (g.defined()) g = out[next++];
+    return grads;
+}
+
+struct EmbedFunction : torch::autograd::Function<EmbedFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& weight, double scale) {
+        Tensor out = embed_fp(tokens, weight, scale);
+        ctx->save_for_backward({tokens});
+        ctx->saved_data["vocab"] = weight.size(0);
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor tokens = ctx->get_saved_variables()[0];
+        return differentiable_once({Tensor(), embed_bp(tokens, grads[0], ctx->saved_data["vocab"].toInt(),
+                                                       ctx->saved_data["scale"].toDouble()),
+                                    Tensor()});
+    }
+};
+
+Tensor embed(const Tensor& tokens, const Tensor& weight, double scale) {
+    return records({&weight}) ? EmbedFunction::apply(tokens, weight, scale) : embed_fp(tokens, weight, scale);
+}
+
+struct GnActFunction : torch::autograd::Function<GnActFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight_gn, const Tensor& bias_gn,
+                          int64_t groups, double eps_gn, const std::string& act) {
+        std::vector<Tensor> r = gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act);
+        ctx->save_for_backward({x, weight_gn, bias_gn, r[0], r[1]});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        return r[2];
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const std::vector<Tensor> g = gn_act_bp(s[0], s[1], s[2], s[3], s[4], ctx->saved_data["groups"].toInt(),
+                                                ctx->saved_data["act"].toStringRef(), grads[0]);
+        return differentiable_once({g[0], g[1], g[2], Tensor(), Tensor(), Tensor()});
+    }
+};
+
+Tensor gn_act(const Tensor& x, const Tensor& weight_gn, const Tensor& bias_gn, int64_t groups, double eps_gn,
+              const std::string& act) {
+    if (records({&x, &weight_gn, &bias_gn})) return GnActFunction::apply(x, weight_gn, bias_gn, groups, eps_gn, act);
+    return gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act)[2];
+}
+
+// Unlike the fire layers this one keeps what its forward computed on the way -- the state before every chunk of 64 steps
+// and the rows added to it: the state passes are bound by latency, running the forward's again would cost a third
+// of the backward, and the memory is there.
+struct GatedDeltaFunction : torch::autograd::Function<GatedDeltaFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                 const Tensor& beta, const MaybeTensor& state, const MaybeTensor& lengths, double scale) {
+        ctx->set_materialize_grads(false);
+        std::vector<Tensor> r = gated_delta_fp(q, k, v, g, beta, state, lengths, scale, true);
+        ctx->save_for_backward({q, k, v, g, beta, state.value_or(Tensor()), lengths.value_or(Tensor()), r[2]});
+        ctx->saved_data["scale"] = scale;
+        return {r[0], r[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (!grads[0].defined() && !grads[1].defined()) return variable_list(8);
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor& v = s[2];
+        const Tensor grad_o = grads[0].defined() ? grads[0] : torch::zeros({v.size(3)}, v.options()).expand(v.sizes());
+        std::vector<Tensor> g = gated_delta_bp(s[0], s[1], v, s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(),
+                                               s[7], grad_o, grads[1]);
+        return differentiable_once({g[0], g[1], g[2], g[3], g[4], g[5], Tensor(), Tensor()});
+    }
+};
+
+std::tuple<Tensor, Tensor> gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                       const Tensor& beta, const MaybeTensor& state, const MaybeTensor& lengths,
+                                       double scale) {
+    const Tensor initial = state.value_or(Tensor());
+    if (records({&q, &k, &v, &g, &beta, &initial})) {
+        const variable_list r = GatedDeltaFunction::apply(q, k, v, g, beta, state, lengths, scale);
+        return {r[0], r[1]};
+    }
+    const std::vector<Tensor> r = gated_delta_fp(q, k, v, g, beta, state, lengths, scale, false);
+    return {r[0], r[1]};
+}
+
 }  // namespace
 
 void bind_token_layers(pybind11::module_& m) {
     m.attr("__seq_abi_version__") = snnseq_abi_version();
+    const auto release = pybind11::call_guard<pybind11::gil_scoped_release>();
+    m.def("embed", &embed, "embedding lookup with a scale, differentiable", release);
+    m.def("gn_act", &gn_act, "group norm with an activation, channels last, differentiable", release);
+    m.def("gated_delta", &gated_delta, "gated delta rule over a sequence, differentiable: (o, state_out)", release);
     m.def("embed_fp", &embed_fp, "embedding lookup with a scale");
     m.def("embed_bp", &embed_bp, "gradient of the embedding table, by sorted tokens");
     m.def("gn_act_fp", &gn_act_fp, "group norm with an activation, channels last: [mean, rstd, y]");

@@ -8,9 +8,9 @@ Same surface as the reference's ``snnlib_func.py`` for every single-GPU layer
 ``BnFireFcDistFunc`` :297-327, ``BnFireConvDistFunc`` :336-377, whose backward runs the native op in
 two halves with ``torch.distributed.all_reduce`` of two ``[C]`` vectors between them.
 
-The token layers -- ``EmbedFunc``, ``GnActFunc``, ``GatedDeltaFunc`` with ``embed_func``, ``gn_act_func``,
-``gated_delta_func`` and ``gated_delta_step`` -- extend the set to networks over token sequences on the same
-time axis; the reference has no counterpart.
+The token layers -- ``embed_func``, ``gn_act_func``, ``gated_delta_func`` and ``gated_delta_step`` -- extend the set to
+networks over token sequences on the same time axis; the reference has no counterpart.  Their autograd functions are
+part of the native module.
 
 Contract shared by all of them, as in the reference: a forward saves only its *inputs* (plus the
 per-channel inverse standard deviation a batch-norm forward returns) -- never spikes or membrane
@@ -19,7 +19,6 @@ recomputes what it needs.  Hyper-parameters are module globals read at call time
 ``snnlib_func.thresh = 0.5`` takes effect on the next call.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._loader import load_snnlib
 
@@ -293,84 +292,16 @@ class BnFireConvDistFunc(BnFireConvFunc):
                            leading=(g_spatial, g_weight_bn, g_bias_bn, None, None, None)) + (None,)
 
 
-class EmbedFunc(torch.autograd.Function):
-    """out = scale * weight[tokens]; a token outside the table (-1, say) gives a row of zeros."""
-
-    @staticmethod
-    def forward(ctx, tokens, weight, scale):
-        ctx.save_for_backward(tokens)
-        ctx.vocab, ctx.scale = weight.shape[0], scale
-        return snnlib.embed_fp(tokens, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        (tokens,) = ctx.saved_tensors
-        return None, snnlib.embed_bp(tokens, grad_out, ctx.vocab, ctx.scale), None
-
-
-class GnActFunc(torch.autograd.Function):
-    """y = act(group_norm(x)) over the last axis of ``[T, B, ..., C]``; saves the statistics with its inputs."""
-
-    @staticmethod
-    def forward(ctx, x, weight_gn, bias_gn, groups, eps_gn, act):
-        mean, rstd, y = snnlib.gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act)
-        ctx.save_for_backward(x, weight_gn, bias_gn, mean, rstd)
-        ctx.groups, ctx.act = groups, act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        # saved: x, weight_gn, bias_gn, mean, rstd
-        return _pad(snnlib.gn_act_bp(*ctx.saved_tensors, ctx.groups, ctx.act, grad_y), 6)
-
-
-class GatedDeltaFunc(torch.autograd.Function):
-    """(o, last state) of the gated delta rule.  Unlike the fire layers this one keeps what its forward
-    computed on the way -- the state before every chunk of 64 steps and the rows added to it -- because the
-    state passes are bound by latency: running them again would cost a third of the backward, and the
-    memory is there."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, lengths, scale):
-        ctx.set_materialize_grads(False)
-        o, state_out, saved = snnlib.gated_delta_fp(q, k, v, g, beta, state, lengths, scale)
-        ctx.save_for_backward(q, k, v, g, beta, state, lengths, saved)
-        ctx.scale = scale
-        return o, state_out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_o, grad_state_out):
-        q, k, v, g, beta, state, lengths, saved = ctx.saved_tensors
-        if grad_o is None:
-            if grad_state_out is None:
-                return (None,) * 8
-            grad_o = v.new_zeros(v.shape[-1]).expand(v.shape)
-        grads = snnlib.gated_delta_bp(q, k, v, g, beta, state, lengths, ctx.scale, saved, grad_o, grad_state_out)
-        return (*grads[:5], grads[5] if state is not None else None, None, None)
-
-
-def _records(*tensors):
-    """Whether autograd would record an operator on these tensors; without that the token layers call the
-    native op directly (a call on a few tokens is over in less time than a recorded node takes)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def embed_func(tokens, weight, scale=1.0):
-    """``scale * weight[tokens]`` for integer ``tokens`` of any shape, ``[*tokens.shape, cout]``."""
-    if _records(weight):
-        return EmbedFunc.apply(tokens, weight, scale)
-    return snnlib.embed_fp(tokens, weight, scale)
+    """``scale * weight[tokens]`` for integer ``tokens`` of any shape, ``[*tokens.shape, cout]``; a token outside the table
+    (-1, say) gives a row of zeros and no gradient."""
+    return snnlib.embed(tokens, weight, scale)
 
 
 def gn_act_func(x, weight_gn, bias_gn, groups, eps_gn=1e-5, act="none"):
     """Group norm over the last axis of ``[T, B, ..., C]`` (per time step, batch entry and group of ``C / groups``
-    channels), then ``act``: "none", "relu", "silu" or "gelu"."""
-    if _records(x, weight_gn, bias_gn):
-        return GnActFunc.apply(x, weight_gn, bias_gn, groups, eps_gn, act)
-    return snnlib.gn_act_fp(x, weight_gn, bias_gn, groups, eps_gn, act)[2]
+    channels), then ``act``: "none", "relu", "silu" or "gelu".  Keeps its inputs and the statistics."""
+    return snnlib.gn_act(x, weight_gn, bias_gn, groups, eps_gn, act)
 
 
 def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
@@ -382,20 +313,14 @@ def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
     ``q``, ``k`` ``[T, B, Hk, Dk]``, ``v`` ``[T, B, Hv, Dv]`` (float32 or bfloat16, any strides with dense rows; ``Hv``
     a multiple of ``Hk``, ``Dk`` up to 128), ``g`` (at most zero) and ``beta`` ``[T, B, Hv]`` float32, ``state``
     ``[B, Hv, Dk, Dv]`` float32, ``lengths`` ``[B]`` int32: steps at or behind a sequence's length do not exist.
-    ``scale`` defaults to ``Dk ** -0.5``."""
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
-    if _records(q, k, v, g, beta, state):
-        return GatedDeltaFunc.apply(q, k, v, g, beta, state, lengths, scale)
-    return tuple(snnlib.gated_delta_fp(q, k, v, g, beta, state, lengths, scale, False)[:2])
+    ``scale`` defaults to ``Dk ** -0.5``.  Where a gradient will be asked for, the state before every 64th step is kept."""
+    return snnlib.gated_delta(q, k, v, g, beta, state, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
 
 
 def gated_delta_step(q, k, v, g, beta, state, scale=None, state_out=None):
     """One step of the gated delta rule for generation: ``q``, ``k`` ``[B, Hk, Dk]``, ``v`` ``[B, Hv, Dv]``, ``g``, ``beta``
     ``[B, Hv]``; returns ``o`` ``[B, Hv, Dv]`` and updates ``state`` in place, or writes the new state to ``state_out``.
-    Not recorded by autograd: operands that require a gradient are refused unless gradients are off."""
-    if _records(q, k, v, g, beta, state):
-        raise RuntimeError("gated_delta_step is not differentiable: call it under torch.no_grad(), or use gated_delta_func")
+    Not differentiable: operands that require a gradient are refused unless gradients are off."""
     return snnlib.gated_delta_step(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale, state_out)
 
 

@@ -117,12 +117,14 @@ def test_helpers_reject_mismatched_buffers_before_any_launch():
 def test_python_surface():
     from snn_gpu_training_bptt_amd import snnlib_func as sf
     from snn_gpu_training_bptt_amd import snnlib_op as sop
-    for name in ("embed_fp", "embed_bp", "gn_act_fp", "gn_act_bp", "gated_delta_fp", "gated_delta_bp", "gated_delta_step"):
+    for name in ("embed", "embed_fp", "embed_bp", "gn_act", "gn_act_fp", "gn_act_bp", "gated_delta", "gated_delta_fp",
+                 "gated_delta_bp", "gated_delta_step"):
         assert callable(getattr(sf.snnlib, name))
     assert sf.snnlib.__seq_abi_version__ == seq_cabi.ABI_VERSION
     for name in ("Embed", "GnAct", "GatedDelta"):
         assert issubclass(getattr(sop, name), torch.nn.Module)
-        assert issubclass(getattr(sf, name + "Func"), torch.autograd.Function)
+    for name in ("embed_func", "gn_act_func", "gated_delta_func", "gated_delta_step"):
+        assert callable(getattr(sf, name))
     embed, norm, delta = sop.Embed(11, 6, 2.0), sop.GnAct(2, 8), sop.GatedDelta()
     assert {n: tuple(t.shape) for n, t in embed.named_parameters()} == {"weight_embed": (11, 6)}
     assert {n: tuple(t.shape) for n, t in norm.named_parameters()} == {"weight_gn": (8,), "bias_gn": (8,)}
