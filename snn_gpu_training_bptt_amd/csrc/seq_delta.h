@@ -27,6 +27,7 @@
 // (delta_state_kernel forwards, delta_state_grad_kernel backwards) walk the chunks of a head, one workgroup per head
 // and 16 columns of the state, which they hold in accumulators.
 //   forward    delta_inverse_kernel -> Tm;   delta_state_kernel -> S of every chunk, R, last state;   delta_output_kernel -> O
+//              without a backward to come: delta_inverse_kernel -> Tm, P;   delta_state_kernel -> O, last state
 //   backward   delta_inner_grad_kernel -> P^T dO;   delta_state_grad_kernel -> dS' of every chunk, dX;
 //              delta_input_grad_kernel -> the gradients;   delta_shared_grad_kernel where heads share keys
 // The state passes are bound by the latency of a chunk's chain of products (three forward, three backward, each
@@ -272,6 +273,10 @@ __device__ __forceinline__ void frag_of(const float (&x)[8], FragF& f) {
     for (int j = 0; j < 8; ++j) f.v[j] = x[j];
 }
 
+// The first two parts of three.
+__device__ __forceinline__ FragH<2> coarse(const FragH<3>& f) { return FragH<2>{{f.p[0], f.p[1]}}; }
+__device__ __forceinline__ const FragF& coarse(const FragF& f) { return f; }
+
 // What a storage type computes with: tiles of inputs, and of derived values on the way to fp32 results (Fine) or to
 // results of the storage type (Coarse).
 template <typename E> struct Mode;
@@ -280,6 +285,7 @@ template <> struct Mode<bf16_t> {
     template <int R, int C> using Fine = TileH<3, R, C>;
     template <int R, int C> using Coarse = TileH<2, R, C>;
     using InputFrag = FragH<1>;
+    using CoarseFrag = FragH<2>;
     using FineFrag = FragH<3>;
 };
 template <> struct Mode<float> {
@@ -287,12 +293,14 @@ template <> struct Mode<float> {
     template <int R, int C> using Fine = TileF<R, C>;
     template <int R, int C> using Coarse = TileF<R, C>;
     using InputFrag = FragF;
+    using CoarseFrag = FragF;
     using FineFrag = FragF;
 };
 
 // Bytes of a chunk's operands in this form: keys (or queries) by rows or transposed, and a 64 x 64 matrix.
 template <typename E> constexpr int keys_bytes(int dkp) { return dkp / 8 * frag_bytes<typename Mode<E>::InputFrag>(); }
 template <typename E> constexpr int square_bytes() { return 8 * frag_bytes<typename Mode<E>::FineFrag>(); }
+template <typename E> constexpr int scores_bytes() { return 8 * frag_bytes<typename Mode<E>::CoarseFrag>(); }
 
 // ---- arguments ----------------------------------------------------------------------------------
 
@@ -328,6 +336,8 @@ struct DeltaArgs {
     char *keys, *keys_t;        // per (batch entry, key head, chunk): K by rows, and transposed, fragments
     float* added;               // R, [cols, 64]
     float* states;              // state before the chunk, [cols, DKP]
+    // a forward with its output in the state pass: Q by rows as keys, and P as fragments of two parts; else nullptr
+    char *queries, *scores;
     // backward
     char* queries_t;            // as keys_t
     float* inner;               // P^T dO, then dX, [cols, 64]
@@ -613,7 +623,8 @@ __device__ __forceinline__ void invert_unit_lower(const Square& a, Square& t, Sq
     }
 }
 
-template <typename E, bool WIDE, int DKP>
+// OUTPUT: and what the state pass needs for the output, the queries and P.
+template <typename E, bool WIDE, int DKP, bool OUTPUT>
 __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
     using M = Mode<E>;
     union First {   // K is done with when the inversion needs its scratch
@@ -621,15 +632,27 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
         Square scratch;
         __device__ First() {}
     };
+    union Second {  // and P is in memory
+        typename M::template Coarse<kChunk, kChunk> p;
+        Square t;
+        __device__ Second() {}
+    };
     __shared__ First u;
-    __shared__ Square a, t;
+    __shared__ Second z;
+    __shared__ Square a;
+    __shared__ typename M::template Input<OUTPUT ? kChunk : 1, DKP> q;
     __shared__ Decay y;
+    Square& t = z.t;
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
     if (w.rows == 0) return;
     Ahead<WIDE, E, kChunk, DKP, 256> k;
     k.load(row_of<E>(args.k, w, w.hk), args.k.t, w.rows, args.Dk);
+    if constexpr (OUTPUT) {
+        Ahead<WIDE, E, kChunk, DKP, 256> q_next;
+        q_next.load(row_of<E>(args.q, w, w.hk), args.q.t, w.rows, args.Dk);
+        q_next.store(q);
+    }
     decay_of(args, w, y);
-    for (int i = threadIdx.x; i < kChunk * (kChunk + 4); i += 256) (&t.v[0][0])[i] = 0.f;
     k.store(u.k);
     __syncthreads();
     if (threadIdx.x < sizeof(Decay) / 16)
@@ -640,7 +663,33 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
         for (int s = 0; s < DKP / 32; ++s)
             store_frag(args.keys + w.key_at * keys_bytes<E>(DKP), wave * (DKP / 32) + s, u.k.rows(wave * 16, s * 32));
         store_transposed<E, DKP, 4>(u.k, args.keys_t + w.key_at * keys_bytes<E>(DKP));
+        if constexpr (OUTPUT) {
+#pragma unroll
+            for (int s = 0; s < DKP / 32; ++s)
+                store_frag(args.queries + w.key_at * keys_bytes<E>(DKP), wave * (DKP / 32) + s, q.rows(wave * 16, s * 32));
+        }
     }
+    if constexpr (OUTPUT) {
+#pragma unroll
+        for (int block = 0; block < 4; ++block) {
+            f32x4 acc = zero4();
+            if (block <= wave) {
+#pragma unroll
+                for (int s = 0; s < DKP; s += 32) acc = mma(q.rows(wave * 16, s), u.k.rows(block * 16, s), acc);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = wave * 16 + (lane >> 4) * 4 + e, j = block * 16 + (lane & 15);
+                z.p.put(i, j, i >= j ? args.scale * acc[e] * gap(y, i, j) : 0.f);
+            }
+        }
+        // a wavefront reads back its own rows only
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            store_frag(args.scores + w.at * scores_bytes<E>(), wave * 2 + s, z.p.rows(wave * 16, s * 32));
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < kChunk * (kChunk + 4); i += 256) (&t.v[0][0])[i] = 0.f;
     for (int block = 0; block <= wave; ++block) {
         f32x4 acc = zero4();
 #pragma unroll
@@ -677,8 +726,11 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
 // A workgroup of four wavefronts holds kStateCols columns of a head's state: wavefront w rows 16 w.. of the chunk in
 // the first two products, DKP / 64 tiles of 16 state rows in the last one.  The chain from chunk to chunk -- three
 // products, each through LDS to the next -- is all that counts, so nothing else is on it: keys and matrices come as
-// fragments, straight into registers, a chunk ahead (two sets of registers take turns), and LDS holds only what the
-// wavefronts exchange.
+// fragments, straight into registers, and LDS holds only what the wavefronts exchange.  The next chunk's operand is
+// requested as soon as a product has used this one's, into the same registers: a chunk's time ahead, while the matrix
+// instructions run.  (Requested all together, or before the products, they cost the chain 1900 cycles of 4800: each
+// occupies the memory path of the CU for 16.)  Loads are never under a condition, which would make every wait one for
+// all of them; behind the last chunk they fetch it once more.
 
 constexpr int kStateThreads = 256;
 
@@ -736,22 +788,29 @@ struct ColumnAhead {
 };
 
 // What the forward pass takes from memory for a chunk.
-template <typename E, int DKP>
+template <typename E, int DKP, bool OUTPUT>
 struct StateOperands {
     using M = Mode<E>;
-    typename M::InputFrag k[DKP / 32], kt[DKP / 64][2];
+    typename M::InputFrag k[DKP / 32], kt[DKP / 64][2], q[OUTPUT ? DKP / 32 : 1];
     typename M::FineFrag inverse[2];
+    typename M::CoarseFrag p[OUTPUT ? 2 : 1];
     f32x4 a, d, beta;
     float a_last;
     ColumnAhead<E> v;
-    DeltaWhere w;
-    // in three parts, each requested while a product waits for LDS: a vector access of a wavefront occupies the
-    // memory path of the CU for 16 cycles, and all of them in a row would stand in the way of the chain
-    __device__ __forceinline__ void load_keys(const DeltaArgs& args, int head, int chunk, int length, int row, int col) {
-        w = delta_where(args, head, chunk, length);
-        const char* keys = args.keys + w.key_at * keys_bytes<E>(DKP);
+    __device__ __forceinline__ void load_keys(const DeltaArgs& args, const DeltaWhere& w) {
+        load_rows(k, args.keys + w.key_at * keys_bytes<E>(DKP));
+        if constexpr (OUTPUT) load_rows(q, args.queries + w.key_at * keys_bytes<E>(DKP));
+    }
+    __device__ __forceinline__ static void load_rows(typename M::InputFrag (&x)[DKP / 32], const char* matrix) {
 #pragma unroll
-        for (int s = 0; s < DKP / 32; ++s) k[s] = load_frag<typename M::InputFrag>(keys, (threadIdx.x >> 6) * (DKP / 32) + s);
+        for (int s = 0; s < DKP / 32; ++s) x[s] = load_frag<typename M::InputFrag>(matrix, (threadIdx.x >> 6) * (DKP / 32) + s);
+    }
+    __device__ __forceinline__ void load_inverse(const DeltaArgs& args, const DeltaWhere& w) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            inverse[s] = load_frag<typename M::FineFrag>(args.inverse + w.at * square_bytes<E>(), (threadIdx.x >> 6) * 2 + s);
+    }
+    __device__ __forceinline__ void load_factors(const DeltaArgs& args, const DeltaWhere& w, int row, int col) {
         const Decay* y = args.decay + w.at;
         a = *reinterpret_cast<const f32x4*>(y->a + row);
         d = *reinterpret_cast<const f32x4*>(y->d + row);
@@ -759,95 +818,132 @@ struct StateOperands {
         a_last = y->a[kChunk - 1];
         v.load(args.v, w, w.hv, row, col, args.Dv);
     }
-    __device__ __forceinline__ void load_inverse(const DeltaArgs& args) {
-        const char* matrix = args.inverse + w.at * square_bytes<E>();
-        inverse[0] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2);
-        inverse[1] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2 + 1);
-    }
-    __device__ __forceinline__ void load_transposed(const DeltaArgs& args) {
-        const char* keys_t = args.keys_t + w.key_at * keys_bytes<E>(DKP);
+    __device__ __forceinline__ void load_transposed(const DeltaArgs& args, const DeltaWhere& w) {
 #pragma unroll
         for (int i = 0; i < DKP / 64; ++i)
 #pragma unroll
             for (int s = 0; s < 2; ++s)
-                kt[i][s] = load_frag<typename M::InputFrag>(keys_t, ((threadIdx.x >> 6) + 4 * i) * 2 + s);
+                kt[i][s] = load_frag<typename M::InputFrag>(args.keys_t + w.key_at * keys_bytes<E>(DKP), ((threadIdx.x >> 6) + 4 * i) * 2 + s);
+    }
+    __device__ __forceinline__ void load_scores(const DeltaArgs& args, const DeltaWhere& w) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            p[s] = load_frag<typename M::CoarseFrag>(args.scores + w.at * scores_bytes<E>(), (threadIdx.x >> 6) * 2 + s);
     }
 };
 
-template <typename E, int DKP>
+// OUTPUT: with the output, for a forward that leaves nothing for a backward; the states and R then never reach memory.
+template <typename E, int DKP, bool OUTPUT>
 __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(DeltaArgs args) {
     using M = Mode<E>;
     constexpr int NV = kStateCols;
     __shared__ typename M::template Fine<NV, DKP> state;     // transposed
-    __shared__ typename M::template Fine<NV, kChunk> x, r;   // transposed
+    __shared__ typename M::template Fine<NV, kChunk> x, r;   // transposed; X and d R
+    __shared__ typename M::template Coarse<NV, OUTPUT ? kChunk : 32> plain_r;
     const int tiles = args.cols / NV;
     const int piece = piece_in_l2(args.B * args.Hv * tiles), head = piece / tiles, v0 = (piece - head * tiles) * NV;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int lc = lane & 15, row = wave * 16 + (lane >> 4) * 4, col = v0 + lc;
     const int length = delta_length(args, head / args.Hv), chunks = (length + kChunk - 1) / kChunk;
 
-    StateOperands<E, DKP> even, odd;
+    StateOperands<E, DKP, OUTPUT> now;
     if (chunks > 0) {
-        even.load_keys(args, head, 0, length, row, col);
-        even.load_inverse(args);
-        even.load_transposed(args);
+        const DeltaWhere w = delta_where(args, head, 0, length);
+        now.load_keys(args, w);
+        now.load_factors(args, w, row, col);
+        now.load_inverse(args, w);
+        now.load_transposed(args, w);
+        if constexpr (OUTPUT) now.load_scores(args, w);
     }
     StateTiles<DKP> s;
     s.load(args.state, head, args.Dk, args.Dv, col);
     s.put(state);
-    const auto step = [&](int chunk, const StateOperands<E, DKP>& now, StateOperands<E, DKP>& next) {
-        // behind the last chunk: the same once more.  Loads under a condition would make every wait one for all of them
-        const int ahead = chunk + 1 < chunks ? chunk + 1 : chunk;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        const DeltaWhere w = delta_where(args, head, chunk + 1 < chunks ? chunk + 1 : chunk, length);   // the next one
+        const int64_t at = static_cast<int64_t>(head) * args.chunks + chunk;
         __syncthreads();
-        f32x4 acc[2] = {zero4(), zero4()};
+        f32x4 acc[2] = {zero4(), zero4()}, o = zero4();   // o sums in the order of delta_output_kernel
         typename M::FineFrag f[DKP / 32];
 #pragma unroll
         for (int c = 0; c < DKP / 32; ++c) f[c] = state.rows(0, c * 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_keys(args, head, ahead, length, row, col);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < DKP / 32; ++c) acc[c % 2] = mma(now.k[c], f[c], acc[c % 2]);
+        if constexpr (OUTPUT) {
+#pragma unroll
+            for (int c = 0; c < DKP / 32; ++c) o = mma(now.q[c], coarse(f[c]), o);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_keys(args, w);
+        __builtin_amdgcn_sched_barrier(0);
         float out[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = now.beta[e] * (now.v.get(e) - now.a[e] * (acc[0][e] + acc[1][e]));
         x.put(lc, row, out);
-        s.keep(args.states + now.w.at * DKP * args.cols, col);
+        if constexpr (OUTPUT) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= args.scale * now.a[e];
+        } else {
+            s.keep(args.states + at * DKP * args.cols, col);
+        }
         __syncthreads();
         f[0] = x.rows(0, 0);
         f[1] = x.rows(0, 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_inverse(args);
-        __builtin_amdgcn_sched_barrier(0);
         acc[0] = mma(now.inverse[0], f[0], zero4());
         if (wave >= 2) {   // rows below 32 have nothing right of column 32
             acc[1] = mma(now.inverse[1], f[1], zero4());
             acc[0] += acc[1];
         }
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_inverse(args, w);
+        __builtin_amdgcn_sched_barrier(0);
         f32x4 next_s[s.n];
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = now.d[e] * acc[0][e];
         r.put(lc, row, out);
-        store_later(args.added + (now.w.at * args.cols + col) * kChunk + row, acc[0]);
+        if constexpr (OUTPUT) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = acc[0][e];
+            plain_r.put(lc, row, out);
+        } else {
+            store_later(args.added + (at * args.cols + col) * kChunk + row, acc[0]);
+        }
 #pragma unroll
         for (int i = 0; i < s.n; ++i) next_s[i] = now.a_last * s.s[i];
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_factors(args, w, row, col);
         __syncthreads();
         f[0] = r.rows(0, 0);
         f[1] = r.rows(0, 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_transposed(args);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < s.n; ++i) next_s[i] = mma(now.kt[i][c], f[c], next_s[i]);
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_transposed(args, w);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < s.n; ++i) s.s[i] = next_s[i];
         s.put(state);
-    };
-    for (int chunk = 0; chunk < chunks; chunk += 2) {
-        step(chunk, even, odd);
-        if (chunk + 1 < chunks) step(chunk + 1, odd, even);
+        if constexpr (OUTPUT) {
+            o = mma(now.p[0], plain_r.rows(0, 0), o);
+            if (wave >= 2) o = mma(now.p[1], plain_r.rows(0, 32), o);
+            now.load_scores(args, w);
+            const int t0 = chunk * kChunk;
+            E* p = static_cast<E*>(args.o) + ((static_cast<int64_t>(t0) + row) * args.B * args.Hv + head) * args.Dv + col;
+            const int64_t stride = static_cast<int64_t>(args.B) * args.Hv * args.Dv;
+            if (col < args.Dv) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (t0 + row + e < args.T) p[e * stride] = narrow<E>(t0 + row + e < length ? o[e] : 0.f);
+            }
+        }
+    }
+    if constexpr (OUTPUT) {   // steps in chunks that no row of the sequence reaches
+        for (int t = chunks * kChunk + static_cast<int>(threadIdx.x >> 4); t < args.T; t += kStateThreads / 16) {
+            const int c = v0 + (threadIdx.x & 15);
+            if (c < args.Dv)
+                static_cast<E*>(args.o)[(static_cast<int64_t>(t) * args.B * args.Hv + head) * args.Dv + c] = narrow<E>(0.f);
+        }
     }
     s.save(args.state_out, head, args.Dk, args.Dv, col);
 }
@@ -1008,32 +1104,31 @@ struct StateGradOperands {
     f32x4 a, d, beta, inner;
     float a_last;
     ColumnAhead<E> go;
-    DeltaWhere w;
-    // in parts, as in the forward pass
-    __device__ __forceinline__ void load_keys(const DeltaArgs& args, int head, int chunk, int length, int row, int col) {
-        w = delta_where(args, head, chunk, length);
-        const char* keys = args.keys + w.key_at * keys_bytes<E>(DKP);
+    __device__ __forceinline__ void load_keys(const DeltaArgs& args, const DeltaWhere& w) {
 #pragma unroll
-        for (int s = 0; s < DKP / 32; ++s) k[s] = load_frag<typename M::InputFrag>(keys, (threadIdx.x >> 6) * (DKP / 32) + s);
-        inner = *reinterpret_cast<const f32x4*>(args.inner + (w.at * args.cols + col) * kChunk + row);
-        go.load(args.grad_o, w, w.hv, row, col, args.Dv);
-        const Decay* y = args.decay + w.at;
-        a = *reinterpret_cast<const f32x4*>(y->a + row);
-        d = *reinterpret_cast<const f32x4*>(y->d + row);
-        beta = *reinterpret_cast<const f32x4*>(y->beta + row);
-        a_last = y->a[kChunk - 1];
+        for (int s = 0; s < DKP / 32; ++s)
+            k[s] = load_frag<typename M::InputFrag>(args.keys + w.key_at * keys_bytes<E>(DKP), (threadIdx.x >> 6) * (DKP / 32) + s);
     }
-    __device__ __forceinline__ void load_inverse(const DeltaArgs& args) {
-        const char* matrix = args.inverse_t + w.at * square_bytes<E>();
-        inverse[1] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2 + 1);
-        inverse[0] = load_frag<typename M::FineFrag>(matrix, (threadIdx.x >> 6) * 2);
+    __device__ __forceinline__ void load_inverse(const DeltaArgs& args, const DeltaWhere& w) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            inverse[s] = load_frag<typename M::FineFrag>(args.inverse_t + w.at * square_bytes<E>(), (threadIdx.x >> 6) * 2 + s);
     }
-    __device__ __forceinline__ void load_transposed(typename M::InputFrag (&x)[DKP / 64][2], const char* matrix) {
+    __device__ __forceinline__ void load_transposed(typename M::InputFrag (&x)[DKP / 64][2], const char* matrix, const DeltaWhere& w) {
 #pragma unroll
         for (int i = 0; i < DKP / 64; ++i)
 #pragma unroll
             for (int s = 0; s < 2; ++s)
                 x[i][s] = load_frag<typename M::InputFrag>(matrix + w.key_at * keys_bytes<E>(DKP), ((threadIdx.x >> 6) + 4 * i) * 2 + s);
+    }
+    __device__ __forceinline__ void load_factors(const DeltaArgs& args, const DeltaWhere& w, int row, int col) {
+        const Decay* y = args.decay + w.at;
+        a = *reinterpret_cast<const f32x4*>(y->a + row);
+        d = *reinterpret_cast<const f32x4*>(y->d + row);
+        beta = *reinterpret_cast<const f32x4*>(y->beta + row);
+        a_last = y->a[kChunk - 1];
+        inner = *reinterpret_cast<const f32x4*>(args.inner + (w.at * args.cols + col) * kChunk + row);
+        go.load(args.grad_o, w, w.hv, row, col, args.Dv);
     }
 };
 
@@ -1049,56 +1144,56 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_grad_kernel(DeltaAr
     const int lc = lane & 15, row = wave * 16 + (lane >> 4) * 4, col = v0 + lc;
     const int length = delta_length(args, head / args.Hv), chunks = (length + kChunk - 1) / kChunk;
 
-    StateGradOperands<E, DKP> even, odd;
+    StateGradOperands<E, DKP> now;
     if (chunks > 0) {
-        even.load_keys(args, head, chunks - 1, length, row, col);
-        even.load_transposed(even.qt, args.queries_t);
-        even.load_inverse(args);
-        even.load_transposed(even.kt, args.keys_t);
+        const DeltaWhere w = delta_where(args, head, chunks - 1, length);
+        now.load_factors(args, w, row, col);
+        now.load_keys(args, w);
+        now.load_inverse(args, w);
+        now.load_transposed(now.qt, args.queries_t, w);
+        now.load_transposed(now.kt, args.keys_t, w);
     }
     StateTiles<DKP> s;
     s.load(args.grad_state, head, args.Dk, args.Dv, col);
     s.put(state);
-    const auto step = [&](int chunk, const StateGradOperands<E, DKP>& now, StateGradOperands<E, DKP>& next) {
+    for (int chunk = chunks - 1; chunk >= 0; --chunk) {
+        const DeltaWhere w = delta_where(args, head, chunk > 0 ? chunk - 1 : 0, length);   // the next one
+        const int64_t at = static_cast<int64_t>(head) * args.chunks + chunk;
         float out[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = args.scale * now.a[e] * now.go.get(e);
         go.put(lc, row, out);   // its readers of the chunk before are behind a barrier
-        const int ahead = chunk > 0 ? chunk - 1 : 0;   // as above
         __syncthreads();
         f32x4 acc[2] = {zero4(), zero4()};
         typename M::FineFrag f[DKP / 32];
 #pragma unroll
         for (int c = 0; c < DKP / 32; ++c) f[c] = state.rows(0, c * 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_keys(args, head, ahead, length, row, col);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < DKP / 32; ++c) acc[c % 2] = mma(now.k[c], f[c], acc[c % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_keys(args, w);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = now.inner[e] + now.d[e] * (acc[0][e] + acc[1][e]);
         r.put(lc, row, out);
-        s.keep(args.state_grads + now.w.at * DKP * args.cols, col);
+        s.keep(args.state_grads + at * DKP * args.cols, col);
         __syncthreads();
         f[0] = r.rows(0, 0);
         f[1] = r.rows(0, 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_inverse(args);
-        __builtin_amdgcn_sched_barrier(0);
         acc[1] = mma(now.inverse[1], f[1], zero4());
         if (wave < 2) {   // columns from 32 on have nothing above row 32
             acc[0] = mma(now.inverse[0], f[0], zero4());
             acc[1] += acc[0];
         }
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_inverse(args, w);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = -now.beta[e] * now.a[e] * acc[1][e];
         x.put(lc, row, out);
-        store_later(args.inner + (now.w.at * args.cols + col) * kChunk + row, acc[1]);
+        store_later(args.inner + (at * args.cols + col) * kChunk + row, acc[1]);
         f[0] = go.rows(0, 0);   // does not wait for dX
         f[1] = go.rows(0, 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_transposed(next.qt, args.queries_t);
-        __builtin_amdgcn_sched_barrier(0);
         f32x4 next_s[s.n];
 #pragma unroll
         for (int i = 0; i < s.n; ++i) next_s[i] = now.a_last * s.s[i];
@@ -1106,23 +1201,22 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_grad_kernel(DeltaAr
         for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < s.n; ++i) next_s[i] = mma(now.qt[i][c], f[c], next_s[i]);
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_transposed(now.qt, args.queries_t, w);
+        now.load_factors(args, w, row, col);
         __syncthreads();
         f[0] = x.rows(0, 0);
         f[1] = x.rows(0, 32);
-        __builtin_amdgcn_sched_barrier(0);
-        next.load_transposed(next.kt, args.keys_t);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < s.n; ++i) next_s[i] = mma(now.kt[i][c], f[c], next_s[i]);
+        __builtin_amdgcn_sched_barrier(0);
+        now.load_transposed(now.kt, args.keys_t, w);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < s.n; ++i) s.s[i] = next_s[i];
         s.put(state);
-    };
-    for (int chunk = chunks - 1; chunk >= 0; chunk -= 2) {
-        step(chunk, even, odd);
-        if (chunk > 0) step(chunk - 1, odd, even);
     }
     s.save(args.grad_initial, head, args.Dk, args.Dv, col);
 }
@@ -1435,8 +1529,13 @@ hipError_t delta_forward_as(const DeltaArgs& a, hipStream_t st) {
     const dim3 pieces(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.Hv));
     const dim3 columns(static_cast<unsigned>(a.cols / kStateCols * a.B * a.Hv));
     hipError_t err = hipSuccess;
-    if (a.chunks > 0) err = launch(delta_inverse_kernel<E, WIDE, DKP>, pieces, dim3(256), st, a);
-    if (err == hipSuccess) err = launch(delta_state_kernel<E, DKP>, columns, dim3(kStateThreads), st, a);
+    if (a.scores != nullptr) {
+        if (a.chunks > 0) err = launch(delta_inverse_kernel<E, WIDE, DKP, true>, pieces, dim3(256), st, a);
+        if (err == hipSuccess) err = launch(delta_state_kernel<E, DKP, true>, columns, dim3(kStateThreads), st, a);
+        return err;
+    }
+    if (a.chunks > 0) err = launch(delta_inverse_kernel<E, WIDE, DKP, false>, pieces, dim3(256), st, a);
+    if (err == hipSuccess) err = launch(delta_state_kernel<E, DKP, false>, columns, dim3(kStateThreads), st, a);
     if (err == hipSuccess && a.chunks > 0) err = launch(delta_output_kernel<E, WIDE, DKP>, pieces, dim3(kPieceThreads), st, a);
     return err;
 }

@@ -182,6 +182,7 @@ DeltaTensor tensor_of(const void* p, const int64_t* strides, int64_t D, size_t e
 struct Sizes {
     int64_t pieces, heads, chunks, cols, dkp;
     size_t decay, inverse, keys, added, states;  // bytes of what the forward leaves behind (inverse and keys: twice)
+    size_t scores;                               // of a forward that leaves nothing behind
     size_t inner, state_grads, queries, partial; // of the backward's
     size_t saved, workspace;                     // in all
 };
@@ -202,7 +203,8 @@ Sizes sizes_of(const snnseq_delta* c, bool for_backward) {
     s.added = s.inner = n * kChunk * static_cast<size_t>(s.cols);
     s.states = s.state_grads = n * static_cast<size_t>(s.dkp * s.cols);
     s.partial = c->Hv == c->Hk ? 0 : round_up(static_cast<size_t>(c->T * s.heads * c->Dk) * sizeof(float), 16);
-    s.saved = s.decay + (for_backward ? 2 : 1) * s.inverse + 2 * s.keys + s.added + s.states;
+    s.scores = static_cast<size_t>(s.pieces) * (f32 ? scores_bytes<float>() : scores_bytes<bf16_t>());
+    s.saved = s.decay + s.inverse + 2 * s.keys + (for_backward ? s.inverse + s.added + s.states : s.queries + s.scores);
     s.workspace = s.inner + s.state_grads + s.queries + 2 * s.partial;
     return s;
 }
@@ -223,11 +225,17 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved, bool for_b
     char* p = static_cast<char*>(saved);
     a.decay = reinterpret_cast<Decay*>(p);
     a.inverse = p + s.decay;
-    a.inverse_t = for_backward ? a.inverse + s.inverse : nullptr;
-    a.keys = a.inverse + (for_backward ? 2 : 1) * s.inverse;
+    a.keys = a.inverse + s.inverse;
     a.keys_t = a.keys + s.keys;
-    a.added = reinterpret_cast<float*>(a.keys_t + s.keys);
-    a.states = reinterpret_cast<float*>(a.keys_t + s.keys + s.added);
+    char* rest = a.keys_t + s.keys;
+    if (for_backward) {
+        a.inverse_t = rest;
+        a.added = reinterpret_cast<float*>(rest + s.inverse);
+        a.states = reinterpret_cast<float*>(rest + s.inverse + s.added);
+    } else {
+        a.queries = rest;
+        a.scores = rest + s.queries;
+    }
     return a;
 }
 
