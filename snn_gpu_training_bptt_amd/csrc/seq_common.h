@@ -72,6 +72,23 @@ __device__ __forceinline__ Vec<E, BYTES> load_vec_once(const E* p) {
     return v;
 }
 
+// The vector at p[at], zero where it is absent; p[0] has to be there all the same.  Loads of two bytes go into half
+// of a register, which the compiler waits for at the end of a condition, and it has put waits between conditional loads
+// of four: narrow ones are under none.
+template <typename E, int BYTES, typename I>
+__device__ __forceinline__ Vec<E, BYTES> load_or_zero(const E* p, I at, bool present, bool once) {
+    using raw_t = typename Vec<E, BYTES>::raw_t;
+    Vec<E, BYTES> v;
+    if constexpr (BYTES > 4) {
+        v.raw = raw_t(0);
+        if (present) v = once ? load_vec_once<E, BYTES>(p + at) : load_vec<E, BYTES>(p + at);
+    } else {
+        v = load_vec<E, BYTES>(p + (present ? at : I(0)));
+        v.raw = present ? v.raw : raw_t(0);
+    }
+    return v;
+}
+
 template <typename E, int BYTES>
 __device__ __forceinline__ void store_vec(E* p, const Vec<E, BYTES>& v) {
     *reinterpret_cast<typename Vec<E, BYTES>::raw_t*>(p) = v.raw;

@@ -10,8 +10,10 @@ namespace {
 // state, and S'^T q = a S^T q + (k . q) e, so the state is read once, held in registers, and written once: 8 bytes
 // per value, the bound.  A workgroup owns 64 columns of a head's state: 16 lanes of four columns share a row, eight
 // rows at a time, and the sums over the rows go through shuffles and LDS.  A thread of 128 holds sixteen vectors of
-// a state of 128 rows; with 256 threads and eight vectors each, 64 sequences of 16 heads took 38 us instead of 22
-// (134 MB: 6 TB/s, part of it from the memory-side cache), with 64 threads and 32 vectors 23.
+// a state of 128 rows (with 256 threads and eight vectors each, 64 sequences of 16 heads took 38 us); registers for
+// four wavefronts per SIMD.  With a state of 128 x 128: 64 sequences of 16 heads 24.6 us (134 MB: 5.5 TB/s), 512 of
+// them 189 us (1.07 GB: 5.7 TB/s); of 64 x 64, 64 sequences 6.7 us and 512 of them 45 us (with a condition around each
+// load the compiler waited for one after another: 9.7 and 79 us).
 
 constexpr int kStepCols = 64, kStepThreads = 128, kStepLanes = kStepCols / 4, kStepRows = kStepThreads / kStepLanes;
 
@@ -26,46 +28,57 @@ struct StepArgs {
 };
 
 template <typename E, int ROWS, bool WIDE>   // ROWS: rows of the state per thread;  WIDE: four columns in one access
-__global__ void __launch_bounds__(kStepThreads) delta_step_kernel(StepArgs a) {
-    __shared__ float qs[ROWS * kStepRows], ks[ROWS * kStepRows];
+__global__ void __launch_bounds__(kStepThreads, WIDE ? 4 : 3) delta_step_kernel(StepArgs a) {
+    static_assert(ROWS * kStepRows <= kStepThreads);
+    __shared__ __align__(16) float qs[kStepThreads], ks[kStepThreads];
     __shared__ float part[2][kStepThreads / 64][kStepCols];
     const int head = blockIdx.y, b = head / a.Hv, hv = head - b * a.Hv, hk = hv / (a.Hv / a.Hk);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = blockIdx.x * kStepCols + (threadIdx.x % kStepLanes) * 4, r0 = threadIdx.x / kStepLanes;
-    const int64_t base = static_cast<int64_t>(head) * a.Dk * a.Dv + c;
-    f32x4 s[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const int r = r0 + i * kStepRows;
-        s[i] = zero4();
-        if (r < a.Dk) {
-            const float* p = a.state + base + static_cast<int64_t>(r) * a.Dv;
-            if (WIDE) {
-                if (c < a.Dv) s[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < a.Dv) s[i][j] = p[j];
-            }
-        }
-    }
+    const int c = blockIdx.x * kStepCols + (threadIdx.x % kStepLanes) * 4, r0 = threadIdx.x / kStepLanes * ROWS;
+    const bool whole = a.Dk == ROWS * kStepRows;
     const E* q = static_cast<const E*>(a.q) + b * a.q_b + hk * a.q_h;
     const E* k = static_cast<const E*>(a.k) + b * a.k_b + hk * a.k_h;
     const E* v = static_cast<const E*>(a.v) + b * a.v_b + hv * a.v_h;
-    for (int r = threadIdx.x; r < ROWS * kStepRows; r += kStepThreads) {
-        qs[r] = r < a.Dk ? widen(q[r]) : 0.f;
-        ks[r] = r < a.Dk ? widen(k[r]) : 0.f;
-    }
-    const float g = a.g[head], beta = a.beta[head];
-    float value[4];
+    const int at = static_cast<int>(threadIdx.x) < a.Dk ? static_cast<int>(threadIdx.x) : a.Dk - 1;
+    const E q_in = q[at], k_in = k[at];
+    E v_in[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) value[j] = c + j < a.Dv ? widen(v[c + j]) : 0.f;
+    for (int j = 0; j < 4; ++j) v_in[j] = v[c + j < a.Dv ? c + j : 0];
+    const float g = a.g[head], beta = a.beta[head];
+    const int64_t base = static_cast<int64_t>(head) * a.Dk * a.Dv;
+    const uint32_t end = static_cast<uint32_t>(a.Dk) * a.Dv, row0 = static_cast<uint32_t>(r0) * a.Dv;   // below 2^23
+    f32x4 s[ROWS];   // requested all at once: none under a condition, absent ones read what is there
+    if (WIDE) {
+        const uint32_t last = end - a.Dv + (c < a.Dv ? c : 0);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const uint32_t x = row0 + i * static_cast<uint32_t>(a.Dv) + c;
+            s[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(a.state + base + (x < last ? x : last)));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t last = end - a.Dv + (c + j < a.Dv ? c + j : 0);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const uint32_t x = row0 + i * static_cast<uint32_t>(a.Dv) + c + j;
+                s[i][j] = a.state[base + (x < last ? x : last)];
+            }
+        }
+    }
+    qs[threadIdx.x] = static_cast<int>(threadIdx.x) < a.Dk ? widen(q_in) : 0.f;
+    ks[threadIdx.x] = static_cast<int>(threadIdx.x) < a.Dk ? widen(k_in) : 0.f;
     __syncthreads();
     f32x4 sk = zero4(), sq = zero4();
     float kq = 0.f;
+    if (!whole) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+            if (r0 + i >= a.Dk) s[i] = zero4();
+    }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const float kr = ks[r0 + i * kStepRows], qr = qs[r0 + i * kStepRows];
+        const float kr = ks[r0 + i], qr = qs[r0 + i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             sk[j] += kr * s[i][j];
@@ -100,25 +113,24 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(StepArgs a) {
     for (int w = 0; w < kStepThreads / 64; ++w) kq_all += kq_part[w];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int at = (threadIdx.x % kStepLanes) * 4 + j;
+        const int col = (threadIdx.x % kStepLanes) * 4 + j;
         float k_sum = 0.f, q_sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kStepThreads / 64; ++w) {
-            k_sum += part[0][w][at];
-            q_sum += part[1][w][at];
+            k_sum += part[0][w][col];
+            q_sum += part[1][w][col];
         }
-        add[j] = beta * (value[j] - decay * k_sum);
+        add[j] = beta * (widen(v_in[j]) - decay * k_sum);
         out[j] = a.scale * (decay * q_sum + kq_all * add[j]);
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int r = r0 + i * kStepRows;
-        if (r >= a.Dk) continue;
-        const float kr = ks[r];
+        const float kr = ks[r0 + i];
         f32x4 n;
 #pragma unroll
         for (int j = 0; j < 4; ++j) n[j] = decay * s[i][j] + kr * add[j];
-        float* p = a.state_out + base + static_cast<int64_t>(r) * a.Dv;
+        if (!whole && r0 + i >= a.Dk) continue;
+        float* p = a.state_out + base + (row0 + i * static_cast<uint32_t>(a.Dv) + c);
         if (WIDE) {
             if (c < a.Dv) __builtin_nontemporal_store(n, reinterpret_cast<f32x4*>(p));
         } else {

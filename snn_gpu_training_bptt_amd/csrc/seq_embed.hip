@@ -48,9 +48,9 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ weight,
     const int64_t first = static_cast<int64_t>(blockIdx.x) * rows * kRowsInFlight + (threadIdx.x >> tpr_log2);
     int row[kRowsInFlight];
 #pragma unroll
-    for (int r = 0; r < kRowsInFlight; ++r) {
+    for (int r = 0; r < kRowsInFlight; ++r) {   // all requested at once: none under a condition
         const int64_t i = first + static_cast<int64_t>(r) * rows;
-        row[r] = i < N ? row_of(tokens, i, V) : -1;
+        row[r] = row_of(tokens, i < N ? i : N - 1, V);
     }
     for (int c = lane * n; c < C; c += tpr * n) {
         Vec<E, BYTES> v[kRowsInFlight];

@@ -91,17 +91,13 @@ gn_rows_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
         for (int k = 0; k < K; ++k) {
             const int c = (k * L + lane) * n;
             const int64_t item = first + u * step;
-            v[u][k].raw = typename Vec<E, BYTES>::raw_t(0);
-            if (c < cpg && item < items) v[u][k] = load_vec_once<E, BYTES>(x + item * cpg + c);
+            v[u][k] = load_or_zero<E, BYTES>(x, item * cpg + c, c < cpg && item < items, true);
         }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * L + lane) * n;
-        w[k].raw = b[k].raw = typename Vec<E, BYTES>::raw_t(0);
-        if (c < cpg) {
-            w[k] = load_vec<E, BYTES>(weight + g * cpg + c);
-            b[k] = load_vec<E, BYTES>(bias + g * cpg + c);
-        }
+        w[k] = load_or_zero<E, BYTES>(weight, g * cpg + c, c < cpg, false);
+        b[k] = load_or_zero<E, BYTES>(bias, g * cpg + c, c < cpg, false);
     }
     const A per = A(1) / A(cpg);
 #pragma unroll
@@ -359,8 +355,7 @@ gn_slab_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int p = t.row + k * t.rows;
-        v[k].raw = typename Vec<E, BYTES>::raw_t(0);
-        if (t.here && p < P) v[k] = load_vec_once<E, BYTES>(px + static_cast<uint32_t>(p * C + c));
+        v[k] = load_or_zero<E, BYTES>(px, static_cast<uint32_t>(p * C + c), t.here && p < P, true);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k)
