@@ -66,6 +66,17 @@ __device__ __forceinline__ A lanes_sum(A v, int lanes) {
     return v;
 }
 
+// The product rounds by itself, as it did in c1's sum: in a group of one value they are equal, and the gradient is 0.
+template <typename A>
+__device__ __forceinline__ A input_grad(A gz, A w, A c1, A xhat, A c2, A rstd) {
+    A h;
+    {
+#pragma clang fp contract(off)
+        h = gz * w;
+    }
+    return rstd * (h - c1 - xhat * c2);
+}
+
 // ---- rows ---------------------------------------------------------------------------------------
 
 constexpr int kRowsBlock = 256;
@@ -221,7 +232,7 @@ gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
 #pragma unroll
                 for (int j = 0; j < n; ++j) {
                     const A xhat = (widen(v[k].e[j]) - m) * r;
-                    o.e[j] = narrow<E>(r * (gz[k * n + j] * widen(w[k].e[j]) - c1 - xhat * c2));
+                    o.e[j] = narrow<E>(input_grad(gz[k * n + j], widen(w[k].e[j]), c1, xhat, c2, r));
                 }
                 store_vec<E, BYTES>(grad_x + item * cpg + c, o);
             }
@@ -493,7 +504,7 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
             Vec<E, BYTES> o;
 #pragma unroll
             for (int j = 0; j < n; ++j) {
-                o.e[j] = narrow<E>(r * (gz[k * n + j] * widen(w.e[j]) - c1 - xh[k * n + j] * c2));
+                o.e[j] = narrow<E>(input_grad(gz[k * n + j], widen(w.e[j]), c1, xh[k * n + j], c2, r));
             }
             store_vec<E, BYTES>(grad_x + s * P * C + static_cast<uint32_t>(p * C + c), o);
         }
@@ -644,7 +655,7 @@ gn_split_apply_kernel(const E* __restrict__ x, const E* __restrict__ weight, con
                 const A z = xhat * widen(w.e[j]) + widen(b.e[j]);
                 o.e[j] = narrow<E>(coefficients == nullptr
                                        ? act_value(z, act)
-                                       : r * (widen(d[u].e[j]) * act_slope(z, act) * widen(w.e[j]) - c1 - xhat * c2));
+                                       : input_grad(widen(d[u].e[j]) * act_slope(z, act), widen(w.e[j]), c1, xhat, c2, r));
             }
             store_vec<E, BYTES>(out + base + static_cast<int64_t>(p) * C, o);
         }

@@ -272,3 +272,20 @@ def test_refusals(sf):
 def test_a_host_tensor_is_refused(sf):
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         sf.gn_act_func(torch.zeros(2, 2, 4), torch.ones(4), torch.zeros(4), 2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("channels", [1, 6, 24, 128])
+def test_a_group_of_one_value_has_no_input_gradient(sf, channels, act, dtype):
+    """The value is its own mean: y is act(bias), and grad_y * w minus its mean over one value is exactly 0."""
+    gen = torch.Generator().manual_seed(channels)
+    x, gy = (torch.randn(7, 3, channels, generator=gen).to(dtype).cuda() for _ in range(2))
+    w, b = (torch.randn(channels, generator=gen).to(dtype).cuda() for _ in range(2))
+    x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    y = sf.gn_act_func(x, w, b, channels, EPS, act)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy)
+    assert torch.equal(y, y[:1, :1].expand_as(y))
+    assert torch.equal(gx, torch.zeros_like(gx))
+    assert torch.equal(gw, torch.zeros_like(gw))
