@@ -3,7 +3,8 @@
 //   forward    y[n, :] = scale * W[token[n], :]                       (a token outside [0, V): a row of zeros)
 //   backward   dW[v, :] = scale * sum over n with token[n] = v, in ascending n, of g[n, :]
 //
-// Both are bound by memory.  The forward reads and writes each row once.  The backward reads g once and
+// Both are bound by memory.  The forward reads and writes each row once (32768 tokens of 1024 bf16 columns: 17 us, 67 MB
+// written, most rows read from the caches).  The backward reads g once and
 // writes all V rows of dW (most of them zero for a large vocabulary); sums are held in 32 bits (64 for
 // double storage), always in the same order, so results are reproducible.
 //
@@ -13,10 +14,11 @@
 //      those below its rows -- where its part of the order begins -- and keeps those of its rows in LDS, from where
 //      it places them.  A wavefront that meets more of them than it can keep reads its tokens once more instead.
 //      32768 tokens, 50000 rows: 40 us with the second reading for all, 14 us with the lists.
-//   2. rows and pieces.  A row with at most kPiece positions is summed by the threads that own its columns.
-//      The positions of longer rows (frequent words) are cut at multiples of kPiece in the sorted order;
+//   2. rows and pieces.  A row with at most a piece's positions is summed by the threads that own its columns.
+//      The positions of longer rows (frequent words) are cut at multiples of a piece in the sorted order;
 //      every piece is summed by a workgroup of its own, in the same launch.
-//   3. merge.  The pieces of each long row, in order.  Not launched where N cannot hold a long row.
+//      The same sizes: 46 us (67 MB read, 102 MB written: 3.7 TB/s; a row's few reads follow each other).
+//   3. merge.  The pieces of each long row, in order (6 us).  Not launched where N cannot hold a long row.
 #include "seq_common.h"
 
 namespace snnseq {
@@ -25,8 +27,41 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kSortBlock = 1024;
 constexpr int kSortWaves = kSortBlock / 64;
-constexpr int kPiece = 64;        // positions of a row that one group of threads adds up by itself
 constexpr int kRowsInFlight = 4;  // rows requested before the first is used
+
+// Rows of any width start at any element: vectors of 16 bytes are moved from wherever they lie, and the last one of a
+// row begins where it ends with the row, sharing columns with the one before (both write the same values there).
+// Narrower vectors are for rows of fewer columns.
+template <typename E, int BYTES>
+struct Anywhere {
+    using type = typename Vec<E, BYTES>::raw_t __attribute__((aligned(sizeof(E))));
+};
+
+template <typename E, int BYTES>
+__device__ __forceinline__ Vec<E, BYTES> load_anywhere(const E* p) {
+    Vec<E, BYTES> v;
+    v.raw = *reinterpret_cast<const typename Anywhere<E, BYTES>::type*>(p);
+    return v;
+}
+
+template <typename E, int BYTES>
+__device__ __forceinline__ Vec<E, BYTES> load_anywhere_once(const E* p) {
+    Vec<E, BYTES> v;
+    v.raw = __builtin_nontemporal_load(reinterpret_cast<const typename Anywhere<E, BYTES>::type*>(p));
+    return v;
+}
+
+template <typename E, int BYTES>
+__device__ __forceinline__ void store_anywhere(E* p, const Vec<E, BYTES>& v) {
+    *reinterpret_cast<typename Anywhere<E, BYTES>::type*>(p) = v.raw;
+}
+
+template <typename E, int BYTES>
+__device__ __forceinline__ void store_anywhere_once(E* p, const Vec<E, BYTES>& v) {
+    __builtin_nontemporal_store(v.raw, reinterpret_cast<typename Anywhere<E, BYTES>::type*>(p));
+}
+
+__device__ __forceinline__ int at_most(int a, int b) { return a < b ? a : b; }
 
 template <typename I>
 __device__ __forceinline__ int row_of(const I* tokens, int64_t n, int V) {
@@ -52,12 +87,13 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ weight,
         const int64_t i = first + static_cast<int64_t>(r) * rows;
         row[r] = row_of(tokens, i < N ? i : N - 1, V);
     }
-    for (int c = lane * n; c < C; c += tpr * n) {
+    for (int c0 = lane * n; c0 < C; c0 += tpr * n) {
+        const int c = at_most(c0, C - n);
         Vec<E, BYTES> v[kRowsInFlight];
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r) {
             v[r].raw = typename Vec<E, BYTES>::raw_t(0);
-            if (row[r] >= 0) v[r] = load_vec<E, BYTES>(weight + row[r] * row_stride + c);
+            if (row[r] >= 0) v[r] = load_anywhere<E, BYTES>(weight + row[r] * row_stride + c);
         }
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r) {
@@ -68,7 +104,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ weight,
 #pragma unroll
                 for (int j = 0; j < n; ++j) v[r].e[j] = narrow<E>(scale * widen(v[r].e[j]));
             }
-            store_vec<E, BYTES>(out + i * C + c, v[r]);
+            store_anywhere<E, BYTES>(out + i * C + c, v[r]);
         }
     }
 }
@@ -226,14 +262,14 @@ __device__ __forceinline__ void add_rows(const E* __restrict__ grad, const int* 
         Vec<E, BYTES> v[kRowsInFlight];
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r)
-            v[r] = load_vec_once<E, BYTES>(grad + static_cast<int64_t>(position[j + r * step]) * C + c);
+            v[r] = load_anywhere_once<E, BYTES>(grad + static_cast<int64_t>(position[j + r * step]) * C + c);
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r)
 #pragma unroll
             for (int k = 0; k < n; ++k) acc[k] += widen(v[r].e[k]);
     }
     for (; j < to; j += step) {
-        const Vec<E, BYTES> v = load_vec_once<E, BYTES>(grad + static_cast<int64_t>(position[j]) * C + c);
+        const Vec<E, BYTES> v = load_anywhere_once<E, BYTES>(grad + static_cast<int64_t>(position[j]) * C + c);
 #pragma unroll
         for (int k = 0; k < n; ++k) acc[k] += widen(v.e[k]);
     }
@@ -244,7 +280,7 @@ __device__ __forceinline__ void store_row(E* p, const arith_t<E> (&acc)[Vec<E, B
     Vec<E, BYTES> v;
 #pragma unroll
     for (int k = 0; k < Vec<E, BYTES>::n; ++k) v.e[k] = narrow<E>(scale * acc[k]);
-    store_vec_once<E, BYTES>(p, v);
+    store_anywhere_once<E, BYTES>(p, v);
 }
 
 // The groups of a workgroup each hold a sum over every (kBlock/tpr)-th row of the same columns: adds them in order.
@@ -267,73 +303,75 @@ template <typename E, int BYTES>
 __global__ void __launch_bounds__(kBlock)
 embed_sum_kernel(const E* __restrict__ grad, const int* __restrict__ start, const int* __restrict__ position,
                  const int* __restrict__ row, E* __restrict__ grad_weight, arith_t<E>* __restrict__ part, int V,
-                 int C, arith_t<E> scale, int row_blocks, int tpr_log2) {
+                 int C, arith_t<E> scale, int row_blocks, int tpr_log2, int piece_log2) {
     using A = arith_t<E>;
     constexpr int n = Vec<E, BYTES>::n;
     __shared__ A shared[n][kBlock];
     const int tpr = 1 << tpr_log2;
     const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x >> tpr_log2, groups = kBlock >> tpr_log2;
+    const int c0 = (blockIdx.y * tpr + lane) * n, c = at_most(c0, C - n), piece = 1 << piece_log2;
     if (static_cast<int>(blockIdx.x) < row_blocks) {
         const int64_t v = static_cast<int64_t>(blockIdx.x) * groups + group;
         if (v >= V) return;
         const int from = start[v], to = start[v + 1];
-        if (to - from > kPiece) return;
-        for (int c = lane * n; c < C; c += tpr * n) {
-            A acc[n] = {};
-            add_rows<E, BYTES>(grad, position, from, to, 1, C, c, acc);
-            store_row<E, BYTES>(grad_weight + v * C + c, acc, scale);
-        }
+        if (to - from > piece) return;
+        if (c0 >= C) return;
+        A acc[n] = {};
+        add_rows<E, BYTES>(grad, position, from, to, 1, C, c, acc);
+        store_row<E, BYTES>(grad_weight + v * C + c, acc, scale);
         return;
     }
     const int p = blockIdx.x - row_blocks;
     const int end = start[V];
-    const int first = p * kPiece;
+    const int first = p * piece;
     if (first >= end) return;
-    const int last = first + kPiece < end ? first + kPiece : end;
+    const int last = first + piece < end ? first + piece : end;
     const int row_a = row[first], row_b = row[last - 1];
     for (int side = 0; side < 2; ++side) {
         const int r = side == 0 ? row_a : row_b;
         if (side == 1 && row_b == row_a) break;
         const int r_from = start[r], r_to = start[r + 1];
-        if (r_to - r_from <= kPiece) continue;
+        if (r_to - r_from <= piece) continue;
         const int from = r_from > first ? r_from : first, to = r_to < last ? r_to : last;
-        for (int c = lane * n; c - lane * n < C; c += tpr * n) {
-            A acc[n] = {};
-            if (c < C) add_rows<E, BYTES>(grad, position, from + group, to, groups, C, c, acc);
-            if (groups > 1) add_groups<A, n>(acc, shared, tpr, group, groups);
-            if (group == 0 && c < C) {
-                A* dst = part + (static_cast<int64_t>(p) * 2 + side) * C + c;
+        A acc[n] = {};
+        if (c0 < C) add_rows<E, BYTES>(grad, position, from + group, to, groups, C, c, acc);
+        if (groups > 1) add_groups<A, n>(acc, shared, tpr, group, groups);
+        if (group == 0 && c0 < C) {
+            A* dst = part + (static_cast<int64_t>(p) * 2 + side) * C + c;
 #pragma unroll
-                for (int k = 0; k < n; ++k) dst[k] = acc[k];
-            }
+            for (int k = 0; k < n; ++k) dst[k] = acc[k];
         }
     }
 }
 
-// Workgroup p: the long row that begins in piece p, if one does (the last row of the piece: a row of more than
-// kPiece positions ends behind the piece it begins in).
+// Most workgroups find no row and cost their launch, which wide ones are fewer for (32768 tokens of 1024 bf16 columns,
+// the whole gradient: 87.7 us with 128 columns each, 92.3 with 32); narrower ones have more threads for a long sum.
+constexpr int kMergeColumns = 128;
+
+// Workgroup p: the long row that begins in piece p, if one does (the last row of the piece: a row of more
+// positions than a piece ends behind the piece it begins in).
 template <typename E>
 __global__ void __launch_bounds__(kBlock)
 embed_merge_kernel(const int* __restrict__ start, const int* __restrict__ row, E* __restrict__ grad_weight,
-                   const arith_t<E>* __restrict__ part, int V, int C, arith_t<E> scale) {
+                   const arith_t<E>* __restrict__ part, int V, int C, arith_t<E> scale, int piece_log2) {
     using A = arith_t<E>;
-    constexpr int kColumns = 32, kGroups = kBlock / kColumns;
+    constexpr int kColumns = kMergeColumns, kGroups = kBlock / kColumns;
     __shared__ A shared[1][kBlock];
-    const int p = blockIdx.x;
+    const int p = blockIdx.x, piece = 1 << piece_log2;
     const int end = start[V];
-    const int first = p * kPiece;
+    const int first = p * piece;
     if (first >= end) return;
-    const int last = first + kPiece < end ? first + kPiece : end;
+    const int last = first + piece < end ? first + piece : end;
     const int r = row[last - 1];
     const int r_from = start[r], r_to = start[r + 1];
-    if (r_to - r_from <= kPiece || r_from < first) return;
+    if (r_to - r_from <= piece || r_from < first) return;
     const int lane = threadIdx.x & (kColumns - 1), group = threadIdx.x / kColumns;
     const int side = r_from == first ? 0 : 1;     // the row opens the piece or follows others
-    const int pieces = (r_to - 1) / kPiece - p + 1;
+    const int pieces = ((r_to - 1) >> piece_log2) - p + 1;
     const int c = blockIdx.y * kColumns + lane;
     A acc[1] = {A(0)};
     if (c < C) {
-#pragma unroll 4
+#pragma unroll 8
         for (int j = group; j < pieces; j += kGroups)
             acc[0] += part[(static_cast<int64_t>(p + j) * 2 + (j == 0 ? side : 0)) * C + c];
     }
@@ -353,21 +391,36 @@ int log2_threads_per_row(int64_t vectors) {
 template <typename E, int BYTES, typename I>
 hipError_t forward_as(const void* tokens, const void* weight, void* out, int64_t N, int64_t V, int64_t C,
                       int64_t row_stride, double scale, hipStream_t st) {
-    const int l = log2_threads_per_row(C / Vec<E, BYTES>::n);
+    const int l = log2_threads_per_row(ceil_div(C, Vec<E, BYTES>::n));
     const int64_t rows = int64_t(kBlock >> l) * kRowsInFlight;
     return launch(embed_forward_kernel<E, BYTES, I>, dim3(static_cast<unsigned>(ceil_div(N, rows))), dim3(kBlock), st,
                   static_cast<const I*>(tokens), static_cast<const E*>(weight), static_cast<E*>(out), N,
                   static_cast<int>(V), static_cast<int>(C), row_stride, static_cast<arith_t<E>>(scale), l);
 }
 
+// Bytes of the widest vector that a row of C elements holds.
+int widest(int64_t C, size_t es) {
+    int bytes = 16;
+    while (bytes > C * static_cast<int64_t>(es)) bytes /= 2;
+    return bytes;
+}
+
 struct Layout {  // byte offsets into the workspace
     size_t start, position, row, part, bytes;
     int64_t pieces;
+    int piece_log2;
 };
+
+// Positions of a row that one group of threads adds up by itself, one after another.  With few tokens the longest such
+// sum is all there is to wait for, with many the sums of the pieces cost more than they save.  Backward with pieces of
+// 16, 32 and 64: 1805 tokens of 2002 bf16 columns 20.6, 24 and 31 us, 6270 of 973 fp32 columns 39, 41 and 48, 16384 of
+// 1024 bf16 columns 67, 64 and 66, 32768 of them 100, 92 and 91.
+int piece_log2_of(int64_t N) { return N <= 8192 ? 4 : 5; }
 
 Layout layout_of(int64_t N, int64_t V, int64_t C, size_t arith) {
     Layout w;
-    w.pieces = N > kPiece ? ceil_div(N, kPiece) : 0;
+    w.piece_log2 = piece_log2_of(N);
+    w.pieces = N > 1 << w.piece_log2 ? ceil_div(N, 1 << w.piece_log2) : 0;
     w.start = 0;
     w.position = round_up(w.start + sizeof(int) * static_cast<size_t>(V + 1), 16);
     w.row = round_up(w.position + sizeof(int) * static_cast<size_t>(N), 16);
@@ -380,20 +433,21 @@ template <typename E, int BYTES>
 hipError_t sums_as(const void* grad, void* grad_weight, char* ws, const Layout& w, int64_t V, int64_t C, double scale,
                    hipStream_t st) {
     using A = arith_t<E>;
-    const int l = log2_threads_per_row(C / Vec<E, BYTES>::n);
+    const int l = log2_threads_per_row(ceil_div(C, Vec<E, BYTES>::n));
     const int64_t row_blocks = ceil_div(V, kBlock >> l);
     const int* start = reinterpret_cast<int*>(ws + w.start);
     const int* position = reinterpret_cast<int*>(ws + w.position);
     const int* row = reinterpret_cast<int*>(ws + w.row);
     A* part = reinterpret_cast<A*>(ws + w.part);
-    hipError_t err = launch(embed_sum_kernel<E, BYTES>, dim3(static_cast<unsigned>(row_blocks + w.pieces)),
-                            dim3(kBlock), st, static_cast<const E*>(grad), start, position, row,
+    const dim3 grid(static_cast<unsigned>(row_blocks + w.pieces),
+                    static_cast<unsigned>(ceil_div(C, int64_t(Vec<E, BYTES>::n) << l)));
+    hipError_t err = launch(embed_sum_kernel<E, BYTES>, grid, dim3(kBlock), st, static_cast<const E*>(grad), start, position, row,
                             static_cast<E*>(grad_weight), part, static_cast<int>(V), static_cast<int>(C),
-                            static_cast<A>(scale), static_cast<int>(row_blocks), l);
+                            static_cast<A>(scale), static_cast<int>(row_blocks), l, w.piece_log2);
     if (err == hipSuccess && w.pieces > 0)
-        err = launch(embed_merge_kernel<E>, dim3(static_cast<unsigned>(w.pieces), static_cast<unsigned>(ceil_div(C, 32))),
+        err = launch(embed_merge_kernel<E>, dim3(static_cast<unsigned>(w.pieces), static_cast<unsigned>(ceil_div(C, kMergeColumns))),
                      dim3(kBlock), st, start, row, static_cast<E*>(grad_weight), const_cast<const A*>(part),
-                     static_cast<int>(V), static_cast<int>(C), static_cast<A>(scale));
+                     static_cast<int>(V), static_cast<int>(C), static_cast<A>(scale), w.piece_log2);
     return err;
 }
 
@@ -436,7 +490,7 @@ extern "C" int snnseq_embed_fp(const void* tokens, const void* weight, void* out
     if (!aligned_to(tokens, token_dtype == SNNSEQ_TOKEN_I32 ? 4 : 8) || !aligned_to(weight, es) || !aligned_to(out, es))
         return SNNLIF_ERR_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int bytes = common_bytes(address(weight), address(out), C * es, static_cast<uint64_t>(row_stride) * es);
+    const int bytes = widest(C, es);
     const bool wide = token_dtype == SNNSEQ_TOKEN_I64;
 #define SNNSEQ_FORWARD(E, B)                                                                                     \
     (wide ? forward_as<E, B, int64_t>(tokens, weight, out, N, V, C, row_stride, scale, st)                       \
@@ -478,7 +532,7 @@ extern "C" int snnseq_embed_bp(const void* tokens, const void* grad, void* grad_
     hipError_t err = token_dtype == SNNSEQ_TOKEN_I64 ? order_as<int64_t>(tokens, N, V, ws, w, st)
                                                      : order_as<int32_t>(tokens, N, V, ws, w, st);
     if (err != hipSuccess) return static_cast<int>(err);
-    const int bytes = common_bytes(address(grad), address(grad_weight), C * es);
+    const int bytes = widest(C, es);
 #define SNNSEQ_SUMS(E, B) sums_as<E, B>(grad, grad_weight, ws, w, V, C, scale, st)
     if (dtype == SNNLIF_DTYPE_F32)
         err = bytes == 16 ? SNNSEQ_SUMS(float, 16) : bytes == 8 ? SNNSEQ_SUMS(float, 8) : SNNSEQ_SUMS(float, 4);

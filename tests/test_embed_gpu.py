@@ -209,3 +209,46 @@ def test_refusals(sf):
 def test_a_host_tensor_is_refused(sf):
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         sf.embed_func(torch.zeros(2, 2, dtype=torch.long), torch.zeros(4, 3))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("C", [2, 5, 7, 9, 15, 17, 31, 33, 513, 2049])
+def test_rows_that_start_and_end_inside_a_vector(sf, C, dtype):
+    check(sf, *make((19, 5), 23, C, dtype, seed=C, pad=0.1), scale=-0.7)
+
+
+@gpu
+@pytest.mark.parametrize("shift", [1, 3])
+def test_neighbours_of_rows_at_odd_addresses_stay_as_they_are(sf, shift):
+    """The gradient written into storage one and three elements off a boundary, with values before and behind it."""
+    from snn_gpu_training_bptt_amd import seq_cabi
+    V, C, N = 11, 21, 37
+    tokens, _, grad = make((N, 1), V, C, torch.bfloat16, seed=shift)
+    held = torch.full((V * C + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = held[shift:shift + V * C].view(V, C)
+    g = torch.zeros(N * C + shift, dtype=torch.bfloat16, device="cuda")[shift:].view(N, C)
+    g.copy_(grad.reshape(N, C))
+    need = seq_cabi.load().snnseq_embed_bp_workspace_bytes(2, N, V, C)
+    seq_cabi.embed_bp_into(tokens.reshape(-1).cuda(), g, out, 1.0, torch.empty(need, dtype=torch.uint8, device="cuda"))
+    plain = torch.zeros(V, C, dtype=torch.float64).index_add_(0, tokens.reshape(-1), grad.reshape(N, C).double())
+    mag = torch.zeros(V, C, dtype=torch.float64).index_add_(0, tokens.reshape(-1), grad.reshape(N, C).double().abs())
+    assert bool(((out.cpu().double() - plain).abs() <= mag * N * 2.0 ** -24 + plain.abs() * 2.0 ** -8).all())
+    assert bool((held[:shift] == 7).all()) and bool((held[shift + V * C:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("n", [15, 16, 17, 31, 33, 8192, 8193])
+def test_one_row_around_the_ends_of_pieces(sf, n):
+    tokens, weight, grad = make((n, 1), 5, 12, torch.float32, seed=n)
+    check(sf, torch.full_like(tokens, 3), weight, grad)
+
+
+@gpu
+def test_short_batches_of_long_rows_that_begin_and_end_anywhere(sf):
+    gen = torch.Generator().manual_seed(8)
+    counts = [1, 16, 17, 14, 18, 50, 3, 100, 16, 32, 33, 1, 20, 20, 20]
+    tokens = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts))
+    tokens = tokens[torch.randperm(tokens.numel(), generator=gen)].reshape(-1, 1)
+    grad = torch.randn(*tokens.shape, 50, generator=gen)
+    check(sf, tokens, torch.randn(len(counts) + 2, 50, generator=gen), grad, scale=0.5)
