@@ -40,7 +40,7 @@ template <> __device__ __forceinline__ bf16_t narrow<bf16_t>(float v) {
     return bf16_t{__builtin_bit_cast(uint16_t, r)};
 }
 
-// BYTES consecutive bytes of storage type E, moved with one memory instruction.
+// BYTES consecutive bytes of storage type E, moved with one memory instruction, from any element on.
 template <int BYTES> struct RawOf;
 template <> struct RawOf<2> { using type = uint16_t; };
 template <> struct RawOf<4> { using type = uint32_t; };
@@ -51,6 +51,7 @@ template <typename E, int BYTES>
 struct Vec {
     static constexpr int n = BYTES / static_cast<int>(sizeof(E));
     using raw_t = typename RawOf<BYTES>::type;
+    using memory_t = raw_t __attribute__((aligned(sizeof(E))));
     union {
         raw_t raw;
         E e[n];
@@ -60,7 +61,7 @@ struct Vec {
 template <typename E, int BYTES>
 __device__ __forceinline__ Vec<E, BYTES> load_vec(const E* p) {
     Vec<E, BYTES> v;
-    v.raw = *reinterpret_cast<const typename Vec<E, BYTES>::raw_t*>(p);
+    v.raw = *reinterpret_cast<const typename Vec<E, BYTES>::memory_t*>(p);
     return v;
 }
 
@@ -68,7 +69,7 @@ __device__ __forceinline__ Vec<E, BYTES> load_vec(const E* p) {
 template <typename E, int BYTES>
 __device__ __forceinline__ Vec<E, BYTES> load_vec_once(const E* p) {
     Vec<E, BYTES> v;
-    v.raw = __builtin_nontemporal_load(reinterpret_cast<const typename Vec<E, BYTES>::raw_t*>(p));
+    v.raw = __builtin_nontemporal_load(reinterpret_cast<const typename Vec<E, BYTES>::memory_t*>(p));
     return v;
 }
 
@@ -91,12 +92,20 @@ __device__ __forceinline__ Vec<E, BYTES> load_or_zero(const E* p, I at, bool pre
 
 template <typename E, int BYTES>
 __device__ __forceinline__ void store_vec(E* p, const Vec<E, BYTES>& v) {
-    *reinterpret_cast<typename Vec<E, BYTES>::raw_t*>(p) = v.raw;
+    *reinterpret_cast<typename Vec<E, BYTES>::memory_t*>(p) = v.raw;
 }
 
 template <typename E, int BYTES>
 __device__ __forceinline__ void store_vec_once(E* p, const Vec<E, BYTES>& v) {
-    __builtin_nontemporal_store(v.raw, reinterpret_cast<typename Vec<E, BYTES>::raw_t*>(p));
+    __builtin_nontemporal_store(v.raw, reinterpret_cast<typename Vec<E, BYTES>::memory_t*>(p));
+}
+
+// Bytes of the widest vector that `count` elements hold.  Rows and groups of any size are covered by such vectors: the
+// last begins where it ends with them, and shares elements with the one before.
+inline int widest_vector(int64_t count, size_t element_bytes) {
+    int bytes = 16;
+    while (bytes > count * static_cast<int64_t>(element_bytes)) bytes /= 2;
+    return bytes;
 }
 
 // Largest power of two of at most 16 that divides every argument: how many bytes one access may move.

@@ -29,38 +29,7 @@ constexpr int kSortBlock = 1024;
 constexpr int kSortWaves = kSortBlock / 64;
 constexpr int kRowsInFlight = 4;  // rows requested before the first is used
 
-// Rows of any width start at any element: vectors of 16 bytes are moved from wherever they lie, and the last one of a
-// row begins where it ends with the row, sharing columns with the one before (both write the same values there).
-// Narrower vectors are for rows of fewer columns.
-template <typename E, int BYTES>
-struct Anywhere {
-    using type = typename Vec<E, BYTES>::raw_t __attribute__((aligned(sizeof(E))));
-};
-
-template <typename E, int BYTES>
-__device__ __forceinline__ Vec<E, BYTES> load_anywhere(const E* p) {
-    Vec<E, BYTES> v;
-    v.raw = *reinterpret_cast<const typename Anywhere<E, BYTES>::type*>(p);
-    return v;
-}
-
-template <typename E, int BYTES>
-__device__ __forceinline__ Vec<E, BYTES> load_anywhere_once(const E* p) {
-    Vec<E, BYTES> v;
-    v.raw = __builtin_nontemporal_load(reinterpret_cast<const typename Anywhere<E, BYTES>::type*>(p));
-    return v;
-}
-
-template <typename E, int BYTES>
-__device__ __forceinline__ void store_anywhere(E* p, const Vec<E, BYTES>& v) {
-    *reinterpret_cast<typename Anywhere<E, BYTES>::type*>(p) = v.raw;
-}
-
-template <typename E, int BYTES>
-__device__ __forceinline__ void store_anywhere_once(E* p, const Vec<E, BYTES>& v) {
-    __builtin_nontemporal_store(v.raw, reinterpret_cast<typename Anywhere<E, BYTES>::type*>(p));
-}
-
+// The last vector of a row shares columns with the one before: both write the same values there.
 __device__ __forceinline__ int at_most(int a, int b) { return a < b ? a : b; }
 
 template <typename I>
@@ -93,7 +62,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ weight,
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r) {
             v[r].raw = typename Vec<E, BYTES>::raw_t(0);
-            if (row[r] >= 0) v[r] = load_anywhere<E, BYTES>(weight + row[r] * row_stride + c);
+            if (row[r] >= 0) v[r] = load_vec<E, BYTES>(weight + row[r] * row_stride + c);
         }
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r) {
@@ -104,7 +73,7 @@ embed_forward_kernel(const I* __restrict__ tokens, const E* __restrict__ weight,
 #pragma unroll
                 for (int j = 0; j < n; ++j) v[r].e[j] = narrow<E>(scale * widen(v[r].e[j]));
             }
-            store_anywhere<E, BYTES>(out + i * C + c, v[r]);
+            store_vec<E, BYTES>(out + i * C + c, v[r]);
         }
     }
 }
@@ -262,14 +231,14 @@ __device__ __forceinline__ void add_rows(const E* __restrict__ grad, const int* 
         Vec<E, BYTES> v[kRowsInFlight];
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r)
-            v[r] = load_anywhere_once<E, BYTES>(grad + static_cast<int64_t>(position[j + r * step]) * C + c);
+            v[r] = load_vec_once<E, BYTES>(grad + static_cast<int64_t>(position[j + r * step]) * C + c);
 #pragma unroll
         for (int r = 0; r < kRowsInFlight; ++r)
 #pragma unroll
             for (int k = 0; k < n; ++k) acc[k] += widen(v[r].e[k]);
     }
     for (; j < to; j += step) {
-        const Vec<E, BYTES> v = load_anywhere_once<E, BYTES>(grad + static_cast<int64_t>(position[j]) * C + c);
+        const Vec<E, BYTES> v = load_vec_once<E, BYTES>(grad + static_cast<int64_t>(position[j]) * C + c);
 #pragma unroll
         for (int k = 0; k < n; ++k) acc[k] += widen(v.e[k]);
     }
@@ -280,7 +249,7 @@ __device__ __forceinline__ void store_row(E* p, const arith_t<E> (&acc)[Vec<E, B
     Vec<E, BYTES> v;
 #pragma unroll
     for (int k = 0; k < Vec<E, BYTES>::n; ++k) v.e[k] = narrow<E>(scale * acc[k]);
-    store_anywhere_once<E, BYTES>(p, v);
+    store_vec_once<E, BYTES>(p, v);
 }
 
 // The groups of a workgroup each hold a sum over every (kBlock/tpr)-th row of the same columns: adds them in order.
@@ -398,13 +367,6 @@ hipError_t forward_as(const void* tokens, const void* weight, void* out, int64_t
                   static_cast<int>(V), static_cast<int>(C), row_stride, static_cast<arith_t<E>>(scale), l);
 }
 
-// Bytes of the widest vector that a row of C elements holds.
-int widest(int64_t C, size_t es) {
-    int bytes = 16;
-    while (bytes > C * static_cast<int64_t>(es)) bytes /= 2;
-    return bytes;
-}
-
 struct Layout {  // byte offsets into the workspace
     size_t start, position, row, part, bytes;
     int64_t pieces;
@@ -490,7 +452,7 @@ extern "C" int snnseq_embed_fp(const void* tokens, const void* weight, void* out
     if (!aligned_to(tokens, token_dtype == SNNSEQ_TOKEN_I32 ? 4 : 8) || !aligned_to(weight, es) || !aligned_to(out, es))
         return SNNLIF_ERR_ALIGN;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int bytes = widest(C, es);
+    const int bytes = widest_vector(C, es);
     const bool wide = token_dtype == SNNSEQ_TOKEN_I64;
 #define SNNSEQ_FORWARD(E, B)                                                                                     \
     (wide ? forward_as<E, B, int64_t>(tokens, weight, out, N, V, C, row_stride, scale, st)                       \
@@ -532,7 +494,7 @@ extern "C" int snnseq_embed_bp(const void* tokens, const void* grad, void* grad_
     hipError_t err = token_dtype == SNNSEQ_TOKEN_I64 ? order_as<int64_t>(tokens, N, V, ws, w, st)
                                                      : order_as<int32_t>(tokens, N, V, ws, w, st);
     if (err != hipSuccess) return static_cast<int>(err);
-    const int bytes = widest(C, es);
+    const int bytes = widest_vector(C, es);
 #define SNNSEQ_SUMS(E, B) sums_as<E, B>(grad, grad_weight, ws, w, V, C, scale, st)
     if (dtype == SNNLIF_DTYPE_F32)
         err = bytes == 16 ? SNNSEQ_SUMS(float, 16) : bytes == 8 ? SNNSEQ_SUMS(float, 8) : SNNSEQ_SUMS(float, 4);

@@ -9,14 +9,18 @@
 // grad_x).  Three layouts reach or approach that:
 //   rows   P == 1 and a group of at most 4 vectors per lane: a group is one run of memory.  L lanes (a power of two)
 //          own it, hold it in registers and reduce by shuffles.  In the backward a lane keeps its channels over many
-//          samples, so the channel sums stay in registers.
+//          samples, so the channel sums stay in registers.  [16384, 8 groups of 128] bf16 silu: forward 21 us (67 MB:
+//          3.2 TB/s, bound by the exponentials' arithmetic and latency), backward 31 us (101 MB: 3.2 TB/s).
 //   slab   the P rows of a bundle of groups fit the registers of a workgroup: read once, reduced through LDS, written
 //          once.  A bundle is as many groups as make a row segment of 128 bytes, a memory line (64 where 128 do not fit).
+//          [8 64 32 32 128] fp32: forward 97 us (537 MB: 5.5 TB/s), backward 219 us (805 MB: 3.7 TB/s; 1024 threads with
+//          all their registers, one workgroup per CU, so that a sample's loads overlap only with the sums before).
 //   split  larger: partial sums over slices of the positions, a small kernel that combines them, and a second read
 //          of the inputs in the pass that writes.
 // Statistics and sums are held in 32 bits (64 for double storage, and in the split layout's statistics); the variance is taken
 // around the mean, in a second sweep over the registers, or around one of the group's values in 64 bits (split).
-// Every sum has a fixed order.
+// Every sum has a fixed order.  Groups of any size, wherever they lie, are covered by vectors of 16 bytes (Spot): [7455,
+// 32 groups of 111] fp32 takes 134 us forward and backward, 235 with single values.
 #include "seq_common.h"
 
 namespace snnseq {
@@ -77,13 +81,29 @@ __device__ __forceinline__ A input_grad(A gz, A w, A c1, A xhat, A c2, A rstd) {
     return rstd * (h - c1 - xhat * c2);
 }
 
+// The `index`-th vector of a group of cpg channels: its first channel within the group, and how many of its values the
+// vector before has too.  Those are computed and stored by both, and counted in sums by the one before.
+// RAGGED: cpg is no multiple of the vector; otherwise `skip` is 0 and costs nothing.
+template <int n, bool RAGGED>
+struct Spot {
+    int first, skip;
+    __device__ __forceinline__ Spot(int index, int cpg) {
+        const int c = index * n;
+        first = RAGGED && c > cpg - n ? cpg - n : c;
+        skip = c - first;
+    }
+    template <typename A>
+    __device__ __forceinline__ A counted(int j, A value) const { return RAGGED && j < skip ? A(0) : value; }
+    __device__ __forceinline__ bool counts(int j) const { return !RAGGED || j >= skip; }
+};
+
 // ---- rows ---------------------------------------------------------------------------------------
 
 constexpr int kRowsBlock = 256;
 
 // U items (sample, group), `step` apart, per group of L lanes: all of them requested before the first is looked at.
 // `step` is a multiple of G, so that they share their channels' weights.
-template <typename E, int BYTES, int K, int U>
+template <typename E, int BYTES, bool RAGGED, int K, int U>
 __global__ void __launch_bounds__(kRowsBlock)
 gn_rows_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                        E* __restrict__ y, arith_t<E>* __restrict__ mean, arith_t<E>* __restrict__ rstd, int64_t items,
@@ -100,15 +120,15 @@ gn_rows_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c = (k * L + lane) * n;
             const int64_t item = first + u * step;
-            v[u][k] = load_or_zero<E, BYTES>(x, item * cpg + c, c < cpg && item < items, true);
+            v[u][k] = load_or_zero<E, BYTES>(x, item * cpg + Spot<n, RAGGED>(k * L + lane, cpg).first,
+                                             (k * L + lane) * n < cpg && item < items, true);
         }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int c = (k * L + lane) * n;
-        w[k] = load_or_zero<E, BYTES>(weight, g * cpg + c, c < cpg, false);
-        b[k] = load_or_zero<E, BYTES>(bias, g * cpg + c, c < cpg, false);
+        const int c = Spot<n, RAGGED>(k * L + lane, cpg).first;
+        w[k] = load_or_zero<E, BYTES>(weight, g * cpg + c, (k * L + lane) * n < cpg, false);
+        b[k] = load_or_zero<E, BYTES>(bias, g * cpg + c, (k * L + lane) * n < cpg, false);
     }
     const A per = A(1) / A(cpg);
 #pragma unroll
@@ -117,18 +137,21 @@ gn_rows_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
         if (item >= items) return;
         A sum = A(0);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            const Spot<n, RAGGED> spot(k * L + lane, cpg);
 #pragma unroll
-            for (int j = 0; j < n; ++j) sum += widen(v[u][k].e[j]);  // absent values are zero
+            for (int j = 0; j < n; ++j) sum += spot.counted(j, widen(v[u][k].e[j]));  // absent values are zero
+        }
         const A m = lanes_sum(sum, L) * per;
         A sq = A(0);
 #pragma unroll
         for (int k = 0; k < K; ++k)
             if ((k * L + lane) * n < cpg) {
+                const Spot<n, RAGGED> spot(k * L + lane, cpg);
 #pragma unroll
                 for (int j = 0; j < n; ++j) {
                     const A d = widen(v[u][k].e[j]) - m;
-                    sq += d * d;
+                    sq += spot.counted(j, d * d);
                 }
             }
         const A r = inverse_root(lanes_sum(sq, L) * per + eps);
@@ -138,20 +161,19 @@ gn_rows_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
         }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c = (k * L + lane) * n;
-            if (c >= cpg) continue;
+            if ((k * L + lane) * n >= cpg) continue;
             Vec<E, BYTES> o;
 #pragma unroll
             for (int j = 0; j < n; ++j)
                 o.e[j] = narrow<E>(act_value((widen(v[u][k].e[j]) - m) * r * widen(w[k].e[j]) + widen(b[k].e[j]), act));
-            store_vec<E, BYTES>(y + item * cpg + c, o);
+            store_vec<E, BYTES>(y + item * cpg + Spot<n, RAGGED>(k * L + lane, cpg).first, o);
         }
     }
 }
 
 // Groups of L lanes: `gpb` groups of channels (blockIdx.y names which) times `spb` samples at a time; blockIdx.x is
 // the sample slice.  part [slices][2][C]: sums of gz * xhat, then of gz.
-template <typename E, int BYTES, int K>
+template <typename E, int BYTES, bool RAGGED, int K>
 __global__ void __launch_bounds__(kRowsBlock)
 gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                         const arith_t<E>* __restrict__ mean, const arith_t<E>* __restrict__ rstd,
@@ -171,9 +193,9 @@ gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
         Vec<E, BYTES> w[K], b[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c = (k * L + lane) * n;
+            const int c = Spot<n, RAGGED>(k * L + lane, cpg).first;
             w[k].raw = b[k].raw = typename Vec<E, BYTES>::raw_t(0);
-            if (c < cpg) {
+            if ((k * L + lane) * n < cpg) {
                 w[k] = load_vec<E, BYTES>(weight + g * cpg + c);
                 b[k] = load_vec<E, BYTES>(bias + g * cpg + c);
             }
@@ -186,9 +208,9 @@ gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
             const int64_t item = (at < S ? at : s) * G + g;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (k * L + lane) * n;
+                const int c = Spot<n, RAGGED>(k * L + lane, cpg).first;
                 v_next[k].raw = d_next[k].raw = typename Vec<E, BYTES>::raw_t(0);
-                if (c < cpg) {
+                if ((k * L + lane) * n < cpg) {
                     v_next[k] = load_vec_once<E, BYTES>(x + item * cpg + c);
                     d_next[k] = load_vec_once<E, BYTES>(grad + item * cpg + c);
                 }
@@ -209,32 +231,33 @@ gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
             request(s + hop);
             A gz[K * n], c1 = A(0), c2 = A(0);
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k) {
+                const Spot<n, RAGGED> spot(k * L + lane, cpg);
 #pragma unroll
                 for (int j = 0; j < n; ++j) {
                     const A xhat = (widen(v[k].e[j]) - m) * r;
                     const A t = widen(d[k].e[j]) * act_slope(xhat * widen(w[k].e[j]) + widen(b[k].e[j]), act);
                     gz[k * n + j] = t;  // zero where there is no channel
-                    if ((k * L + lane) * n < cpg) {
+                    if ((k * L + lane) * n < cpg && spot.counts(j)) {
                         acc_a[k * n + j] += t * xhat;
                         acc_b[k * n + j] += t;
                         c1 += t * widen(w[k].e[j]);
                         c2 += t * widen(w[k].e[j]) * xhat;
                     }
                 }
+            }
             c1 = lanes_sum(c1, L) / A(cpg);
             c2 = lanes_sum(c2, L) / A(cpg);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (k * L + lane) * n;
-                if (c >= cpg) continue;
+                if ((k * L + lane) * n >= cpg) continue;
                 Vec<E, BYTES> o;
 #pragma unroll
                 for (int j = 0; j < n; ++j) {
                     const A xhat = (widen(v[k].e[j]) - m) * r;
                     o.e[j] = narrow<E>(input_grad(gz[k * n + j], widen(w[k].e[j]), c1, xhat, c2, r));
                 }
-                store_vec<E, BYTES>(grad_x + item * cpg + c, o);
+                store_vec<E, BYTES>(grad_x + item * cpg + Spot<n, RAGGED>(k * L + lane, cpg).first, o);
             }
         }
     }
@@ -255,8 +278,9 @@ gn_rows_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
                     if (sample == 0)
                         for (int o = 1; o < spb; ++o) v += shared[threadIdx.x + o * gpb * L];
                 }
-                const int c = (k * L + lane) * n + j;
-                if (here && sample == 0 && c < cpg) row[which * C + g * cpg + c] = v;
+                const Spot<n, RAGGED> spot(k * L + lane, cpg);
+                if (here && sample == 0 && (k * L + lane) * n < cpg && spot.counts(j))
+                    row[which * C + g * cpg + spot.first + j] = v;
             }
 }
 
@@ -300,18 +324,33 @@ __device__ __forceinline__ int64_t piece_of_work() {
     return blockIdx.x < per * 8 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
 }
 
-// sm[q][tid] (q < Q, rows of `cols` threads): adds the rows up; the sums are left in sm[q][0 .. cols).
+// sm[q][tid] (q < Q, rows of `cols` threads): adds the rows up; the sums are left in sm[q][0 .. cols).  Eight rows become
+// one in a step.  All threads share the Q * kept * cols sums of a step, and the values of one are requested together:
+// with Q sums one after another in the threads that keep a row, the backward of [205 samples, 220 positions, 9 groups
+// of 43] bf16 took 171 us instead of 82.  The forward's single sum has too few to share and wants its registers.
 template <typename A, int Q, int BT>
 __device__ __forceinline__ void fold_rows(A (*sm)[BT], int rows, int cols, int tid) {
     __syncthreads();
     while (rows > 1) {
-        const int kept = (rows + 7) >> 3;
-        if (tid < kept * cols) {
+        const int kept = (rows + 7) >> 3, slots = kept * cols, end = rows * cols;
+        if constexpr (Q == 1) {
+            if (tid < slots) {
+                A s = sm[0][tid];
+                for (int r = tid + slots; r < end; r += slots) s += sm[0][r];
+                sm[0][tid] = s;
+            }
+        } else {
+            for (int i = tid; i < Q * slots; i += BT) {
+                const int q = i / slots, slot = i - q * slots;
+                A s = sm[q][slot], v[7];
 #pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                A s = sm[q][tid];
-                for (int r = tid + kept * cols; r < rows * cols; r += kept * cols) s += sm[q][r];
-                sm[q][tid] = s;
+                for (int r = 0; r < 7; ++r) {
+                    const int at = slot + (r + 1) * slots;
+                    v[r] = at < end ? sm[q][at] : A(0);
+                }
+#pragma unroll
+                for (int r = 0; r < 7; ++r) s += v[r];
+                sm[q][slot] = s;
             }
         }
         rows = kept;
@@ -347,7 +386,7 @@ __device__ __forceinline__ Bundle bundle_of(int bundle, int gpb, int G, int vpg)
 }
 
 // Workgroup (sample, bundle of `gpb` groups); vpg = vectors per group and position.
-template <typename E, int BYTES, int BT>
+template <typename E, int BYTES, bool RAGGED, int BT>
 __global__ void __launch_bounds__(BT)
 gn_slab_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                        E* __restrict__ y, arith_t<E>* __restrict__ mean, arith_t<E>* __restrict__ rstd, int bundles,
@@ -355,11 +394,12 @@ gn_slab_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
     using A = arith_t<E>;
     constexpr int n = Vec<E, BYTES>::n, K = held_vectors(sizeof(E), n, BT, false);
     __shared__ A sm[1][BT];
-    const int vpg = cpg / n, C = G * cpg;
+    const int vpg = (cpg + n - 1) / n, C = G * cpg;
     const int64_t piece = piece_of_work();
     const int64_t s = piece / bundles;
     const Bundle t = bundle_of<BT>(static_cast<int>(piece - s * bundles), gpb, G, vpg);
-    const int c = t.first_group * cpg + t.col * n;
+    const Spot<n, RAGGED> spot(t.col - t.group * vpg, cpg);
+    const int c = (t.first_group + t.group) * cpg + spot.first;
     const E* px = x + s * P * C;  // one sample is below 2 GiB: 32-bit offsets from here
     Vec<E, BYTES> v[K];
     A sum = A(0);
@@ -371,7 +411,7 @@ gn_slab_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < n; ++j) sum += widen(v[k].e[j]);
+        for (int j = 0; j < n; ++j) sum += spot.counted(j, widen(v[k].e[j]));
     sm[0][threadIdx.x] = sum;
     fold_rows<A, 1, BT>(sm, t.rows, t.cols, threadIdx.x);
     const A count = A(P) * A(cpg);
@@ -384,7 +424,7 @@ gn_slab_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
 #pragma unroll
             for (int j = 0; j < n; ++j) {
                 const A d = widen(v[k].e[j]) - m;
-                sq += d * d;
+                sq += spot.counted(j, d * d);
             }
         }
     sm[0][threadIdx.x] = sq;
@@ -409,7 +449,7 @@ gn_slab_forward_kernel(const E* __restrict__ x, const E* __restrict__ weight, co
 }
 
 // Workgroup (slice of the samples, bundle): samples slice, slice + slices, ...; part [slices][2][C].
-template <typename E, int BYTES, int BT>
+template <typename E, int BYTES, bool RAGGED, int BT>
 __global__ void __launch_bounds__(BT)
 gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                         const arith_t<E>* __restrict__ mean, const arith_t<E>* __restrict__ rstd,
@@ -418,11 +458,12 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
     using A = arith_t<E>;
     constexpr int n = Vec<E, BYTES>::n, K = held_vectors(sizeof(E), n, BT, true);
     __shared__ A sm[2 * n][BT];
-    const int vpg = cpg / n, C = G * cpg;
+    const int vpg = (cpg + n - 1) / n, C = G * cpg;
     const int64_t piece = piece_of_work();
     const int slice = static_cast<int>(piece / bundles);
     const Bundle t = bundle_of<BT>(static_cast<int>(piece - static_cast<int64_t>(slice) * bundles), gpb, G, vpg);
-    const int c = t.first_group * cpg + t.col * n;
+    const Spot<n, RAGGED> spot(t.col - t.group * vpg, cpg);
+    const int c = (t.first_group + t.group) * cpg + spot.first;
     const int first_col = t.here ? t.group * vpg : 0;
     const A count = A(P) * A(cpg);
     Vec<E, BYTES> w, b;
@@ -435,9 +476,10 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
     Vec<E, BYTES> v[K], d[K];
     A m_next = A(0), r_next = A(0);
     // The one workgroup of 1024 threads that a CU holds requests a sample while the one before is summed up and stored
-    // ([8 64 32 32 128] fp32: 267 us, 301 without); smaller ones overlap each other, and the registers are theirs.
+    // ([8 64 32 32 128] fp32, with the sums one after another: 267 us, 301 without); smaller ones overlap each other, and the registers are theirs.
     // What does not exist is read at the slab's beginning and left out below.
-    constexpr bool kRequestAhead = BT == 1024 && sizeof(E) == 4;
+    // Narrow vectors (more addresses) and counting have no registers for it.
+    constexpr bool kRequestAhead = BT == 1024 && sizeof(E) == 4 && BYTES == 16 && !RAGGED;
     const auto request = [&](int64_t s) {
         const E *px = x + s * P * C, *pg = grad + s * P * C;
 #pragma unroll
@@ -464,7 +506,7 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
             for (int j = 0; j < n; ++j) {
                 const A xhat = (widen(v[k].e[j]) - m) * r;
                 const A q = widen(d[k].e[j]) * act_slope(xhat * widen(w.e[j]) + widen(b.e[j]), act);
-                const bool valid = t.here && t.row + k * t.rows < P;
+                const bool valid = t.here && t.row + k * t.rows < P && spot.counts(j);
                 xh[k * n + j] = xhat;
                 gz[k * n + j] = q;
                 acc_a[j] += valid ? q * xhat : A(0);
@@ -513,6 +555,7 @@ gn_slab_backward_kernel(const E* __restrict__ x, const E* __restrict__ weight, c
         A* row = part + static_cast<int64_t>(slice) * 2 * C;
 #pragma unroll
         for (int j = 0; j < n; ++j) {
+            if (!spot.counts(j)) continue;
             row[c + j] = total_a[j];
             row[C + c + j] = total_b[j];
         }
@@ -541,33 +584,35 @@ __device__ __forceinline__ Patch patch_of(int cols, int columns, int span, int P
 }
 
 // part [S][slices][2][columns]: sums of d and d * d, d = x - (the group's first value), in 64 bits.
-template <typename E, int BYTES>
+template <typename E, int BYTES, bool RAGGED>
 __global__ void __launch_bounds__(kSplitBlock)
 gn_split_statistics_kernel(const E* __restrict__ x, double* __restrict__ part, int P, int C, int cpg, int cols,
                            int span) {
     constexpr int n = Vec<E, BYTES>::n;
     __shared__ double sm[2][kSplitBlock];
-    const int columns = C / n;
+    const int vpg = (cpg + n - 1) / n, columns = C / cpg * vpg;
     const Patch t = patch_of(cols, columns, span, P);
+    const int group = t.col / vpg;
+    const Spot<n, RAGGED> spot(t.col - group * vpg, cpg);
     const int64_t s = blockIdx.x;
     const E* px = x + s * P * C;
     double sum = 0.0, sq = 0.0;
     if (t.here) {
-        const double shift = static_cast<double>(widen(px[t.col * n / cpg * cpg]));
+        const double shift = static_cast<double>(widen(px[group * cpg]));
         constexpr int U = 4;
         for (int p0 = t.begin + t.row; p0 < t.end; p0 += U * t.rows) {
             Vec<E, BYTES> v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int p = p0 + u * t.rows;
-                v[u] = load_vec<E, BYTES>(px + static_cast<int64_t>(p < t.end ? p : p0) * C + t.col * n);
+                v[u] = load_vec<E, BYTES>(px + static_cast<int64_t>(p < t.end ? p : p0) * C + group * cpg + spot.first);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (p0 + u * t.rows < t.end) {
 #pragma unroll
                     for (int j = 0; j < n; ++j) {
-                        const double d = static_cast<double>(widen(v[u].e[j])) - shift;
+                        const double d = spot.counted(j, static_cast<double>(widen(v[u].e[j])) - shift);
                         sum += d;
                         sq += d * d;
                     }
@@ -594,6 +639,7 @@ gn_split_finish_kernel(const E* __restrict__ x, const double* __restrict__ part,
     const int g = static_cast<int>(item - s * G);
     const int vpg = columns / G, cpg = C / G;
     double sum = 0.0, sq = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < slices * vpg; i += 64) {
         const int slice = i / vpg, col = g * vpg + i - slice * vpg;
         const double* q = part + (s * slices + slice) * 2 * columns;
@@ -613,7 +659,7 @@ gn_split_finish_kernel(const E* __restrict__ x, const double* __restrict__ part,
 }
 
 // coefficients == nullptr: y = act(z).  Otherwise grad_x, with coefficients [S][G][2] = (c1, c2).
-template <typename E, int BYTES>
+template <typename E, int BYTES, bool RAGGED>
 __global__ void __launch_bounds__(kSplitBlock)
 gn_split_apply_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                       const arith_t<E>* __restrict__ mean, const arith_t<E>* __restrict__ rstd,
@@ -621,10 +667,11 @@ gn_split_apply_kernel(const E* __restrict__ x, const E* __restrict__ weight, con
                       int P, int C, int G, int cols, int span, int act) {
     using A = arith_t<E>;
     constexpr int n = Vec<E, BYTES>::n;
-    const Patch t = patch_of(cols, C / n, span, P);
+    const int cpg = C / G, vpg = (cpg + n - 1) / n;
+    const Patch t = patch_of(cols, G * vpg, span, P);
     if (!t.here) return;
     const int64_t s = blockIdx.x;
-    const int c = t.col * n, g = c / (C / G);
+    const int g = t.col / vpg, c = g * cpg + Spot<n, RAGGED>(t.col - g * vpg, cpg).first;
     const int64_t base = s * P * C + c;
     const Vec<E, BYTES> w = load_vec<E, BYTES>(weight + c), b = load_vec<E, BYTES>(bias + c);
     const A m = mean[s * G + g], r = rstd[s * G + g];
@@ -663,7 +710,7 @@ gn_split_apply_kernel(const E* __restrict__ x, const E* __restrict__ weight, con
 }
 
 // part [S][slices][2][C]: sums of gz * xhat and of gz.
-template <typename E, int BYTES>
+template <typename E, int BYTES, bool RAGGED>
 __global__ void __launch_bounds__(kSplitBlock)
 gn_split_sums_kernel(const E* __restrict__ x, const E* __restrict__ weight, const E* __restrict__ bias,
                      const arith_t<E>* __restrict__ mean, const arith_t<E>* __restrict__ rstd,
@@ -672,12 +719,14 @@ gn_split_sums_kernel(const E* __restrict__ x, const E* __restrict__ weight, cons
     using A = arith_t<E>;
     constexpr int n = Vec<E, BYTES>::n;
     __shared__ A sm[2 * n][kSplitBlock];
-    const Patch t = patch_of(cols, C / n, span, P);
+    const int cpg = C / G, vpg = (cpg + n - 1) / n;
+    const Patch t = patch_of(cols, G * vpg, span, P);
     const int64_t s = blockIdx.x;
-    const int c = t.col * n;
+    const int g = t.col / vpg;
+    const Spot<n, RAGGED> spot(t.col - g * vpg, cpg);
+    const int c = g * cpg + spot.first;
     A acc_a[n] = {}, acc_b[n] = {};
     if (t.here) {
-        const int g = c / (C / G);
         const int64_t base = s * P * C + c;
         const Vec<E, BYTES> w = load_vec<E, BYTES>(weight + c), b = load_vec<E, BYTES>(bias + c);
         const A m = mean[s * G + g], r = rstd[s * G + g];
@@ -714,6 +763,7 @@ gn_split_sums_kernel(const E* __restrict__ x, const E* __restrict__ weight, cons
         A* q = part + (s * gridDim.y + blockIdx.y) * 2 * C;
 #pragma unroll
         for (int j = 0; j < n; ++j) {
+            if (!spot.counts(j)) continue;
             q[c + j] = sm[j][threadIdx.x];
             q[C + c + j] = sm[n + j][threadIdx.x];
         }
@@ -730,6 +780,7 @@ gn_split_coefficients_kernel(const arith_t<E>* __restrict__ part, const E* __res
     const int64_t s = item / G;
     const int cpg = C / G, first = static_cast<int>(item - s * G) * cpg;
     A c1 = A(0), c2 = A(0);
+#pragma unroll 8
     for (int i = threadIdx.x; i < slices * cpg; i += 64) {
         const int slice = i / cpg, c = first + i - slice * cpg;
         const A* q = part + (s * slices + slice) * 2 * C;
@@ -761,12 +812,12 @@ struct Plan {
     size_t part, coefficients, bytes;
 };
 
-// `vec_bytes`: what one access moves; a vector never leaves its group.
-Plan plan_of(int dtype, int vec_bytes, int64_t S, int64_t P, int64_t C, int64_t G, bool backward) {
+// A vector never leaves its group.
+Plan plan_of(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, bool backward) {
     Plan p{};
     const int64_t es = static_cast<int64_t>(element_size(dtype));
     const size_t arith = dtype == SNNLIF_DTYPE_F64 ? 8 : 4;
-    const int64_t n = vec_bytes / es, cpg = C / G, vpg = cpg / n;
+    const int64_t cpg = C / G, n = widest_vector(cpg, es) / es, vpg = ceil_div(cpg, n);
     if (P == 1 && vpg <= 64 * 4) {
         p.way = Way::rows;
         while ((1 << p.lanes_log2) < vpg && p.lanes_log2 < 6) ++p.lanes_log2;
@@ -782,7 +833,7 @@ Plan plan_of(int dtype, int vec_bytes, int64_t S, int64_t P, int64_t C, int64_t 
     } else {
         p.way = Way::split;
         // 1024 threads only where 256 cannot hold the slab: more workgroups per CU overlap loads with stores.  Segments
-        // of 32 bytes, which 256 threads could hold, cost twice the time ([8 64 32 32 128] fp32: backward 475 us against 276)
+        // of 32 bytes, which 256 threads could hold, cost twice the time ([8 64 32 32 128] fp32: backward 475 us against 276, both with the sums one after another)
         const bool small_sample = P * C * es < (int64_t(1) << 31);
         for (int64_t segment = 128; segment >= 64 && p.way == Way::split && small_sample; segment >>= 1) {
             int64_t gpb = ceil_div(segment, cpg * es);
@@ -803,7 +854,7 @@ Plan plan_of(int dtype, int vec_bytes, int64_t S, int64_t P, int64_t C, int64_t 
             const int64_t wanted = ceil_div(p.block == 256 ? 2048 : 512, p.bundles);
             p.part_rows = wanted < S ? wanted : S;
         } else {
-            const int64_t columns = C / n;
+            const int64_t columns = G * vpg;
             p.cols = static_cast<int>(columns < 64 ? columns : 64);
             p.col_blocks = static_cast<int>(ceil_div(columns, p.cols));
             const int64_t rows = kSplitBlock / p.cols;
@@ -820,7 +871,7 @@ Plan plan_of(int dtype, int vec_bytes, int64_t S, int64_t P, int64_t C, int64_t 
         p.coefficients = p.bytes;
         if (p.way == Way::split) p.bytes += static_cast<size_t>(S) * static_cast<size_t>(G) * 2 * arith;
     } else if (p.way == Way::split) {
-        p.bytes = static_cast<size_t>(S) * p.slices * 2 * static_cast<size_t>(C / n) * sizeof(double);
+        p.bytes = static_cast<size_t>(S) * p.slices * 2 * static_cast<size_t>(G * vpg) * sizeof(double);
     }
     return p;
 }
@@ -835,29 +886,29 @@ struct Call {
     hipStream_t stream;
 };
 
-template <typename E, int BYTES, int K, int U>
+template <typename E, int BYTES, bool RAGGED, int K, int U>
 hipError_t rows_forward_by(const Call& a, const Plan& p) {
     using A = arith_t<E>;
     const int64_t items = a.S * a.G, step = ceil_div(a.S, U) * a.G;
-    return launch(gn_rows_forward_kernel<E, BYTES, K, U>,
+    return launch(gn_rows_forward_kernel<E, BYTES, RAGGED, K, U>,
                   dim3(static_cast<unsigned>(ceil_div(step, kRowsBlock >> p.lanes_log2))), dim3(kRowsBlock), a.stream,
                   static_cast<const E*>(a.x), static_cast<const E*>(a.weight), static_cast<const E*>(a.bias),
                   static_cast<E*>(a.out), static_cast<A*>(a.mean_out), static_cast<A*>(a.rstd_out), items, step,
                   static_cast<int>(a.G), static_cast<int>(a.C / a.G), static_cast<A>(a.eps), a.act, p.lanes_log2);
 }
 
-template <typename E, int BYTES, int K>
+template <typename E, int BYTES, bool RAGGED, int K>
 hipError_t rows_forward(const Call& a, const Plan& p) {
     // four samples per group of lanes where that leaves eight workgroups for every CU: more requests in flight
     // ([16384, 8 groups of 128] bf16 silu: 21.5 us); fewer samples want the workgroups
-    if (K == 1 && a.S * a.G >= int64_t(4) * 8 * 256 * (kRowsBlock >> p.lanes_log2)) return rows_forward_by<E, BYTES, K, 4>(a, p);
-    return rows_forward_by<E, BYTES, K, 1>(a, p);
+    if (K == 1 && a.S * a.G >= int64_t(4) * 8 * 256 * (kRowsBlock >> p.lanes_log2)) return rows_forward_by<E, BYTES, RAGGED, K, 4>(a, p);
+    return rows_forward_by<E, BYTES, RAGGED, K, 1>(a, p);
 }
 
-template <typename E, int BYTES, int K>
+template <typename E, int BYTES, bool RAGGED, int K>
 hipError_t rows_backward(const Call& a, const Plan& p) {
     using A = arith_t<E>;
-    return launch(gn_rows_backward_kernel<E, BYTES, K>,
+    return launch(gn_rows_backward_kernel<E, BYTES, RAGGED, K>,
                   dim3(static_cast<unsigned>(p.part_rows), static_cast<unsigned>(p.group_blocks)), dim3(kRowsBlock),
                   a.stream, static_cast<const E*>(a.x), static_cast<const E*>(a.weight), static_cast<const E*>(a.bias),
                   static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd), static_cast<const E*>(a.grad),
@@ -865,20 +916,20 @@ hipError_t rows_backward(const Call& a, const Plan& p) {
                   static_cast<int>(a.C / a.G), a.act, p.lanes_log2, p.gpb, p.spb);
 }
 
-template <typename E, int BYTES, int BT>
+template <typename E, int BYTES, bool RAGGED, int BT>
 hipError_t slab_forward(const Call& a, const Plan& p) {
     using A = arith_t<E>;
-    return launch(gn_slab_forward_kernel<E, BYTES, BT>, dim3(static_cast<unsigned>(a.S * p.bundles)), dim3(BT),
+    return launch(gn_slab_forward_kernel<E, BYTES, RAGGED, BT>, dim3(static_cast<unsigned>(a.S * p.bundles)), dim3(BT),
                   a.stream, static_cast<const E*>(a.x), static_cast<const E*>(a.weight), static_cast<const E*>(a.bias),
                   static_cast<E*>(a.out), static_cast<A*>(a.mean_out), static_cast<A*>(a.rstd_out), p.bundles,
                   static_cast<int>(a.P), static_cast<int>(a.G), static_cast<int>(a.C / a.G), p.gpb,
                   static_cast<A>(a.eps), a.act);
 }
 
-template <typename E, int BYTES, int BT>
+template <typename E, int BYTES, bool RAGGED, int BT>
 hipError_t slab_backward(const Call& a, const Plan& p) {
     using A = arith_t<E>;
-    return launch(gn_slab_backward_kernel<E, BYTES, BT>, dim3(static_cast<unsigned>(p.part_rows * p.bundles)),
+    return launch(gn_slab_backward_kernel<E, BYTES, RAGGED, BT>, dim3(static_cast<unsigned>(p.part_rows * p.bundles)),
                   dim3(BT), a.stream, static_cast<const E*>(a.x), static_cast<const E*>(a.weight),
                   static_cast<const E*>(a.bias), static_cast<const A*>(a.mean), static_cast<const A*>(a.rstd),
                   static_cast<const E*>(a.grad), static_cast<E*>(a.out), reinterpret_cast<A*>(a.ws), a.S, p.bundles,
@@ -886,21 +937,21 @@ hipError_t slab_backward(const Call& a, const Plan& p) {
                   static_cast<int>(a.C / a.G), p.gpb, a.act);
 }
 
-template <typename E, int BYTES>
+template <typename E, int BYTES, bool RAGGED>
 hipError_t split_forward(const Call& a, const Plan& p) {
     using A = arith_t<E>;
     const int P = static_cast<int>(a.P), C = static_cast<int>(a.C), G = static_cast<int>(a.G);
     const dim3 grid(static_cast<unsigned>(a.S), static_cast<unsigned>(p.slices), static_cast<unsigned>(p.col_blocks));
     const E* x = static_cast<const E*>(a.x);
     double* part = reinterpret_cast<double*>(a.ws);
-    hipError_t err = launch(gn_split_statistics_kernel<E, BYTES>, grid, dim3(kSplitBlock), a.stream, x, part, P, C,
+    hipError_t err = launch(gn_split_statistics_kernel<E, BYTES, RAGGED>, grid, dim3(kSplitBlock), a.stream, x, part, P, C,
                             C / G, p.cols, p.span);
     if (err == hipSuccess)
         err = launch(gn_split_finish_kernel<E>, dim3(static_cast<unsigned>(a.S * a.G)), dim3(64), a.stream, x,
                      const_cast<const double*>(part), static_cast<A*>(a.mean_out), static_cast<A*>(a.rstd_out), P, C, G,
-                     C / Vec<E, BYTES>::n, p.slices, a.eps);
+                     G * static_cast<int>(ceil_div(C / G, Vec<E, BYTES>::n)), p.slices, a.eps);
     if (err == hipSuccess)
-        err = launch(gn_split_apply_kernel<E, BYTES>, grid, dim3(kSplitBlock), a.stream, x,
+        err = launch(gn_split_apply_kernel<E, BYTES, RAGGED>, grid, dim3(kSplitBlock), a.stream, x,
                      static_cast<const E*>(a.weight), static_cast<const E*>(a.bias),
                      static_cast<const A*>(a.mean_out), static_cast<const A*>(a.rstd_out),
                      static_cast<const E*>(nullptr), static_cast<const A*>(nullptr), static_cast<E*>(a.out), P, C, G,
@@ -908,7 +959,7 @@ hipError_t split_forward(const Call& a, const Plan& p) {
     return err;
 }
 
-template <typename E, int BYTES>
+template <typename E, int BYTES, bool RAGGED>
 hipError_t split_backward(const Call& a, const Plan& p) {
     using A = arith_t<E>;
     const int P = static_cast<int>(a.P), C = static_cast<int>(a.C), G = static_cast<int>(a.G);
@@ -918,30 +969,30 @@ hipError_t split_backward(const Call& a, const Plan& p) {
     const A *mean = static_cast<const A*>(a.mean), *rstd = static_cast<const A*>(a.rstd);
     A* part = reinterpret_cast<A*>(a.ws);
     A* coefficients = reinterpret_cast<A*>(a.ws + p.coefficients);
-    hipError_t err = launch(gn_split_sums_kernel<E, BYTES>, grid, dim3(kSplitBlock), a.stream, x, weight, bias, mean,
+    hipError_t err = launch(gn_split_sums_kernel<E, BYTES, RAGGED>, grid, dim3(kSplitBlock), a.stream, x, weight, bias, mean,
                             rstd, grad, part, P, C, G, p.cols, p.span, a.act);
     if (err == hipSuccess)
         err = launch(gn_split_coefficients_kernel<E>, dim3(static_cast<unsigned>(a.S * a.G)), dim3(64), a.stream,
                      const_cast<const A*>(part), weight, coefficients, P, C, G, p.slices);
     if (err == hipSuccess)
-        err = launch(gn_split_apply_kernel<E, BYTES>, grid, dim3(kSplitBlock), a.stream, x, weight, bias, mean, rstd,
+        err = launch(gn_split_apply_kernel<E, BYTES, RAGGED>, grid, dim3(kSplitBlock), a.stream, x, weight, bias, mean, rstd,
                      grad, const_cast<const A*>(coefficients), static_cast<E*>(a.out), P, C, G, p.cols, p.span, a.act);
     return err;
 }
 
-template <typename E, int BYTES>
+template <typename E, int BYTES, bool RAGGED>
 hipError_t run_as(const Call& a, const Plan& p, bool backward) {
     hipError_t err;
     if (p.way == Way::rows) {
-        if (p.vectors == 1) err = backward ? rows_backward<E, BYTES, 1>(a, p) : rows_forward<E, BYTES, 1>(a, p);
-        else if (p.vectors == 2) err = backward ? rows_backward<E, BYTES, 2>(a, p) : rows_forward<E, BYTES, 2>(a, p);
-        else err = backward ? rows_backward<E, BYTES, 4>(a, p) : rows_forward<E, BYTES, 4>(a, p);
+        if (p.vectors == 1) err = backward ? rows_backward<E, BYTES, RAGGED, 1>(a, p) : rows_forward<E, BYTES, RAGGED, 1>(a, p);
+        else if (p.vectors == 2) err = backward ? rows_backward<E, BYTES, RAGGED, 2>(a, p) : rows_forward<E, BYTES, RAGGED, 2>(a, p);
+        else err = backward ? rows_backward<E, BYTES, RAGGED, 4>(a, p) : rows_forward<E, BYTES, RAGGED, 4>(a, p);
     } else if (p.way == Way::slab) {
-        if (p.block == 256) err = backward ? slab_backward<E, BYTES, 256>(a, p) : slab_forward<E, BYTES, 256>(a, p);
-        else if constexpr (sizeof(E) == 8) err = slab_forward<E, BYTES, 1024>(a, p);
-        else err = backward ? slab_backward<E, BYTES, 1024>(a, p) : slab_forward<E, BYTES, 1024>(a, p);
+        if (p.block == 256) err = backward ? slab_backward<E, BYTES, RAGGED, 256>(a, p) : slab_forward<E, BYTES, RAGGED, 256>(a, p);
+        else if constexpr (sizeof(E) == 8) err = slab_forward<E, BYTES, RAGGED, 1024>(a, p);
+        else err = backward ? slab_backward<E, BYTES, RAGGED, 1024>(a, p) : slab_forward<E, BYTES, RAGGED, 1024>(a, p);
     } else {
-        err = backward ? split_backward<E, BYTES>(a, p) : split_forward<E, BYTES>(a, p);
+        err = backward ? split_backward<E, BYTES, RAGGED>(a, p) : split_forward<E, BYTES, RAGGED>(a, p);
     }
     if (err == hipSuccess && backward)
         err = launch(gn_parameters_kernel<E>, dim3(static_cast<unsigned>(ceil_div(2 * a.C, 32))), dim3(1024), a.stream,
@@ -950,17 +1001,25 @@ hipError_t run_as(const Call& a, const Plan& p, bool backward) {
     return err;
 }
 
-hipError_t run(int dtype, int bytes, const Call& a, const Plan& p, bool backward) {
+template <typename E, int BYTES>
+hipError_t run_by(const Call& a, const Plan& p, bool backward) {
+    if constexpr (BYTES > static_cast<int>(sizeof(E)))
+        if (a.C / a.G % Vec<E, BYTES>::n != 0) return run_as<E, BYTES, true>(a, p, backward);
+    return run_as<E, BYTES, false>(a, p, backward);
+}
+
+hipError_t run(int dtype, const Call& a, const Plan& p, bool backward) {
+    const int bytes = widest_vector(a.C / a.G, element_size(dtype));
     if (dtype == SNNLIF_DTYPE_F32)
-        return bytes == 16  ? run_as<float, 16>(a, p, backward)
-               : bytes == 8 ? run_as<float, 8>(a, p, backward)
-                            : run_as<float, 4>(a, p, backward);
+        return bytes == 16  ? run_by<float, 16>(a, p, backward)
+               : bytes == 8 ? run_by<float, 8>(a, p, backward)
+                            : run_by<float, 4>(a, p, backward);
     if (dtype == SNNLIF_DTYPE_F64)
-        return bytes == 16 ? run_as<double, 16>(a, p, backward) : run_as<double, 8>(a, p, backward);
-    return bytes == 16  ? run_as<bf16_t, 16>(a, p, backward)
-           : bytes == 8 ? run_as<bf16_t, 8>(a, p, backward)
-           : bytes == 4 ? run_as<bf16_t, 4>(a, p, backward)
-                        : run_as<bf16_t, 2>(a, p, backward);
+        return bytes == 16 ? run_by<double, 16>(a, p, backward) : run_by<double, 8>(a, p, backward);
+    return bytes == 16  ? run_by<bf16_t, 16>(a, p, backward)
+           : bytes == 8 ? run_by<bf16_t, 8>(a, p, backward)
+           : bytes == 4 ? run_by<bf16_t, 4>(a, p, backward)
+                        : run_by<bf16_t, 2>(a, p, backward);
 }
 
 int gn_shape_error(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, int act) {
@@ -978,17 +1037,9 @@ int gn_shape_error(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, int ac
 
 using namespace snnseq;
 
-// The vector width, and with it the plan, follow from the sizes and the alignment of every tensor: the workspace is
-// sized for the worst case over alignments.
 extern "C" size_t snnseq_gn_act_workspace_bytes(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, int backward) {
     if (gn_shape_error(dtype, S, P, C, G, SNNSEQ_ACT_NONE) != SNNLIF_OK || S == 0) return 0;
-    const int es = static_cast<int>(element_size(dtype));
-    size_t most = 0;
-    for (int bytes = common_bytes(static_cast<uint64_t>(C / G) * es); bytes >= es; bytes >>= 1) {
-        const size_t need = plan_of(dtype, bytes, S, P, C, G, backward != 0).bytes;
-        most = need > most ? need : most;
-    }
-    return most;
+    return plan_of(dtype, S, P, C, G, backward != 0).bytes;
 }
 
 extern "C" int snnseq_gn_act_fp(const void* x, const void* weight, const void* bias, void* y, void* mean, void* rstd,
@@ -1003,15 +1054,14 @@ extern "C" int snnseq_gn_act_fp(const void* x, const void* weight, const void* b
     if (!aligned_to(x, es) || !aligned_to(weight, es) || !aligned_to(bias, es) || !aligned_to(y, es) ||
         !aligned_to(mean, as) || !aligned_to(rstd, as) || !aligned_to(workspace, 16))
         return SNNLIF_ERR_ALIGN;
-    const int bytes = common_bytes(address(x), address(y), address(weight), address(bias), C / G * es);
-    const Plan p = plan_of(dtype, bytes, S, P, C, G, false);
+    const Plan p = plan_of(dtype, S, P, C, G, false);
     if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes)) return SNNLIF_ERR_WORKSPACE;
     Call a{};
     a.x = x; a.weight = weight; a.bias = bias; a.out = y; a.mean_out = mean; a.rstd_out = rstd;
     a.S = S; a.P = P; a.C = C; a.G = G; a.eps = eps; a.act = act;
     a.ws = static_cast<char*>(workspace);
     a.stream = static_cast<hipStream_t>(stream);
-    return static_cast<int>(run(dtype, bytes, a, p, false));
+    return static_cast<int>(run(dtype, a, p, false));
 }
 
 extern "C" int snnseq_gn_act_bp(const void* x, const void* weight, const void* bias, const void* mean,
@@ -1029,9 +1079,7 @@ extern "C" int snnseq_gn_act_bp(const void* x, const void* weight, const void* b
         !aligned_to(grad_x, es) || !aligned_to(grad_weight, es) || !aligned_to(grad_bias, es) ||
         !aligned_to(mean, as) || !aligned_to(rstd, as) || !aligned_to(workspace, 16))
         return SNNLIF_ERR_ALIGN;
-    const int bytes = common_bytes(address(x) | address(grad_y), address(grad_x), address(weight), address(bias),
-                                   C / G * es);
-    const Plan p = plan_of(dtype, bytes, S, P, C, G, true);
+    const Plan p = plan_of(dtype, S, P, C, G, true);
     if (workspace == nullptr || workspace_bytes < p.bytes) return SNNLIF_ERR_WORKSPACE;
     Call a{};
     a.x = x; a.weight = weight; a.bias = bias; a.mean = mean; a.rstd = rstd; a.grad = grad_y; a.out = grad_x;
@@ -1039,5 +1087,5 @@ extern "C" int snnseq_gn_act_bp(const void* x, const void* weight, const void* b
     a.S = S; a.P = P; a.C = C; a.G = G; a.act = act;
     a.ws = static_cast<char*>(workspace);
     a.stream = static_cast<hipStream_t>(stream);
-    return static_cast<int>(run(dtype, bytes, a, p, true));
+    return static_cast<int>(run(dtype, a, p, true));
 }

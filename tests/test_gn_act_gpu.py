@@ -289,3 +289,31 @@ def test_a_group_of_one_value_has_no_input_gradient(sf, channels, act, dtype):
     assert torch.equal(y, y[:1, :1].expand_as(y))
     assert torch.equal(gx, torch.zeros_like(gx))
     assert torch.equal(gw, torch.zeros_like(gw))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape,groups", [
+    ((9, 3, 3 * 5), 3),              # rows: a vector and one value of the next
+    ((9, 3, 2 * 111), 2),
+    ((3, 2, 6, 5, 4 * 3), 4),        # slab: groups narrower than a vector
+    ((5, 3, 11, 20, 9 * 43), 9),     # slab of 1024 threads
+    ((1, 2, 60, 70, 2 * 13), 2),     # split
+])
+def test_groups_that_end_inside_a_vector(sf, shape, groups, dtype):
+    check(sf, shape, groups, "silu", dtype, seed=groups)
+
+
+@gpu
+@pytest.mark.parametrize("shape,groups", [((3, 2, 2 * 7), 2), ((2, 2, 6, 6, 3 * 5), 3), ((1, 1, 80, 80, 2 * 11), 2)])
+def test_values_that_are_not_finite_stay_in_their_group_where_vectors_overlap(sf, shape, groups):
+    x, w, b, gy = (t.cuda() for t in make(shape, torch.float32, 3))
+    first = run(sf, x, w, b, gy, groups, "silu")
+    cpg = shape[-1] // groups
+    bad = x.clone()
+    bad.reshape(-1, shape[-1])[0, cpg - 1] = float("nan")      # the last value of the first sample's first group
+    second = run(sf, bad, w, b, gy, groups, "silu")
+    for a, c in zip(first[:2], second[:2]):
+        a, c = (t.reshape(shape[0] * shape[1], -1, groups, cpg) for t in (a, c))
+        assert bool(c[0, :, 0].isnan().all())
+        assert torch.equal(a[0, :, 1:], c[0, :, 1:]) and torch.equal(a[1:], c[1:])
