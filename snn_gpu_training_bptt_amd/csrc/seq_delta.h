@@ -380,20 +380,24 @@ __device__ __forceinline__ DeltaWhere delta_where(const DeltaArgs& a, int head, 
 
 // ---- staging ------------------------------------------------------------------------------------
 
-// Eight consecutive values of a row.  Without a branch and without a look at the values, so that all loads of a thread
-// are under way together: what lies behind `valid` is read at the row's beginning, and keep_valid takes it out later.
+// Eight consecutive values of a row, from any element on.  Without a look at the values, so that all loads of a thread
+// are under way together.  WIDE: rows of a multiple of eight values; what lies behind `valid` is read at the row's
+// beginning, and keep_valid takes it out later.  Otherwise the eight that would reach over the row's end are the last
+// eight instead, and keep_valid moves them to their places.
 template <bool WIDE, typename E>
 __device__ __forceinline__ Raw8<E> load_raw8(const E* row, int c, int valid) {
+    using memory_t = u32x4 __attribute__((aligned(sizeof(E))));
     Raw8<E> x;
-    if constexpr (WIDE) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(row + (c < valid ? c : 0));
+    if (WIDE || valid >= 8) {
+        const int at = WIDE ? (c < valid ? c : 0) : (c < valid - 8 ? c : valid - 8);
+        const memory_t* p = reinterpret_cast<const memory_t*>(row + at);
 #pragma unroll
         for (int h = 0; h < static_cast<int>(sizeof(E) / 2); ++h) x.r[h] = p[h];
-    } else {
+    } else {   // fewer than eight: those behind are in front, and moved out
         uint32_t bits[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const E v = row[c + j < valid ? c + j : 0];
+            const E v = row[valid - 8 + j > 0 ? valid - 8 + j : 0];
             if constexpr (sizeof(E) == 4) bits[j] = __builtin_bit_cast(uint32_t, v);
             else bits[j] = v.bits;
         }
@@ -407,22 +411,34 @@ __device__ __forceinline__ Raw8<E> load_raw8(const E* row, int c, int valid) {
     return x;
 }
 
-// Zero at and behind `valid` (wide rows end at a multiple of eight).
+// Zero at and behind `valid`, and everywhere where the row does not exist.
 template <bool WIDE, typename E>
-__device__ __forceinline__ Raw8<E> keep_valid(Raw8<E> x, int c, int valid) {
+__device__ __forceinline__ Raw8<E> keep_valid(Raw8<E> x, int c, int valid, bool exists) {
+    constexpr int words = 2 * static_cast<int>(sizeof(E)), per = 4 / static_cast<int>(sizeof(E));   // values per word
     if constexpr (WIDE) {
 #pragma unroll
-        for (int h = 0; h < static_cast<int>(sizeof(E) / 2); ++h) x.r[h] = c < valid ? x.r[h] : u32x4{0, 0, 0, 0};
+        for (int h = 0; h < words / 4; ++h) x.r[h] = exists && c < valid ? x.r[h] : u32x4{0, 0, 0, 0};
     } else {
-        constexpr int per = 4 / static_cast<int>(sizeof(E));   // values per word
+        const int last = valid - 8, by = exists ? (c > last ? c - last : 0) : 8;   // places to move down, zeros behind
+        uint32_t w[words];
 #pragma unroll
-        for (int j = 0; j < 8 / per; ++j) {
-            const int left = valid - c - j * per;
-            uint32_t word = x.r[j / 4][j % 4];
-            if constexpr (per == 2) word = left > 1 ? word : left == 1 ? word & 0xffffu : 0u;
-            else word = left > 0 ? word : 0u;
-            x.r[j / 4][j % 4] = word;
+        for (int j = 0; j < words; ++j) w[j] = by < 8 ? x.r[j / 4][j % 4] : 0u;
+#pragma unroll
+        for (int step = 4; step >= per; step >>= 1)
+#pragma unroll
+            for (int j = 0; j < words; ++j) {
+                const uint32_t from = j + step / per < words ? w[j + step / per] : 0u;
+                w[j] = by & step ? from : w[j];
+            }
+        if constexpr (per == 2) {
+#pragma unroll
+            for (int j = 0; j < words; ++j) {
+                const uint32_t above = j + 1 < words ? w[j + 1] : 0u;
+                w[j] = by & 1 ? w[j] >> 16 | above << 16 : w[j];
+            }
         }
+#pragma unroll
+        for (int j = 0; j < words; ++j) x.r[j / 4][j % 4] = w[j];
     }
     return x;
 }
@@ -461,7 +477,7 @@ struct Ahead {
     }
     __device__ __forceinline__ Raw8<E> get(int i) const {
         const int seg = i * THREADS + threadIdx.x, r = seg / (COLS / 8), c = seg % (COLS / 8) * 8;
-        return keep_valid<WIDE, E>(x[i], c, r < rows ? valid : 0);
+        return keep_valid<WIDE, E>(x[i], c, valid, r < rows);
     }
     template <typename Tile>
     __device__ __forceinline__ void store(Tile& tile) const {
@@ -1559,7 +1575,7 @@ hipError_t delta_backward_as(const DeltaArgs& a, void* grad_q, void* grad_k, hip
                   static_cast<E*>(grad_k), rows, a.Dk, a.Hv / a.Hk);
 }
 
-// Keys of up to 64 values and of up to 128; rows that can be read in vectors of 16 bytes, and any others.
+// Keys of up to 64 values and of up to 128; rows of a multiple of eight values, and any others.
 #define SNNSEQ_DEFINE_DELTA(NAME, E)                                                                           \
     hipError_t delta_forward_##NAME(const DeltaArgs& a, hipStream_t st) {                                      \
         const bool wide = a.q.wide && a.k.wide;                                                                \

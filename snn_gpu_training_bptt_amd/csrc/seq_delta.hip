@@ -184,10 +184,9 @@ int missing(const snnseq_delta* c) {
     return SNNLIF_OK;
 }
 
-DeltaTensor tensor_of(const void* p, const int64_t* strides, int64_t D, size_t es) {
+DeltaTensor tensor_of(const void* p, const int64_t* strides, int64_t D) {
     DeltaTensor x{p, strides[0], strides[1], strides[2], 0};
-    x.wide = D % 8 == 0 && common_bytes(address(p), static_cast<uint64_t>(strides[0]) * es,
-                                        static_cast<uint64_t>(strides[1]) * es, static_cast<uint64_t>(strides[2]) * es) == 16;
+    x.wide = D % 8 == 0;
     return x;
 }
 
@@ -230,9 +229,9 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved, bool for_b
     a.chunks = static_cast<int>(s.chunks); a.cols = static_cast<int>(s.cols);
     a.scale = static_cast<float>(c->scale);
     a.lengths = c->lengths;
-    a.q = tensor_of(c->q, c->q_strides, c->Dk, es);
-    a.k = tensor_of(c->k, c->k_strides, c->Dk, es);
-    a.v = tensor_of(c->v, c->v_strides, c->Dv, es);
+    a.q = tensor_of(c->q, c->q_strides, c->Dk);
+    a.k = tensor_of(c->k, c->k_strides, c->Dk);
+    a.v = tensor_of(c->v, c->v_strides, c->Dv);
     a.g = c->g; a.beta = c->beta; a.state = c->state;
     char* p = static_cast<char*>(saved);
     a.decay = reinterpret_cast<Decay*>(p);
@@ -309,7 +308,7 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
         return SNNLIF_ERR_WORKSPACE;
     DeltaArgs a = args_of(call, s, const_cast<void*>(saved), true);
     char* p = static_cast<char*>(workspace);
-    a.grad_o = tensor_of(grad_o, grad_o_strides, call->Dv, es);
+    a.grad_o = tensor_of(grad_o, grad_o_strides, call->Dv);
     a.grad_state = grad_state_out;
     a.inner = reinterpret_cast<float*>(p);
     a.state_grads = reinterpret_cast<float*>(p + s.inner);
@@ -317,7 +316,7 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
     a.grad_q = s.partial ? a.queries_t + s.queries : grad_q;
     a.grad_k = s.partial ? a.queries_t + s.queries + s.partial : grad_k;
     a.grad_v = grad_v;
-    a.wide_grad_v = call->Dv % 4 == 0 && aligned_to(grad_v, 4 * es);
+    a.wide_grad_v = call->Dv % 4 == 0;
     a.grad_g = grad_g;
     a.grad_beta = grad_beta;
     a.grad_initial = grad_state;

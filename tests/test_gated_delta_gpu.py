@@ -387,3 +387,10 @@ def test_a_host_tensor_is_refused(sf):
         sf.gated_delta_func(*(x[n] for n in NAMES))
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         sf.gated_delta_step(*(x[n][0] for n in NAMES[:5]), x["state"])
+
+
+@gpu
+@both
+@pytest.mark.parametrize("Dk,Dv", [(1, 1), (3, 5), (7, 8), (8, 7), (9, 9), (15, 33), (33, 39), (66, 70), (127, 101)])
+def test_rows_that_end_inside_a_vector(sf, Dk, Dv, dtype):
+    check(sf, 70, 2, 1, 2, Dk, Dv, dtype, seed=Dk + Dv, lengths=[70, 41])
