@@ -87,7 +87,8 @@ int snnseq_gn_act_bp(const void* x, const void* weight, const void* bias, const 
 /* Bytes of device workspace of the two calls above (backward = 0 / 1); 0 also where none is needed. */
 size_t snnseq_gn_act_workspace_bytes(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, int backward);
 
-/* Most values of a key and of a value, and most heads times batch entries, of a gated delta call. */
+/* Most values of a key and of a value, and most heads times batch entries, of a gated delta call.  Over more than one
+ * step, heads times batch entries times 2 * ceil(Dv / 32) may be no more than SNNSEQ_MAX_TOKENS. */
 #define SNNSEQ_MAX_KEY   128
 #define SNNSEQ_MAX_VALUE 65536
 #define SNNSEQ_MAX_HEADS 65535

@@ -172,6 +172,13 @@ int delta_error(const snnseq_delta* c) {
     return SNNLIF_OK;
 }
 
+// The passes over the chunks launch a workgroup of 256 per head and 16 columns: what a launch can hold.
+int chunked_error(const snnseq_delta* c) {
+    const int bad = delta_error(c);
+    if (bad != SNNLIF_OK) return bad;
+    return c->B * c->Hv * ceil_div(c->Dv, kCols) * (kCols / kStateCols) > SNNSEQ_MAX_TOKENS ? SNNLIF_ERR_ARG : SNNLIF_OK;
+}
+
 bool empty(const snnseq_delta* c) { return c->B == 0; }
 
 int missing(const snnseq_delta* c) {
@@ -256,13 +263,13 @@ DeltaArgs args_of(const snnseq_delta* c, const Sizes& s, void* saved, bool for_b
 using namespace snnseq;
 
 extern "C" size_t snnseq_gated_delta_saved_bytes(const snnseq_delta* call, int for_backward) {
-    if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
+    if (chunked_error(call) != SNNLIF_OK || empty(call)) return 0;
     return sizes_of(call, for_backward != 0).saved;
 }
 
 extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* state_out, void* saved,
                                      size_t saved_bytes, int for_backward, void* stream) {
-    const int bad = delta_error(call);
+    const int bad = chunked_error(call);
     if (bad != SNNLIF_OK) return bad;
     if (empty(call)) return SNNLIF_OK;
     const int lost = missing(call);
@@ -280,7 +287,7 @@ extern "C" int snnseq_gated_delta_fp(const snnseq_delta* call, void* o, float* s
 }
 
 extern "C" size_t snnseq_gated_delta_bp_workspace_bytes(const snnseq_delta* call) {
-    if (delta_error(call) != SNNLIF_OK || empty(call)) return 0;
+    if (chunked_error(call) != SNNLIF_OK || empty(call)) return 0;
     return sizes_of(call, true).workspace;
 }
 
@@ -288,7 +295,7 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
                                      const void* grad_o, const int64_t* grad_o_strides, const float* grad_state_out,
                                      void* grad_q, void* grad_k, void* grad_v, float* grad_g, float* grad_beta,
                                      float* grad_state, void* workspace, size_t workspace_bytes, void* stream) {
-    const int bad = delta_error(call);
+    const int bad = chunked_error(call);
     if (bad != SNNLIF_OK) return bad;
     if (empty(call)) return SNNLIF_OK;
     const int lost = missing(call);

@@ -843,6 +843,7 @@ Plan plan_of(int dtype, int64_t S, int64_t P, int64_t C, int64_t G, bool backwar
                 if (backward && block == 1024 && es == 8) continue;  // 64-bit sums do not fit 128 registers
                 const int held = held_vectors(static_cast<int>(es), static_cast<int>(n), block, backward);
                 if (cols > block || ceil_div(P, block / cols) > held) continue;
+                if (!backward && S * ceil_div(G, gpb) * block > (int64_t(1) << 31)) continue;   // more threads than a launch
                 p.way = Way::slab;
                 p.block = block;
                 p.gpb = static_cast<int>(gpb);

@@ -394,3 +394,23 @@ def test_a_host_tensor_is_refused(sf):
 @pytest.mark.parametrize("Dk,Dv", [(1, 1), (3, 5), (7, 8), (8, 7), (9, 9), (15, 33), (33, 39), (66, 70), (127, 101)])
 def test_rows_that_end_inside_a_vector(sf, Dk, Dv, dtype):
     check(sf, 70, 2, 1, 2, Dk, Dv, dtype, seed=Dk + Dv, lengths=[70, 41])
+
+
+@gpu
+@both
+@pytest.mark.parametrize("T,Hk,Hv,Dk,Dv,lengths", [
+    (1, 1, 1, 64, 32, None), (64, 2, 2, 128, 128, None), (150, 1, 4, 96, 80, [150, 70]), (200, 2, 4, 33, 70, [0, 129]),
+    (130, 1, 2, 17, 16, [64, 1]),
+])
+def test_without_gradients_the_same_bits(sf, T, Hk, Hv, Dk, Dv, lengths, dtype):
+    """The forward that leaves nothing behind, with what does not exist set to NaN."""
+    x, go, gs = make(T, 2, Hk, Hv, Dk, Dv, dtype, seed=T)
+    t = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    first = run(sf, x, go, gs, t, 0.2)
+    if lengths is not None:
+        for b, n in enumerate(lengths):
+            for name in ("q", "k", "v", "g", "beta"):
+                x[name][n:, b] = float("nan")
+    with torch.no_grad():
+        o, last = sf.gated_delta_func(*(x[n].cuda() for n in NAMES), None if t is None else t.cuda(), 0.2)
+    assert torch.equal(o, first["o"]) and torch.equal(last, first["last"])

@@ -47,7 +47,7 @@ def test_argument_errors_need_no_gpu():
     assert fp(w=odd) == fp(t=odd) == seq_cabi.ERR_ALIGN
     assert fp(N=0, t=None) == fp(C=0, t=None) == seq_cabi.OK
     need = lib.snnseq_embed_bp_workspace_bytes(F32, 100, 50, 8)
-    assert need == 208 + 400 + 400 + 2 * 2 * 8 * 4             # start, positions, tokens, two pieces' sums
+    assert need == 208 + 400 + 400 + 7 * 2 * 8 * 4             # start, positions, tokens, seven pieces' sums
     bp = lambda ws=p, n=need: lib.snnseq_embed_bp(p, p, p, F32, 1, 100, 50, 8, 1.0, ws, n, None)
     assert bp(n=need - 1) == bp(ws=None) == seq_cabi.ERR_WORKSPACE and bp(ws=odd) == seq_cabi.ERR_ALIGN
     assert lib.snnseq_embed_bp_workspace_bytes(F32, -1, 50, 8) == 0
@@ -88,6 +88,22 @@ def test_argument_errors_need_no_gpu():
     step = lambda **change: lib.snnseq_gated_delta_step(call(**{"T": 1, "state": p, **change}), p, p, None)
     assert step(T=2) == step(state=None) == step(lengths=p) == step(v=None) == seq_cabi.ERR_ARG
     assert step(B=0) == seq_cabi.OK
+
+
+def test_launches_hold_what_is_accepted():
+    """Sizes whose launch would have more workgroups or threads than one can: refused, or worked on in another layout."""
+    lib = seq_cabi.load()
+    call = seq_cabi.DeltaCall(T=70, B=1024, Hk=4, Hv=4, Dk=1, Dv=65536, scale=1.0, dtype=F32)
+    for n in ("q", "k", "v", "g", "beta"):
+        setattr(call, n, 4096)
+    assert lib.snnseq_gated_delta_saved_bytes(call, 1) == lib.snnseq_gated_delta_bp_workspace_bytes(call) == 0
+    p = ctypes.c_void_p(4096)
+    assert lib.snnseq_gated_delta_fp(call, p, p, p, 1 << 62, 1, None) == seq_cabi.ERR_ARG
+    call.B = 512
+    assert lib.snnseq_gated_delta_saved_bytes(call, 1) > 0
+    # a sample of 4096 positions of one group of four is a workgroup's of 1024 threads, unless there are too many of them
+    assert lib.snnseq_gn_act_workspace_bytes(F32, 1000, 4096, 4, 1, 0) == 0
+    assert lib.snnseq_gn_act_workspace_bytes(F32, seq_cabi.MAX_TOKENS, 4096, 4, 1, 0) > 0
 
 
 def test_helpers_reject_mismatched_buffers_before_any_launch():
