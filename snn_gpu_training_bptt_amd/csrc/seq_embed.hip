@@ -17,7 +17,8 @@
 //   2. rows and pieces.  A row with at most a piece's positions is summed by the threads that own its columns.
 //      The positions of longer rows (frequent words) are cut at multiples of a piece in the sorted order;
 //      every piece is summed by a workgroup of its own, in the same launch.
-//      The same sizes: 46 us (67 MB read, 102 MB written: 3.7 TB/s; a row's few reads follow each other).
+//      The same sizes, 1024 bf16 columns: 43 us (67 MB read, 102 MB written: 3.9 TB/s; a row's few reads follow each
+//      other, so a group of threads begins four rows at a time).
 //   3. merge.  The pieces of each long row, in order (6 us).  Not launched where N cannot hold a long row.
 #include "seq_common.h"
 
@@ -28,6 +29,7 @@ constexpr int kBlock = 256;
 constexpr int kSortBlock = 1024;
 constexpr int kSortWaves = kSortBlock / 64;
 constexpr int kRowsInFlight = 4;  // rows requested before the first is used
+constexpr int kRowsTogether = 4;  // rows of the gradient whose first tokens are requested together
 
 // The last vector of a row shares columns with the one before: both write the same values there.
 __device__ __forceinline__ int at_most(int a, int b) { return a < b ? a : b; }
@@ -268,7 +270,7 @@ __device__ __forceinline__ void add_groups(A (&acc)[n], A (*shared)[kBlock], int
 
 // Workgroups below row_blocks: whole rows.  The others: one piece of the order each; piece p leaves the sum over
 // its first long row in part[p][0] and over the long row it ends in (if another) in part[p][1].
-template <typename E, int BYTES>
+template <typename E, int BYTES, int TOGETHER>
 __global__ void __launch_bounds__(kBlock)
 embed_sum_kernel(const E* __restrict__ grad, const int* __restrict__ start, const int* __restrict__ position,
                  const int* __restrict__ row, E* __restrict__ grad_weight, arith_t<E>* __restrict__ part, int V,
@@ -280,14 +282,36 @@ embed_sum_kernel(const E* __restrict__ grad, const int* __restrict__ start, cons
     const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x >> tpr_log2, groups = kBlock >> tpr_log2;
     const int c0 = (blockIdx.y * tpr + lane) * n, c = at_most(c0, C - n), piece = 1 << piece_log2;
     if (static_cast<int>(blockIdx.x) < row_blocks) {
-        const int64_t v = static_cast<int64_t>(blockIdx.x) * groups + group;
-        if (v >= V) return;
-        const int from = start[v], to = start[v + 1];
-        if (to - from > piece) return;
-        if (c0 >= C) return;
-        A acc[n] = {};
-        add_rows<E, BYTES>(grad, position, from, to, 1, C, c, acc);
-        store_row<E, BYTES>(grad_weight + v * C + c, acc, scale);
+        // rows far apart: frequent words are often neighbours
+        const int64_t v0 = static_cast<int64_t>(blockIdx.x) * groups + group, hop = static_cast<int64_t>(row_blocks) * groups;
+        if (v0 >= V || c0 >= C) return;
+        int from[TOGETHER], count[TOGETHER], at[TOGETHER];
+        Vec<E, BYTES> first[TOGETHER];
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) {
+            const int64_t v = v0 + i * hop < V ? v0 + i * hop : V - 1;
+            from[i] = start[v];
+            count[i] = start[v + 1] - from[i];
+        }
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) {
+            if (v0 + i * hop >= V) count[i] = piece + 1;   // as the long rows: not written here
+            at[i] = count[i] > 0 && count[i] <= piece ? position[from[i]] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) {
+            first[i].raw = typename Vec<E, BYTES>::raw_t(0);
+            if (at[i] >= 0) first[i] = load_vec_once<E, BYTES>(grad + static_cast<int64_t>(at[i]) * C + c);
+        }
+#pragma unroll
+        for (int i = 0; i < TOGETHER; ++i) {
+            if (count[i] > piece) continue;
+            A acc[n];
+#pragma unroll
+            for (int k = 0; k < n; ++k) acc[k] = widen(first[i].e[k]);
+            if (count[i] > 1) add_rows<E, BYTES>(grad, position, from[i] + 1, from[i] + count[i], 1, C, c, acc);
+            store_row<E, BYTES>(grad_weight + (v0 + i * hop) * C + c, acc, scale);
+        }
         return;
     }
     const int p = blockIdx.x - row_blocks;
@@ -396,14 +420,18 @@ hipError_t sums_as(const void* grad, void* grad_weight, char* ws, const Layout& 
                    hipStream_t st) {
     using A = arith_t<E>;
     const int l = log2_threads_per_row(ceil_div(C, Vec<E, BYTES>::n));
-    const int64_t row_blocks = ceil_div(V, kBlock >> l);
+    const int64_t groups = kBlock >> l;
+    // where that leaves eight workgroups for every CU: 32768 tokens, 50000 rows of 512 fp32 columns, the whole gradient
+    // 79 us, 86 with a row each
+    const bool many = V >= kRowsTogether * groups * 2048;
+    const int64_t row_blocks = ceil_div(V, many ? kRowsTogether * groups : groups);
     const int* start = reinterpret_cast<int*>(ws + w.start);
     const int* position = reinterpret_cast<int*>(ws + w.position);
     const int* row = reinterpret_cast<int*>(ws + w.row);
     A* part = reinterpret_cast<A*>(ws + w.part);
     const dim3 grid(static_cast<unsigned>(row_blocks + w.pieces),
                     static_cast<unsigned>(ceil_div(C, int64_t(Vec<E, BYTES>::n) << l)));
-    hipError_t err = launch(embed_sum_kernel<E, BYTES>, grid, dim3(kBlock), st, static_cast<const E*>(grad), start, position, row,
+    hipError_t err = launch(many ? embed_sum_kernel<E, BYTES, kRowsTogether> : embed_sum_kernel<E, BYTES, 1>, grid, dim3(kBlock), st, static_cast<const E*>(grad), start, position, row,
                             static_cast<E*>(grad_weight), part, static_cast<int>(V), static_cast<int>(C),
                             static_cast<A>(scale), static_cast<int>(row_blocks), l, w.piece_log2);
     if (err == hipSuccess && w.pieces > 0)

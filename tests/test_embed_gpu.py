@@ -252,3 +252,18 @@ def test_short_batches_of_long_rows_that_begin_and_end_anywhere(sf):
     tokens = tokens[torch.randperm(tokens.numel(), generator=gen)].reshape(-1, 1)
     grad = torch.randn(*tokens.shape, 50, generator=gen)
     check(sf, tokens, torch.randn(len(counts) + 2, 50, generator=gen), grad, scale=0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("V,C", [(50003, 40), (20001, 7), (17000, 1030)])
+def test_large_tables_with_rows_of_every_length(sf, V, C, dtype):
+    """Tables large enough that a group of threads sums several rows, with 0 to 200 tokens each and pad among them."""
+    gen = torch.Generator().manual_seed(V)
+    rows = torch.randperm(V, generator=gen)[:120]
+    tokens = torch.repeat_interleave(rows, torch.randint(1, 40, (120,), generator=gen))
+    tokens = torch.cat([tokens, torch.full((200,), int(rows[0])), torch.full((3,), V - 1), torch.zeros(2, dtype=torch.long),
+                        torch.full((9,), -1)])
+    tokens = tokens[torch.randperm(tokens.numel(), generator=gen)].reshape(-1, 1)
+    grad = torch.randn(*tokens.shape, C, generator=gen).to(dtype)
+    check(sf, tokens, torch.randn(V, C, generator=gen).to(dtype), grad, scale=0.5)
