@@ -395,6 +395,8 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Ten
     }
     Tensor o = torch::empty(v.sizes(), v.options());
     check_rc(snnseq_gated_delta_step(&d.call, o.data_ptr(), out.data_ptr<float>(), current_stream()), op);
+    // a graph that kept the tensor for its backward has to notice
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     return o;
 }
 

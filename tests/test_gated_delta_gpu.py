@@ -414,3 +414,19 @@ def test_without_gradients_the_same_bits(sf, T, Hk, Hv, Dk, Dv, lengths, dtype):
     with torch.no_grad():
         o, last = sf.gated_delta_func(*(x[n].cuda() for n in NAMES), None if t is None else t.cuda(), 0.2)
     assert torch.equal(o, first["o"]) and torch.equal(last, first["last"])
+
+
+@gpu
+def test_a_step_in_place_is_seen_by_a_graph_that_kept_the_state(sf):
+    x, go, gs = make(3, 1, 1, 1, 16, 16, torch.float32, seed=4)
+    leaf = {n: t.cuda() for n, t in x.items()}
+    leaf["q"].requires_grad_(True)
+    o, last = sf.gated_delta_func(*(leaf[n] for n in NAMES))
+    with torch.no_grad():
+        sf.gated_delta_step(*(leaf[n][0] for n in NAMES[:5]), leaf["state"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():
+        state = torch.zeros(1, 1, 16, 16, device="cuda")
+        sf.gated_delta_step(*(leaf[n][0].detach() for n in NAMES[:5]), state)
+    assert bool((state != 0).any())
