@@ -108,11 +108,6 @@ inline int widest_vector(int64_t count, size_t element_bytes) {
     return bytes;
 }
 
-// Largest power of two of at most 16 that divides every argument: how many bytes one access may move.
-inline int common_bytes(uint64_t a, uint64_t b = 0, uint64_t c = 0, uint64_t d = 0, uint64_t e = 0) {
-    const uint64_t bits = a | b | c | d | e | 16;
-    return static_cast<int>(bits & (~bits + 1));
-}
 inline uint64_t address(const void* p) { return reinterpret_cast<uint64_t>(p); }
 inline bool aligned_to(const void* p, size_t bytes) { return address(p) % bytes == 0; }
 
@@ -126,11 +121,6 @@ inline size_t element_size(int dtype) {
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline int pow2_at_least(int64_t n) {
-    int p = 1;
-    while (p < n) p <<= 1;
-    return p;
-}
 inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 // Launches and returns this launch's own error (an error some earlier call left behind stays there).

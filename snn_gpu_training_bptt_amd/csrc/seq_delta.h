@@ -313,7 +313,7 @@ template <typename E> constexpr int scores_bytes() { return 8 * frag_bytes<typen
 struct DeltaTensor {
     const void* p;
     int64_t t, b, h;   // strides in elements
-    int wide;          // every row begins on 16 bytes and D is a multiple of 8
+    int wide;          // D is a multiple of 8
 };
 
 // Decay of a chunk: the sums c in 64 bits and in units of log 2, a = e^c, d = e^{c_last - c}, and beta.  A row that
@@ -349,7 +349,6 @@ struct DeltaArgs {
     float* state_grads;         // gradient of the state after the chunk, [cols, DKP]
     void *grad_q, *grad_k;      // [T, B, Hk, Dk] of the storage type, or fp32 [T, B, Hv, Dk] where heads share keys
     void* grad_v;               // [T, B, Hv, Dv]
-    int wide_grad_v;            // four of its values in one access
     float *grad_g, *grad_beta;  // [T, B, Hv]
     float* grad_initial;        // [B, Hv, Dk, Dv] or nullptr
 };
@@ -1367,7 +1366,7 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
             for (int j = 0; j < 4; ++j) out.e[j] = narrow<E>(i < w.rows ? beta * dx[j] : 0.f);
             if (i < present && at < args.Dv) {
                 E* p = gv + i * row_step * args.Dv + at;
-                if (args.wide_grad_v) {
+                if (at + 4 <= args.Dv) {
                     store_vec<E, 4 * sizeof(E)>(p, out);
                 } else {
 #pragma unroll

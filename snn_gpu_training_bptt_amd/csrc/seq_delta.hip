@@ -323,7 +323,6 @@ extern "C" int snnseq_gated_delta_bp(const snnseq_delta* call, const void* saved
     a.grad_q = s.partial ? a.queries_t + s.queries : grad_q;
     a.grad_k = s.partial ? a.queries_t + s.queries + s.partial : grad_k;
     a.grad_v = grad_v;
-    a.wide_grad_v = call->Dv % 4 == 0;
     a.grad_g = grad_g;
     a.grad_beta = grad_beta;
     a.grad_initial = grad_state;
