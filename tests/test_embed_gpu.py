@@ -267,3 +267,19 @@ def test_large_tables_with_rows_of_every_length(sf, V, C, dtype):
     tokens = tokens[torch.randperm(tokens.numel(), generator=gen)].reshape(-1, 1)
     grad = torch.randn(*tokens.shape, C, generator=gen).to(dtype)
     check(sf, tokens, torch.randn(V, C, generator=gen).to(dtype), grad, scale=0.5)
+
+
+@gpu
+def test_rows_whose_offset_passes_32_bits(sf):
+    V, C = 4194500, 1024                                        # 4.3e9 values
+    weight = torch.zeros(V, C, dtype=torch.bfloat16, device="cuda")
+    weight[-2:] = torch.randn(2, C, device="cuda").bfloat16()
+    weight.requires_grad_(True)
+    tokens = torch.tensor([[V - 1], [V - 2], [0], [V - 1]], device="cuda")
+    y = sf.embed_func(tokens, weight)
+    assert torch.equal(y.detach(), weight.detach()[tokens])
+    grad = torch.randn(4, 1, C, device="cuda").bfloat16()
+    gw, = torch.autograd.grad(y, weight, grad)
+    assert torch.equal(gw[-1], (grad[0, 0].float() + grad[3, 0].float()).bfloat16())
+    assert torch.equal(gw[-2], grad[1, 0]) and torch.equal(gw[0], grad[2, 0])
+    assert not bool(gw[1:-2].any())

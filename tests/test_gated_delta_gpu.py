@@ -430,3 +430,31 @@ def test_a_step_in_place_is_seen_by_a_graph_that_kept_the_state(sf):
         state = torch.zeros(1, 1, 16, 16, device="cuda")
         sf.gated_delta_step(*(leaf[n][0].detach() for n in NAMES[:5]), state)
     assert bool((state != 0).any())
+
+
+@gpu
+@pytest.mark.parametrize("axis", [0, 1, 2])
+def test_rows_whose_offset_passes_32_bits(sf, axis):
+    """Steps, batch entries or heads 2**31 + 64 values apart, against the same values packed: the same bits."""
+    shape, hop = [(3, 1, 1, 64), (1, 3, 1, 64), (1, 1, 3, 64)][axis], 2 ** 31 + 64
+    room = torch.empty(2 * hop + 64 * 4, dtype=torch.bfloat16, device="cuda")
+    strides = [0, 0, 0, 1]
+    strides[axis] = hop
+    x, go, gs = make(*shape[:3], shape[2], 64, 64, torch.bfloat16, seed=6)
+    far = {}
+    for i, n in enumerate(("q", "k", "v")):
+        far[n] = room.as_strided(shape, strides, 64 * i)
+        far[n].copy_(x[n])
+    far_go = room.as_strided(shape, strides, 64 * 3)
+    far_go.copy_(go)
+    near = run(sf, x, go, gs, None, 0.125)
+    leaf = {n: (far[n] if n in far else x[n].cuda()).requires_grad_(True) for n in NAMES}
+    o, last = sf.gated_delta_func(*(leaf[n] for n in NAMES), None, 0.125)
+    grads = torch.autograd.grad((o, last), [leaf[n] for n in NAMES], (far_go, gs.cuda()))
+    for name, a in zip(["o", "last"] + ["grad_" + n for n in NAMES], (o, last) + grads):
+        assert torch.equal(a.detach(), near[name]), name
+    if axis > 0:
+        with torch.no_grad():
+            step = [sf.gated_delta_step(*(t[n].cuda()[0] for n in NAMES[:5]), x["state"].cuda(), 0.125)
+                    for t in (x, {**x, **{n: far[n].detach() for n in far}})]
+        assert torch.equal(*step)

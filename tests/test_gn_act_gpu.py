@@ -317,3 +317,21 @@ def test_values_that_are_not_finite_stay_in_their_group_where_vectors_overlap(sf
         a, c = (t.reshape(shape[0] * shape[1], -1, groups, cpg) for t in (a, c))
         assert bool(c[0, :, 0].isnan().all())
         assert torch.equal(a[0, :, 1:], c[0, :, 1:]) and torch.equal(a[1:], c[1:])
+
+
+@gpu
+@pytest.mark.parametrize("shape,groups", [((2, 33000, 65536), 64), ((3, 1400, 16, 16, 4096), 64), ((1, 270, 128, 128, 1024), 4)])
+def test_samples_whose_offset_passes_32_bits(sf, shape, groups):
+    """Rows, slab and split layouts over more than 2**32 values: the first and the last sample by themselves."""
+    C = shape[-1]
+    x = torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_()
+    w, b = 1 + 0.1 * torch.randn(C, device="cuda").bfloat16(), 0.1 * torch.randn(C, device="cuda").bfloat16()
+    x.requires_grad_(True)
+    y = sf.gn_act_func(x, w, b, groups, EPS, "silu")
+    gx, = torch.autograd.grad(y, x, x.detach())
+    for t, s in ((0, 0), (shape[0] - 1, shape[1] - 1)):
+        one = x.detach()[t:t + 1, s:s + 1]
+        (y_ref, gx_ref, _, _), (b_y, b_gx, _, _) = with_bounds(one.cpu(), w.cpu(), b.cpu(), one.cpu(), groups, "silu")
+        for a, e, bound in ((y.detach(), y_ref, b_y), (gx, gx_ref, b_gx)):
+            err = (a[t:t + 1, s:s + 1].cpu().double() - e).abs()
+            assert bool((err <= 1.05 * bound + 1e-37).all())
