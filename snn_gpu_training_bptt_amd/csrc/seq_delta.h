@@ -39,12 +39,11 @@
 // (b) 8192 steps of one sequence of 16 heads, nothing kept: inverse 58, state and output 223 (1.74 per chunk).
 //
 // Numbers.  States, R, Tm, dX and every sum are fp32.  In bf16 storage the products run on the bf16 matrix
-// instructions; an input is exact there, and what is derived (Tm, X, R, P, the state, ...) is given as a sum of bf16
-// parts.  Three parts keep all 24 bits and are used wherever a product reaches an fp32 result (the state, the
-// gradients of g and beta): with two, their errors came out ten times those of an fp32 evaluation (4e-6 against 4e-7).
-// Two parts (16 bits) are used where all that follows is a bf16 store.  Products of parts below the last bit kept are
-// left out.  In fp32 storage the products run on the fp32 matrix instructions.  The sums c are held in 64 bits: G
-// needs their differences.
+// instructions; an input is exact there, and what is derived (Tm, X, R, P, the state, ...) is given as a sum of three
+// bf16 parts, which keep all 24 bits.  With two parts errors came out ten times those of an fp32 evaluation (4e-6
+// against 4e-7), and bf16 results were 1.2e-4 by norm from an fp32 evaluation's, 4e-5 with three, as more of them rounded
+// the other way; the third part costs 12 us of 274 on a prompt of 8192 steps.  Products of parts below the last bit kept are left out.  In fp32 storage the products run on the fp32 matrix
+// instructions.  The sums c are held in 64 bits: G needs their differences.
 //
 // Time steps at or behind a sequence's length have no row: they leave the state alone and their outputs are zero.
 #ifndef SNNLIF_SEQ_DELTA_H
@@ -278,34 +277,24 @@ __device__ __forceinline__ void frag_of(const float (&x)[8], FragF& f) {
     for (int j = 0; j < 8; ++j) f.v[j] = x[j];
 }
 
-// The first two parts of three.
-__device__ __forceinline__ FragH<2> coarse(const FragH<3>& f) { return FragH<2>{{f.p[0], f.p[1]}}; }
-__device__ __forceinline__ const FragF& coarse(const FragF& f) { return f; }
-
-// What a storage type computes with: tiles of inputs, and of derived values on the way to fp32 results (Fine) or to
-// results of the storage type (Coarse).
+// What a storage type computes with: tiles of inputs, and of derived values (Fine).
 template <typename E> struct Mode;
 template <> struct Mode<bf16_t> {
     template <int R, int C> using Input = TileH<1, R, C>;
     template <int R, int C> using Fine = TileH<3, R, C>;
-    template <int R, int C> using Coarse = TileH<2, R, C>;
     using InputFrag = FragH<1>;
-    using CoarseFrag = FragH<2>;
     using FineFrag = FragH<3>;
 };
 template <> struct Mode<float> {
     template <int R, int C> using Input = TileF<R, C>;
     template <int R, int C> using Fine = TileF<R, C>;
-    template <int R, int C> using Coarse = TileF<R, C>;
     using InputFrag = FragF;
-    using CoarseFrag = FragF;
     using FineFrag = FragF;
 };
 
 // Bytes of a chunk's operands in this form: keys (or queries) by rows or transposed, and a 64 x 64 matrix.
 template <typename E> constexpr int keys_bytes(int dkp) { return dkp / 8 * frag_bytes<typename Mode<E>::InputFrag>(); }
 template <typename E> constexpr int square_bytes() { return 8 * frag_bytes<typename Mode<E>::FineFrag>(); }
-template <typename E> constexpr int scores_bytes() { return 8 * frag_bytes<typename Mode<E>::CoarseFrag>(); }
 
 // ---- arguments ----------------------------------------------------------------------------------
 
@@ -341,7 +330,7 @@ struct DeltaArgs {
     char *keys, *keys_t;        // per (batch entry, key head, chunk): K by rows, and transposed, fragments
     float* added;               // R, [cols, 64]
     float* states;              // state before the chunk, [cols, DKP]
-    // a forward with its output in the state pass: Q by rows as keys, and P as fragments of two parts; else nullptr
+    // a forward with its output in the state pass: Q by rows as keys, and P as Tm; else nullptr
     char *queries, *scores;
     // backward
     char* queries_t;            // as keys_t
@@ -653,7 +642,7 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
         __device__ First() {}
     };
     union Second {  // and P is in memory
-        typename M::template Coarse<kChunk, kChunk> p;
+        typename M::template Fine<kChunk, kChunk> p;
         Square t;
         __device__ Second() {}
     };
@@ -706,7 +695,7 @@ __global__ void __launch_bounds__(256) delta_inverse_kernel(DeltaArgs args) {
         // a wavefront reads back its own rows only
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-            store_frag(args.scores + w.at * scores_bytes<E>(), wave * 2 + s, z.p.rows(wave * 16, s * 32));
+            store_frag(args.scores + w.at * square_bytes<E>(), wave * 2 + s, z.p.rows(wave * 16, s * 32));
         __syncthreads();
     }
     for (int i = threadIdx.x; i < kChunk * (kChunk + 4); i += 256) (&t.v[0][0])[i] = 0.f;
@@ -813,7 +802,7 @@ struct StateOperands {
     using M = Mode<E>;
     typename M::InputFrag k[DKP / 32], kt[DKP / 64][2], q[OUTPUT ? DKP / 32 : 1];
     typename M::FineFrag inverse[2];
-    typename M::CoarseFrag p[OUTPUT ? 2 : 1];
+    typename M::FineFrag p[OUTPUT ? 2 : 1];
     f32x4 a, d, beta;
     float a_last;
     ColumnAhead<E> v;
@@ -848,7 +837,7 @@ struct StateOperands {
     __device__ __forceinline__ void load_scores(const DeltaArgs& args, const DeltaWhere& w) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-            p[s] = load_frag<typename M::CoarseFrag>(args.scores + w.at * scores_bytes<E>(), (threadIdx.x >> 6) * 2 + s);
+            p[s] = load_frag<typename M::FineFrag>(args.scores + w.at * square_bytes<E>(), (threadIdx.x >> 6) * 2 + s);
     }
 };
 
@@ -859,7 +848,7 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(DeltaArgs ar
     constexpr int NV = kStateCols;
     __shared__ typename M::template Fine<NV, DKP> state;     // transposed
     __shared__ typename M::template Fine<NV, kChunk> x, r;   // transposed; X and d R
-    __shared__ typename M::template Coarse<NV, OUTPUT ? kChunk : 32> plain_r;
+    __shared__ typename M::template Fine<NV, OUTPUT ? kChunk : 32> plain_r;
     const int tiles = args.cols / NV;
     const int piece = piece_in_l2(args.B * args.Hv * tiles), head = piece / tiles, v0 = (piece - head * tiles) * NV;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -890,7 +879,7 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(DeltaArgs ar
         for (int c = 0; c < DKP / 32; ++c) acc[c % 2] = mma(now.k[c], f[c], acc[c % 2]);
         if constexpr (OUTPUT) {
 #pragma unroll
-            for (int c = 0; c < DKP / 32; ++c) o = mma(now.q[c], coarse(f[c]), o);
+            for (int c = 0; c < DKP / 32; ++c) o = mma(now.q[c], f[c], o);
         }
         __builtin_amdgcn_sched_barrier(0);
         now.load_keys(args, w);
@@ -1003,16 +992,19 @@ __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs a
     using M = Mode<E>;
     constexpr int NV = kCols;
     struct Columns {
-        typename M::template Coarse<NV, DKP> state;
-        typename M::template Coarse<NV, kChunk> r;
+        typename M::template Fine<NV, DKP> state;
+        typename M::template Fine<NV, kChunk> r;
     };
-    union Later {   // K is done with before the columns come
+    struct Scores {
         typename M::template Input<kChunk, DKP> k;
+        typename M::template Fine<kChunk, kChunk> p;
+    };
+    union Later {   // K is done with before the columns come, and P is in registers
+        Scores s;
         Columns c;
         __device__ Later() {}
     };
     __shared__ typename M::template Input<kChunk, DKP> q;
-    __shared__ typename M::template Coarse<kChunk, kChunk> p;
     __shared__ Decay y;
     __shared__ Later u;
     const DeltaWhere w = delta_where(args, blockIdx.y, blockIdx.x);
@@ -1041,10 +1033,12 @@ __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs a
         request(0);
         y_next.store(y);
         q_next.store(q);
-        k_next.store(u.k);
+        k_next.store(u.s.k);
     }
     __syncthreads();
-    scores_of<DKP>(q, u.k, y, args.scale, p);
+    scores_of<DKP>(q, u.s.k, y, args.scale, u.s.p);
+    __syncthreads();
+    const typename M::FineFrag p[2] = {u.s.p.rows(band * 16, 0), u.s.p.rows(band * 16, 32)};
     for (int v0 = 0; v0 < args.cols; v0 += NV) {
         __syncthreads();
         state_next.store(u.c.state);
@@ -1056,7 +1050,8 @@ __global__ void __launch_bounds__(kPieceThreads) delta_output_kernel(DeltaArgs a
         for (int s = 0; s < DKP; s += 32) acc = mma(q.rows(band * 16, s), u.c.state.rows(half * 16, s), acc);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] *= args.scale * y.a[lr + e];
-        for (int s = 0; s < band * 16 + 16; s += 32) acc = mma(p.rows(band * 16, s), u.c.r.rows(half * 16, s), acc);
+        acc = mma(p[0], u.c.r.rows(half * 16, 0), acc);
+        if (band >= 2) acc = mma(p[1], u.c.r.rows(half * 16, 32), acc);   // rows below 32 have nothing right of column 32
         const int col = v0 + half * 16 + lc;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -1272,7 +1267,7 @@ __global__ void __launch_bounds__(kPieceThreads) delta_input_grad_kernel(DeltaAr
         typename M::template Fine<NV, DKP> s, ds;
     };
     struct Squares {
-        typename M::template Coarse<kChunk, kChunk> m, n;   // transposed
+        typename M::template Fine<kChunk, kChunk> m, n;   // transposed
     };
     union Shared {   // the columns are done with when M and N come
         Columns c;

@@ -221,7 +221,7 @@ Sizes sizes_of(const snnseq_delta* c, bool for_backward) {
     s.added = s.inner = n * kChunk * static_cast<size_t>(s.cols);
     s.states = s.state_grads = n * static_cast<size_t>(s.dkp * s.cols);
     s.partial = c->Hv == c->Hk ? 0 : round_up(static_cast<size_t>(c->T * s.heads * c->Dk) * sizeof(float), 16);
-    s.scores = static_cast<size_t>(s.pieces) * (f32 ? scores_bytes<float>() : scores_bytes<bf16_t>());
+    s.scores = static_cast<size_t>(s.pieces) * (f32 ? square_bytes<float>() : square_bytes<bf16_t>());
     s.saved = s.decay + s.inverse + 2 * s.keys + (for_backward ? s.inverse + s.added + s.states : s.queries + s.scores);
     s.workspace = s.inner + s.state_grads + s.queries + 2 * s.partial;
     return s;
