@@ -33,6 +33,13 @@ namespace {
 using torch::Tensor;
 using DeviceGuard = c10::hip::HIPGuardMasqueradingAsCUDA;
 
+// The kernels know nothing of tangents: an operand that carries one would give a result without, a derivative of zero.
+void check_no_tangent(const char* op, std::initializer_list<const Tensor*> operands) {
+    for (const Tensor* t : operands)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "snnlib.", op,
+                    ": forward-mode derivatives are not supported");
+}
+
 void check_on_gpu(const Tensor& t, const char* op, const char* name) {
     TORCH_CHECK(t.defined(), "snnlib.", op, ": ", name, " is undefined");
     TORCH_CHECK(t.is_cuda(), "snnlib.", op, ": ", name,
@@ -84,6 +91,7 @@ int token_dtype(const Tensor& tokens, const char* op) {
 
 Tensor embed_fp(Tensor tokens, Tensor weight, double scale) {
     const char* op = "embed_fp";
+    check_no_tangent(op, {&weight});
     const int tdtype = token_dtype(tokens, op);
     check_on_gpu(weight, op, "weight");
     TORCH_CHECK(weight.device() == tokens.device(), "snnlib.", op, ": weight (", weight.device(),
@@ -105,6 +113,7 @@ Tensor embed_fp(Tensor tokens, Tensor weight, double scale) {
 
 Tensor embed_bp(Tensor tokens, Tensor grad_out, int64_t vocab, double scale) {
     const char* op = "embed_bp";
+    check_no_tangent(op, {&grad_out});
     const int tdtype = token_dtype(tokens, op);
     check_on_gpu(grad_out, op, "grad_out");
     TORCH_CHECK(grad_out.device() == tokens.device(), "snnlib.", op, ": grad_out (", grad_out.device(),
@@ -171,6 +180,7 @@ GnOperands gn_operands(const Tensor& x, const Tensor& weight_gn, const Tensor& b
 std::vector<Tensor> gn_act_fp(Tensor x, Tensor weight_gn, Tensor bias_gn, int64_t groups, double eps_gn,
                               const std::string& act) {
     const char* op = "gn_act_fp";
+    check_no_tangent(op, {&x, &weight_gn, &bias_gn});
     const int code = act_code(act, op);
     TORCH_CHECK(eps_gn >= 0, "snnlib.", op, ": eps_gn must not be negative, got ", eps_gn);
     check_on_gpu(x, op, "x");
@@ -193,6 +203,7 @@ std::vector<Tensor> gn_act_fp(Tensor x, Tensor weight_gn, Tensor bias_gn, int64_
 std::vector<Tensor> gn_act_bp(Tensor x, Tensor weight_gn, Tensor bias_gn, Tensor mean, Tensor rstd, int64_t groups,
                               const std::string& act, Tensor grad_y) {
     const char* op = "gn_act_bp";
+    check_no_tangent(op, {&x, &weight_gn, &bias_gn, &mean, &rstd, &grad_y});
     const int code = act_code(act, op);
     check_on_gpu(x, op, "x");
     const DeviceGuard guard(x.device());
@@ -318,6 +329,8 @@ DeltaOperands delta_operands(const Tensor& q, const Tensor& k, const Tensor& v, 
 std::vector<Tensor> gated_delta_fp(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, MaybeTensor state,
                                    MaybeTensor lengths, double scale, bool for_backward) {
     const char* op = "gated_delta_fp";
+    const Tensor initial = state.value_or(Tensor());
+    check_no_tangent(op, {&q, &k, &v, &g, &beta, &initial});
     check_on_gpu(q, op, "q");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
@@ -336,6 +349,8 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
                                    MaybeTensor lengths, double scale, Tensor saved, Tensor grad_o,
                                    MaybeTensor grad_state_out) {
     const char* op = "gated_delta_bp";
+    const Tensor initial = state.value_or(Tensor()), grad_last = grad_state_out.value_or(Tensor());
+    check_no_tangent(op, {&q, &k, &v, &g, &beta, &initial, &grad_o, &grad_last});
     check_on_gpu(q, op, "q");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
@@ -347,8 +362,8 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
                     static_cast<size_t>(saved.numel()) == snnseq_gated_delta_saved_bytes(&d.call, 1),
                 "snnlib.", op, ": saved must be what gated_delta_fp returned for these operands");
     Tensor go = dense_rows(grad_o), gs;
-    if (grad_state_out.has_value() && grad_state_out->defined()) {
-        gs = *grad_state_out;
+    if (grad_last.defined()) {
+        gs = grad_last;
         TORCH_CHECK(gs.is_cuda() && gs.device() == q.device() && gs.scalar_type() == at::kFloat && gs.dim() == 4 &&
                         gs.size(0) == d.call.B && gs.size(1) == d.call.Hv && gs.size(2) == d.call.Dk &&
                         gs.size(3) == d.call.Dv,
@@ -379,11 +394,13 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Ten
     const char* op = "gated_delta_step";
     TORCH_CHECK(!records({&q, &k, &v, &g, &beta, &state}), "snnlib.", op, ": a step is not differentiable: call it with "
                 "gradients off, or use gated_delta");
+    const Tensor result = state_out.value_or(Tensor());
+    check_no_tangent(op, {&q, &k, &v, &g, &beta, &state, &result});
     check_on_gpu(q, op, "q");
     check_on_gpu(state, op, "state");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, c10::nullopt, scale, 3, op);
-    Tensor out = state_out.has_value() && state_out->defined() ? *state_out : state;
+    Tensor out = result.defined() ? result : state;
     TORCH_CHECK(state.is_contiguous() && out.is_contiguous() && out.device() == q.device() &&
                     out.scalar_type() == at::kFloat && out.sizes() == state.sizes(),
                 "snnlib.", op, ": the state is updated in place, or into state_out: both must be dense float32 ",

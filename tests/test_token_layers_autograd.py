@@ -1,0 +1,66 @@
+"""What autograd and graph tracers must not get from the token layers in silence: every entry either takes part or refuses."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from snn_gpu_training_bptt_amd import lif_cabi  # noqa: F401  (fails loudly without the built library)
+from snn_gpu_training_bptt_amd import snnlib_func as sf
+
+devices = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+
+
+def operands(device):
+    """Per entry: the call, and its floating operands by name."""
+    gen = torch.Generator().manual_seed(0)
+    rand = lambda *s: torch.randn(*s, generator=gen).to(device)
+    tokens = torch.randint(0, 5, (3, 2), generator=gen).to(device)
+    rule = dict(q=rand(3, 2, 1, 4), k=0.3 * rand(3, 2, 1, 4), v=rand(3, 2, 1, 4), g=-rand(3, 2, 1).abs(),
+                beta=rand(3, 2, 1).sigmoid(), state=rand(2, 1, 4, 4))
+    row = {n: t if n == "state" else t[0] for n, t in rule.items()}
+    norm = dict(x=rand(3, 2, 4), weight=rand(4), bias=rand(4))
+    six = lambda a: [a[n] for n in ("q", "k", "v", "g", "beta", "state")]
+    return {
+        "embed": (lambda a: sf.embed_func(tokens, a["weight"]), dict(weight=rand(5, 4))),
+        "embed_fp": (lambda a: sf.snnlib.embed_fp(tokens, a["weight"], 1.0), dict(weight=rand(5, 4))),
+        "embed_bp": (lambda a: sf.snnlib.embed_bp(tokens, a["grad"], 5, 1.0), dict(grad=rand(3, 2, 4))),
+        "gn_act": (lambda a: sf.gn_act_func(a["x"], a["weight"], a["bias"], 2), norm),
+        "gn_act_fp": (lambda a: sf.snnlib.gn_act_fp(a["x"], a["weight"], a["bias"], 2, 1e-5, "silu"), norm),
+        "gn_act_bp": (lambda a: sf.snnlib.gn_act_bp(a["x"], a["weight"], a["bias"], a["mean"], a["rstd"], 2, "silu", a["grad"]),
+                      dict(norm, mean=rand(3, 2, 2), rstd=rand(3, 2, 2).abs(), grad=rand(3, 2, 4))),
+        "gated_delta": (lambda a: sf.gated_delta_func(*six(a)), rule),
+        "gated_delta_fp": (lambda a: sf.snnlib.gated_delta_fp(*six(a), None, 1.0), rule),
+        "gated_delta_bp": (lambda a: sf.snnlib.gated_delta_bp(*six(a), None, 1.0, torch.empty(0, dtype=torch.uint8, device=device),
+                                                              a["grad"], a["grad_state"]),
+                           dict(rule, grad=rand(3, 2, 1, 4), grad_state=rand(2, 1, 4, 4))),
+        "gated_delta_step": (lambda a: sf.gated_delta_step(*six(a), None, a["state_out"]), dict(row, state_out=rand(2, 1, 4, 4))),
+    }
+
+
+ENTRIES = list(operands("cpu"))
+
+
+@devices
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_forward_mode_is_refused(entry, device):
+    """A tangent on any operand, with and without gradients: an error, never an output without a tangent."""
+    call, args = operands(device)[entry]
+    for name in args:
+        for grad in (False, True):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                dual = dict(args)
+                primal = args[name].clone().requires_grad_(grad and entry in ("embed", "gn_act", "gated_delta"))
+                dual[name] = forward_ad.make_dual(primal, torch.ones_like(primal))
+                with pytest.raises((RuntimeError, NotImplementedError), match="forward-mode|Jacobian-vector product"):
+                    call(dual)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entry", ["embed", "gn_act", "gated_delta"])
+def test_forward_mode_through_a_backward_is_refused(entry):
+    call, args = operands("cuda")[entry]
+    leaf = {n: t.requires_grad_(True) for n, t in args.items()}
+    y = call(leaf)
+    y = y[0] if isinstance(y, tuple) else y
+    with forward_ad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward-mode"):
+            torch.autograd.grad(y, list(leaf.values()), forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), allow_unused=True)
