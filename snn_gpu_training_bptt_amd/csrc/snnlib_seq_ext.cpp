@@ -19,6 +19,9 @@
 // code and no fallback.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -33,8 +36,13 @@ namespace {
 using torch::Tensor;
 using DeviceGuard = c10::hip::HIPGuardMasqueradingAsCUDA;
 
-// The kernels know nothing of tangents: an operand that carries one would give a result without, a derivative of zero.
-void check_no_tangent(const char* op, std::initializer_list<const Tensor*> operands) {
+// What would come out wrong without an error.  A tracer records the allocation of an output and not the kernel that fills
+// it: the graph would return whatever the memory holds.  And the kernels know nothing of tangents: an operand that carries
+// one would give a result without, a derivative of zero.
+void check_eager(const char* op, std::initializer_list<const Tensor*> operands) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                "snnlib.", op, ": cannot be recorded by torch.jit.trace or make_fx");
     for (const Tensor* t : operands)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "snnlib.", op,
                     ": forward-mode derivatives are not supported");
@@ -91,7 +99,7 @@ int token_dtype(const Tensor& tokens, const char* op) {
 
 Tensor embed_fp(Tensor tokens, Tensor weight, double scale) {
     const char* op = "embed_fp";
-    check_no_tangent(op, {&weight});
+    check_eager(op, {&weight});
     const int tdtype = token_dtype(tokens, op);
     check_on_gpu(weight, op, "weight");
     TORCH_CHECK(weight.device() == tokens.device(), "snnlib.", op, ": weight (", weight.device(),
@@ -113,7 +121,7 @@ Tensor embed_fp(Tensor tokens, Tensor weight, double scale) {
 
 Tensor embed_bp(Tensor tokens, Tensor grad_out, int64_t vocab, double scale) {
     const char* op = "embed_bp";
-    check_no_tangent(op, {&grad_out});
+    check_eager(op, {&grad_out});
     const int tdtype = token_dtype(tokens, op);
     check_on_gpu(grad_out, op, "grad_out");
     TORCH_CHECK(grad_out.device() == tokens.device(), "snnlib.", op, ": grad_out (", grad_out.device(),
@@ -180,7 +188,7 @@ GnOperands gn_operands(const Tensor& x, const Tensor& weight_gn, const Tensor& b
 std::vector<Tensor> gn_act_fp(Tensor x, Tensor weight_gn, Tensor bias_gn, int64_t groups, double eps_gn,
                               const std::string& act) {
     const char* op = "gn_act_fp";
-    check_no_tangent(op, {&x, &weight_gn, &bias_gn});
+    check_eager(op, {&x, &weight_gn, &bias_gn});
     const int code = act_code(act, op);
     TORCH_CHECK(eps_gn >= 0, "snnlib.", op, ": eps_gn must not be negative, got ", eps_gn);
     check_on_gpu(x, op, "x");
@@ -203,7 +211,7 @@ std::vector<Tensor> gn_act_fp(Tensor x, Tensor weight_gn, Tensor bias_gn, int64_
 std::vector<Tensor> gn_act_bp(Tensor x, Tensor weight_gn, Tensor bias_gn, Tensor mean, Tensor rstd, int64_t groups,
                               const std::string& act, Tensor grad_y) {
     const char* op = "gn_act_bp";
-    check_no_tangent(op, {&x, &weight_gn, &bias_gn, &mean, &rstd, &grad_y});
+    check_eager(op, {&x, &weight_gn, &bias_gn, &mean, &rstd, &grad_y});
     const int code = act_code(act, op);
     check_on_gpu(x, op, "x");
     const DeviceGuard guard(x.device());
@@ -330,7 +338,7 @@ std::vector<Tensor> gated_delta_fp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
                                    MaybeTensor lengths, double scale, bool for_backward) {
     const char* op = "gated_delta_fp";
     const Tensor initial = state.value_or(Tensor());
-    check_no_tangent(op, {&q, &k, &v, &g, &beta, &initial});
+    check_eager(op, {&q, &k, &v, &g, &beta, &initial});
     check_on_gpu(q, op, "q");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
@@ -350,7 +358,7 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
                                    MaybeTensor grad_state_out) {
     const char* op = "gated_delta_bp";
     const Tensor initial = state.value_or(Tensor()), grad_last = grad_state_out.value_or(Tensor());
-    check_no_tangent(op, {&q, &k, &v, &g, &beta, &initial, &grad_o, &grad_last});
+    check_eager(op, {&q, &k, &v, &g, &beta, &initial, &grad_o, &grad_last});
     check_on_gpu(q, op, "q");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, lengths, scale, 4, op);
@@ -395,7 +403,7 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Ten
     TORCH_CHECK(!records({&q, &k, &v, &g, &beta, &state}), "snnlib.", op, ": a step is not differentiable: call it with "
                 "gradients off, or use gated_delta");
     const Tensor result = state_out.value_or(Tensor());
-    check_no_tangent(op, {&q, &k, &v, &g, &beta, &state, &result});
+    check_eager(op, {&q, &k, &v, &g, &beta, &state, &result});
     check_on_gpu(q, op, "q");
     check_on_gpu(state, op, "state");
     const DeviceGuard guard(q.device());

@@ -64,3 +64,21 @@ def test_forward_mode_through_a_backward_is_refused(entry):
     with forward_ad.dual_level():
         with pytest.raises((RuntimeError, NotImplementedError), match="forward-mode"):
             torch.autograd.grad(y, list(leaf.values()), forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), allow_unused=True)
+
+
+@devices
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_recording_a_graph_is_refused(entry, grad, device):
+    """A tracer sees an output's allocation and not the kernel that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, args = operands(device)[entry]
+    names = list(args)
+    tracked = grad and entry in ("embed", "gn_act", "gated_delta")
+    values = tuple(args[n].clone().requires_grad_(tracked) for n in names)
+    run = lambda *t: call(dict(zip(names, t)))
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        torch.jit.trace(run, values, check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        make_fx(run)(*(t.detach() for t in values))
+
