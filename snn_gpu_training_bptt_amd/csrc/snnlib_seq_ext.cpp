@@ -52,6 +52,8 @@ void check_on_gpu(const Tensor& t, const char* op, const char* name) {
     TORCH_CHECK(t.defined(), "snnlib.", op, ": ", name, " is undefined");
     TORCH_CHECK(t.is_cuda(), "snnlib.", op, ": ", name,
                 " must live on a ROCm GPU (this build has no CPU path), got device ", t.device());
+    // a fake tensor's address is its offset alone, and a kernel would follow it
+    TORCH_CHECK(t.numel() == 0 || t.storage().data() != nullptr, "snnlib.", op, ": ", name, " has no memory (a fake tensor)");
 }
 
 int storage_dtype(const Tensor& t, const char* op, const char* name) {
@@ -365,14 +367,15 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
     check_like(grad_o, q, op, "grad_o", "q");
     TORCH_CHECK(grad_o.sizes() == v.sizes(), "snnlib.", op, ": grad_o ", grad_o.sizes(), " and v ", v.sizes(),
                 " must have the same shape");
-    TORCH_CHECK(saved.defined() && saved.is_cuda() && saved.device() == q.device() && saved.scalar_type() == at::kByte &&
-                    saved.is_contiguous() &&
+    check_on_gpu(saved, op, "saved");
+    TORCH_CHECK(saved.device() == q.device() && saved.scalar_type() == at::kByte && saved.is_contiguous() &&
                     static_cast<size_t>(saved.numel()) == snnseq_gated_delta_saved_bytes(&d.call, 1),
                 "snnlib.", op, ": saved must be what gated_delta_fp returned for these operands");
     Tensor go = dense_rows(grad_o), gs;
     if (grad_last.defined()) {
         gs = grad_last;
-        TORCH_CHECK(gs.is_cuda() && gs.device() == q.device() && gs.scalar_type() == at::kFloat && gs.dim() == 4 &&
+        check_on_gpu(gs, op, "grad_state_out");
+        TORCH_CHECK(gs.device() == q.device() && gs.scalar_type() == at::kFloat && gs.dim() == 4 &&
                         gs.size(0) == d.call.B && gs.size(1) == d.call.Hv && gs.size(2) == d.call.Dk &&
                         gs.size(3) == d.call.Dv,
                     "snnlib.", op, ": grad_state_out must be shaped and typed as the state, got ", gs.scalar_type(), " ",
@@ -408,6 +411,7 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Ten
     check_on_gpu(state, op, "state");
     const DeviceGuard guard(q.device());
     const DeltaOperands d = delta_operands(q, k, v, g, beta, state, c10::nullopt, scale, 3, op);
+    if (result.defined()) check_on_gpu(result, op, "state_out");
     Tensor out = result.defined() ? result : state;
     TORCH_CHECK(state.is_contiguous() && out.is_contiguous() && out.device() == q.device() &&
                     out.scalar_type() == at::kFloat && out.sizes() == state.sizes(),

@@ -82,3 +82,49 @@ def test_recording_a_graph_is_refused(entry, grad, device):
     with pytest.raises(RuntimeError, match="cannot be recorded"):
         make_fx(run)(*(t.detach() for t in values))
 
+
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_fake_tensors_are_refused(entry):
+    """They are on a GPU by name, and their address is their offset: nothing a kernel may follow."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        call, args = operands("cuda")[entry]
+        for offset in (0, 3):
+            views = {}
+            for n, t in args.items():
+                wide = torch.empty(t.numel() + offset, device="cuda")
+                views[n] = wide[offset:].view(t.shape)
+            with pytest.raises(RuntimeError, match="has no memory"):
+                call(views)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_one_fake_tensor_among_others_is_refused(entry):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    call, args = operands("cuda")[entry]
+    for name in args:
+        mode = FakeTensorMode()
+        fake = mode.from_tensor(torch.empty(args[name].numel() + 3, device="cuda"))
+        with mode:
+            fake = fake[3:].view(args[name].shape)
+        with pytest.raises(RuntimeError, match="has no memory|what gated_delta_fp returned"):
+            call({**args, name: fake})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entry", ["embed", "gn_act", "gated_delta"])
+def test_function_transforms_are_refused(entry):
+    call, args = operands("cuda")[entry]
+    names = list(args)
+
+    def run(*t):
+        y = call(dict(zip(names, t)))
+        return (y[0] if isinstance(y, tuple) else y).sum()
+
+    with pytest.raises(RuntimeError):
+        torch.func.grad(run)(*args.values())
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(run, tuple(args.values()), tuple(args.values()))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(run)(*(t.expand(2, *t.shape) for t in args.values()))
