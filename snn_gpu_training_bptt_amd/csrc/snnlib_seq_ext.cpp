@@ -403,9 +403,9 @@ std::vector<Tensor> gated_delta_bp(Tensor q, Tensor k, Tensor v, Tensor g, Tenso
 Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor state, double scale,
                         MaybeTensor state_out) {
     const char* op = "gated_delta_step";
-    TORCH_CHECK(!records({&q, &k, &v, &g, &beta, &state}), "snnlib.", op, ": a step is not differentiable: call it with "
-                "gradients off, or use gated_delta");
     const Tensor result = state_out.value_or(Tensor());
+    TORCH_CHECK(!records({&q, &k, &v, &g, &beta, &state, &result}), "snnlib.", op, ": a step is not differentiable: call it "
+                "with gradients off, or use gated_delta");
     check_eager(op, {&q, &k, &v, &g, &beta, &state, &result});
     check_on_gpu(q, op, "q");
     check_on_gpu(state, op, "state");

@@ -320,7 +320,7 @@ def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
 def gated_delta_step(q, k, v, g, beta, state, scale=None, state_out=None):
     """One step of the gated delta rule for generation: ``q``, ``k`` ``[B, Hk, Dk]``, ``v`` ``[B, Hv, Dv]``, ``g``, ``beta``
     ``[B, Hv]``; returns ``o`` ``[B, Hv, Dv]`` and updates ``state`` in place, or writes the new state to ``state_out``.
-    Not differentiable: operands that require a gradient are refused unless gradients are off."""
+    Not differentiable: operands (and a ``state_out``) that require a gradient are refused unless gradients are off."""
     return snnlib.gated_delta_step(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale, state_out)
 
 

@@ -128,3 +128,20 @@ def test_function_transforms_are_refused(entry):
         torch.func.jvp(run, tuple(args.values()), tuple(args.values()))
     with pytest.raises(RuntimeError):
         torch.func.vmap(run)(*(t.expand(2, *t.shape) for t in args.values()))
+
+
+@devices
+def test_a_step_into_a_tracked_state_is_refused(device):
+    """state_out is overwritten: with gradients on, a parameter or a result with a history would keep what it no longer
+    is the result of."""
+    call, args = operands(device)["gated_delta_step"]
+    leaf = args["state_out"].requires_grad_(True)
+    for tracked in (leaf, leaf * 2):
+        kept = tracked.detach().clone()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call({**args, "state_out": tracked})
+        assert torch.equal(tracked.detach(), kept)
+    if device == "cuda":
+        with torch.no_grad():
+            call({**args, "state_out": leaf})
+        assert not torch.equal(leaf.detach(), kept)
