@@ -310,7 +310,8 @@ embed_sum_kernel(const E* __restrict__ grad, const int* __restrict__ start, cons
 #pragma unroll
             for (int k = 0; k < n; ++k) acc[k] = widen(first[i].e[k]);
             if (count[i] > 1) add_rows<E, BYTES>(grad, position, from[i] + 1, from[i] + count[i], 1, C, c, acc);
-            store_row<E, BYTES>(grad_weight + (v0 + i * hop) * C + c, acc, scale);
+            // a row without a token is zero: scale * 0 would be NaN for an infinite scale
+            store_row<E, BYTES>(grad_weight + (v0 + i * hop) * C + c, acc, count[i] > 0 ? scale : A(0));
         }
         return;
     }

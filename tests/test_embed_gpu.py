@@ -283,3 +283,18 @@ def test_rows_whose_offset_passes_32_bits(sf):
     assert torch.equal(gw[-1], (grad[0, 0].float() + grad[3, 0].float()).bfloat16())
     assert torch.equal(gw[-2], grad[1, 0]) and torch.equal(gw[0], grad[2, 0])
     assert not bool(gw[1:-2].any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("V,C", [(9, 12), (50003, 40)])
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan")])
+def test_a_scale_that_is_not_finite_leaves_rows_without_a_token_zero(sf, scale, V, C, dtype):
+    tokens = torch.tensor([[3, -1], [V - 1, V]]).cuda()
+    w = torch.ones(V, C, dtype=dtype, device="cuda", requires_grad=True)
+    y = sf.embed_func(tokens, w, scale)
+    assert bool((y[0, 1] == 0).all()) and bool((y[1, 1] == 0).all())
+    gw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    held = torch.zeros(V, dtype=torch.bool, device="cuda")
+    held[[3, V - 1]] = True
+    assert bool((gw[~held] == 0).all()) and not bool(gw[held].isfinite().any())
