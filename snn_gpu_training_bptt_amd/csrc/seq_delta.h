@@ -42,8 +42,9 @@
 // instructions; an input is exact there, and what is derived (Tm, X, R, P, the state, ...) is given as a sum of three
 // bf16 parts, which keep all 24 bits.  With two parts errors came out ten times those of an fp32 evaluation (4e-6
 // against 4e-7), and bf16 results were 1.2e-4 by norm from an fp32 evaluation's, 4e-5 with three, as more of them rounded
-// the other way; the third part costs 12 us of 274 on a prompt of 8192 steps.  Products of parts below the last bit kept are left out.  In fp32 storage the products run on the fp32 matrix
-// instructions.  The sums c are held in 64 bits: G needs their differences.
+// the other way; the third part costs 12 us of 274 on a prompt of 8192 steps.  Products of parts below the last bit kept
+// are left out.  In fp32 storage the products run on the fp32 matrix instructions.  The sums c are held in 64 bits: G
+// needs their differences.
 //
 // Time steps at or behind a sequence's length have no row: they leave the state alone and their outputs are zero.
 #ifndef SNNLIF_SEQ_DELTA_H
@@ -121,11 +122,12 @@ __device__ __forceinline__ void split(const float (&x)[n], uint32_t (&words)[N][
         }
 }
 
-// A matrix in LDS as N bf16 parts, row-major; 16 bytes of padding per row spread the rows over the banks.
+// A matrix in LDS as N bf16 parts, row-major; 16 bytes of padding per row spread the rows over the banks.  Read and
+// written in vectors of 16 bytes, like every struct below that lies in LDS: each asks for that alignment.
 template <int N, int ROWS, int COLS>
 struct TileH {
     static constexpr int ld = COLS + 8;
-    uint16_t v[N][ROWS * ld];
+    alignas(16) uint16_t v[N][ROWS * ld];
 
     // n consecutive columns, c a multiple of 4
     template <int n>
@@ -201,7 +203,7 @@ struct TileH {
 template <int ROWS, int COLS>
 struct TileF {
     static constexpr int ld = COLS + 4;
-    float v[ROWS * ld];
+    alignas(16) float v[ROWS * ld];
 
     template <int n>
     __device__ __forceinline__ void put(int r, int c, const float (&x)[n]) {
@@ -241,6 +243,8 @@ struct TileF {
         return f;
     }
 };
+
+static_assert(alignof(TileH<1, 16, 32>) == 16 && alignof(TileF<16, 32>) == 16, "tiles are accessed in vectors of 16 bytes");
 
 // Fragments in memory: 64 lanes times 16 bytes are one run, so that a wavefront reads an operand of its products
 // straight into registers, one access of 1 KiB per part, without LDS and with one address.
@@ -307,7 +311,7 @@ struct DeltaTensor {
 
 // Decay of a chunk: the sums c in 64 bits and in units of log 2, a = e^c, d = e^{c_last - c}, and beta.  A row that
 // does not exist has g = 0 and beta = 0.
-struct Decay {
+struct alignas(16) Decay {
     double c[kChunk];
     float a[kChunk], d[kChunk], beta[kChunk];
 };
@@ -550,7 +554,7 @@ struct DecayAhead {
         if (threadIdx.x < n) reinterpret_cast<u32x4*>(&out)[threadIdx.x] = x;
     }
 };
-static_assert(sizeof(Decay) % 16 == 0, "a Decay is copied in vectors");
+static_assert(alignof(Decay) == 16, "a Decay is copied in vectors");
 
 __device__ __forceinline__ float gap(const Decay& y, int i, int j) {  // G_ij
     return __builtin_amdgcn_exp2f(static_cast<float>(y.c[i] - y.c[j]));
@@ -583,7 +587,7 @@ __device__ __forceinline__ void store_transposed(const Tile& tile, char* out) {
 
 // ---- Tm = (I + A)^-1 ----------------------------------------------------------------------------
 
-struct Square { float v[kChunk][kChunk + 4]; };
+struct Square { alignas(16) float v[kChunk][kChunk + 4]; };
 
 // 16 x 16 products of blocks of fp32 squares on the fp32 matrix instructions (16 x 16 x 4).
 __device__ __forceinline__ f32x4 block_product(const Square& x, int xr, int xc, const Square& y, int yr, int yc, f32x4 acc) {
