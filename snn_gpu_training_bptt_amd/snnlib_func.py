@@ -304,6 +304,10 @@ def gn_act_func(x, weight_gn, bias_gn, groups, eps_gn=1e-5, act="none"):
     return snnlib.gn_act(x, weight_gn, bias_gn, groups, eps_gn, act)
 
 
+def _key_scale(q):
+    return max(q.shape[-1], 1) ** -0.5      # keys of no values are refused by the call
+
+
 def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
     """The gated delta rule over ``T`` steps: ``(o, last state)``.
 
@@ -314,14 +318,14 @@ def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
     a multiple of ``Hk``, ``Dk`` up to 128), ``g`` (at most zero) and ``beta`` ``[T, B, Hv]`` float32, ``state``
     ``[B, Hv, Dk, Dv]`` float32, ``lengths`` ``[B]`` int32: steps at or behind a sequence's length do not exist.
     ``scale`` defaults to ``Dk ** -0.5``.  Where a gradient will be asked for, the state before every 64th step is kept."""
-    return snnlib.gated_delta(q, k, v, g, beta, state, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
+    return snnlib.gated_delta(q, k, v, g, beta, state, lengths, _key_scale(q) if scale is None else scale)
 
 
 def gated_delta_step(q, k, v, g, beta, state, scale=None, state_out=None):
     """One step of the gated delta rule for generation: ``q``, ``k`` ``[B, Hk, Dk]``, ``v`` ``[B, Hv, Dv]``, ``g``, ``beta``
     ``[B, Hv]``; returns ``o`` ``[B, Hv, Dv]`` and updates ``state`` in place, or writes the new state to ``state_out``.
     Not differentiable: operands (and a ``state_out``) that require a gradient are refused unless gradients are off."""
-    return snnlib.gated_delta_step(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale, state_out)
+    return snnlib.gated_delta_step(q, k, v, g, beta, state, _key_scale(q) if scale is None else scale, state_out)
 
 
 fire_func = FireFunc.apply

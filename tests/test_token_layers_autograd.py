@@ -145,3 +145,15 @@ def test_a_step_into_a_tracked_state_is_refused(device):
         with torch.no_grad():
             call({**args, "state_out": leaf})
         assert not torch.equal(leaf.detach(), kept)
+
+
+@devices
+def test_keys_without_values_are_refused_as_such(device):
+    """Also where the scale is left to its default, Dk ** -0.5."""
+    q, g = torch.zeros(3, 2, 1, 0, device=device), torch.zeros(3, 2, 1, device=device)
+    v, state = torch.zeros(3, 2, 1, 4, device=device), torch.zeros(2, 1, 0, 4, device=device)
+    match = "ROCm GPU" if device == "cpu" else "keys of 1 to 128"
+    with pytest.raises(RuntimeError, match=match):
+        sf.gated_delta_func(q, q, v, g, g, state)
+    with pytest.raises(RuntimeError, match=match):
+        sf.gated_delta_step(q[0], q[0], v[0], g[0], g[0], state)
