@@ -458,3 +458,40 @@ def test_rows_whose_offset_passes_32_bits(sf, axis):
             step = [sf.gated_delta_step(*(t[n].cuda()[0] for n in NAMES[:5]), x["state"].cuda(), 0.125)
                     for t in (x, {**x, **{n: far[n].detach() for n in far}})]
         assert torch.equal(*step)
+
+
+@gpu
+@both
+def test_steps_captured_and_replayed(sf, dtype):
+    """A generated token per replay, the state updated in place, with eager work and waits between the replays."""
+    T = 6
+    x, _, _ = make(T, 3, 1, 2, 64, 40, dtype, seed=21)
+    y = {n: t.cuda() for n, t in x.items()}
+    row = {n: y[n][0].clone() for n in NAMES[:5]}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sf.gated_delta_step(*row.values(), y["state"].clone(), 0.3)
+    torch.cuda.current_stream().wait_stream(side)
+    eager, replayed = y["state"].clone(), y["state"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sf.gated_delta_step(*row.values(), replayed, 0.3)
+    for t in range(T):
+        for n in row:
+            row[n].copy_(y[n][t])
+        graph.replay()
+        want = sf.gated_delta_step(*row.values(), eager, 0.3)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(replayed, eager)
+
+
+@gpu
+@both
+def test_a_backward_leaves_what_it_reads_as_it_was(sf, dtype):
+    """Twice over one graph: the same bits."""
+    x, go, gs = make(150, 2, 1, 2, 64, 40, dtype, seed=22)
+    leaf = {n: t.cuda().requires_grad_(True) for n, t in x.items()}
+    o, last = sf.gated_delta_func(*(leaf[n] for n in NAMES), None, 0.3)
+    grads = [torch.autograd.grad((o, last), list(leaf.values()), (go.cuda(), gs.cuda()), retain_graph=True) for _ in range(2)]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
