@@ -31,7 +31,7 @@ int snnseq_abi_version(void);
 #define SNNSEQ_TOKEN_I32 0
 #define SNNSEQ_TOKEN_I64 1
 
-/* Most tokens in a call, most rows in a table, and most columns of a row. */
+/* Most tokens in a call (or positions of a sample, or samples times groups), most rows in a table, most columns of a row. */
 #define SNNSEQ_MAX_TOKENS   8388608
 #define SNNSEQ_MAX_CHANNELS 1048576
 
@@ -44,7 +44,7 @@ int snnseq_embed_fp(const void* tokens, const void* weight, void* out, int dtype
                     int64_t V, int64_t C, int64_t row_stride, double scale, void* stream);
 
 /* Bytes of device workspace snnseq_embed_bp needs: the sorted order (8 bytes per token, 4 per table row) and two
- * partial sums of a row per 64 tokens.  0 for invalid arguments. */
+ * partial sums of a row per 16 tokens, 32 where there are more than 8192.  0 for invalid arguments. */
 size_t snnseq_embed_bp_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t C);
 
 /*
@@ -67,8 +67,8 @@ int snnseq_embed_bp(const void* tokens, const void* grad, void* grad_weight, int
  * group, over its P * C/G values:
  *   mean = E[x],  rstd = 1 / sqrt(E[(x - mean)^2] + eps),  y = act((x - mean) * rstd * weight[c] + bias[c])
  * mean, rstd [S, G] of the arithmetic type (float for F32 and BF16, double for F64), for the backward.
- * C must be a multiple of G.  P == 0 or C == 0 with S*G > 0 groups is SNNLIF_ERR_ARG (a group without values
- * has no statistics).  `workspace`: snnseq_gn_act_workspace_bytes() bytes.
+ * C must be a multiple of G; S * G and P may be no more than SNNSEQ_MAX_TOKENS.  P == 0 or C == 0 with S*G > 0 groups
+ * is SNNLIF_ERR_ARG (a group without values has no statistics).  `workspace`: snnseq_gn_act_workspace_bytes() bytes.
  */
 int snnseq_gn_act_fp(const void* x, const void* weight, const void* bias, void* y, void* mean, void* rstd, int dtype,
                      int64_t S, int64_t P, int64_t C, int64_t G, double eps, int act, void* workspace,
@@ -102,7 +102,9 @@ size_t snnseq_gn_act_workspace_bytes(int dtype, int64_t S, int64_t P, int64_t C,
  * of Hk; value head h uses key head h / (Hv / Hk).  g <= 0 is the decay's logarithm (-inf forgets everything);
  * keys are expected at length one or below, as the recurrence multiplies by up to |k|^2 - 1 otherwise.
  * `lengths` ([B] int32, may be NULL): the time steps of batch entry b at or behind lengths[b] do not exist.  They leave the
- * state alone, their outputs and gradients are zero, and what the operands hold there is not looked at.
+ * state alone, their outputs and gradients are zero, and what the operands hold there is not looked at.  A value within a
+ * sequence that is not finite reaches all later outputs, and may reach earlier ones of its chunk of 64 steps (and the
+ * gradients of its chunk); a single step does not have the latter.
  */
 typedef struct snnseq_delta {
     int64_t T, B, Hk, Hv, Dk, Dv;

@@ -33,10 +33,11 @@
 // The state passes are bound by the latency of a chunk's chain of products (three forward, three backward, each
 // through LDS), the others by memory.
 //
-// Measured, keys and values of 128 in bf16.  (a) 2048 steps of 4 sequences of 8 heads, with a backward: inverse 29 us
-// (98 MB: 3.4 TB/s), state 58 (1.8 per chunk), output 33 (147 MB: 4.5 TB/s), inner gradients 26 (98 MB: 3.8 TB/s), state
-// gradients 90 (2.8 per chunk), input gradients 107 (311 MB: 2.9 TB/s, one workgroup of 129 KB of LDS per CU).
-// (b) 8192 steps of one sequence of 16 heads, nothing kept: inverse 58, state and output 223 (1.74 per chunk).
+// Measured, keys and values of 128 in bf16.  (a) 2048 steps of 4 sequences of 8 heads, with a backward: inverse 26 us
+// (98 MB: 3.7 TB/s), state 57 (1.8 per chunk), output 37 (147 MB: 4.0 TB/s), inner gradients 27 (98 MB: 3.7 TB/s), state
+// gradients 91 (2.9 per chunk), input gradients 112 (311 MB: 2.8 TB/s, one workgroup of 129 KB of LDS per CU).
+// (b) 8192 steps of one sequence of 16 heads, nothing kept: inverse 52, state and output 234 (1.8 per chunk); in fp32 112
+// and 399.
 //
 // Numbers.  States, R, Tm, dX and every sum are fp32.  In bf16 storage the products run on the bf16 matrix
 // instructions; an input is exact there, and what is derived (Tm, X, R, P, the state, ...) is given as a sum of three

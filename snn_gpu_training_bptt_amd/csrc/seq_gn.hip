@@ -10,13 +10,16 @@
 //   rows   P == 1 and a group of at most 4 vectors per lane: a group is one run of memory.  L lanes (a power of two)
 //          own it, hold it in registers and reduce by shuffles.  In the backward a lane keeps its channels over many
 //          samples, so the channel sums stay in registers.  [16384, 8 groups of 128] bf16 silu: forward 21 us (67 MB:
-//          3.2 TB/s, bound by the exponentials' arithmetic and latency), backward 31 us (101 MB: 3.2 TB/s).
+//          3.2 TB/s), backward 32 us (101 MB: 3.2 TB/s); without an activation 18 and 28 us.  Bound by arithmetic: vector
+//          instructions are under way 85 % and 78 % of the time (77 % and 69 % without the activation).
 //   slab   the P rows of a bundle of groups fit the registers of a workgroup: read once, reduced through LDS, written
 //          once.  A bundle is as many groups as make a row segment of 128 bytes, a memory line (64 where 128 do not fit).
 //          [8 64 32 32 128] fp32: forward 97 us (537 MB: 5.5 TB/s), backward 219 us (805 MB: 3.7 TB/s; 1024 threads with
 //          all their registers, one workgroup per CU, so that a sample's loads overlap only with the sums before).
 //   split  larger: partial sums over slices of the positions, a small kernel that combines them, and a second read
-//          of the inputs in the pass that writes.
+//          of the inputs in the pass that writes.  [32 samples of 4096 positions, 8 groups of 32] silu: fp32 forward 100 us
+//          (403 MB), backward 159 us (671 MB); bf16 55 and 85 us.  The backward of [8 64 32 32 128] in 32 groups bf16, whose
+//          sums do not fit the slab's registers, takes 160 us here (671 MB: 4.2 TB/s); its slab forward 78 us.
 // Statistics and sums are held in 32 bits (64 for double storage, and in the split layout's statistics); the variance is taken
 // around the mean, in a second sweep over the registers, or around one of the group's values in 64 bits (split).
 // Every sum has a fixed order.  Groups of any size, wherever they lie, are covered by vectors of 16 bytes (Spot): [7455,
@@ -26,8 +29,8 @@
 namespace snnseq {
 namespace {
 
-// Two instructions, off by a unit in the last place and |v| * 2^-24: that of v's own rounding.  The library's exponential,
-// four times as many, made the norm of bf16 tokens bound by arithmetic.
+// Two instructions, off by a unit in the last place and |v| * 2^-24: that of v's own rounding.  The library's exponential
+// takes four times as many, and instructions are what the norm of bf16 tokens is bound by.
 __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 __device__ __forceinline__ float erf_of(float v) { return erff(v); }

@@ -10,7 +10,8 @@ two halves with ``torch.distributed.all_reduce`` of two ``[C]`` vectors between 
 
 The token layers -- ``embed_func``, ``gn_act_func``, ``gated_delta_func`` and ``gated_delta_step`` -- extend the set to
 networks over token sequences on the same time axis; the reference has no counterpart.  Their autograd functions are
-part of the native module.
+part of the native module; forward-mode derivatives, second derivatives, function transforms, fake tensors and recording
+by ``torch.jit.trace`` or ``make_fx`` are refused.
 
 Contract shared by all of them, as in the reference: a forward saves only its *inputs* (plus the
 per-channel inverse standard deviation a batch-norm forward returns) -- never spikes or membrane
@@ -300,7 +301,8 @@ def embed_func(tokens, weight, scale=1.0):
 
 def gn_act_func(x, weight_gn, bias_gn, groups, eps_gn=1e-5, act="none"):
     """Group norm over the last axis of ``[T, B, ..., C]`` (per time step, batch entry and group of ``C / groups``
-    channels), then ``act``: "none", "relu", "silu" or "gelu".  Keeps its inputs and the statistics."""
+    channels), then ``act``: "none", "relu", "silu" or "gelu".  Keeps its inputs and the statistics.  Samples (``T * B``)
+    times groups, and positions, up to 8388608."""
     return snnlib.gn_act(x, weight_gn, bias_gn, groups, eps_gn, act)
 
 
@@ -317,7 +319,8 @@ def gated_delta_func(q, k, v, g, beta, state=None, lengths=None, scale=None):
     ``q``, ``k`` ``[T, B, Hk, Dk]``, ``v`` ``[T, B, Hv, Dv]`` (float32 or bfloat16, any strides with dense rows; ``Hv``
     a multiple of ``Hk``, ``Dk`` up to 128), ``g`` (at most zero) and ``beta`` ``[T, B, Hv]`` float32, ``state``
     ``[B, Hv, Dk, Dv]`` float32, ``lengths`` ``[B]`` int32: steps at or behind a sequence's length do not exist.
-    ``scale`` defaults to ``Dk ** -0.5``.  Where a gradient will be asked for, the state before every 64th step is kept."""
+    ``scale`` defaults to ``Dk ** -0.5``.  Where a gradient will be asked for, the state before every 64th step is kept.
+    A value that is not finite reaches all later outputs, and may reach earlier ones of its chunk of 64 steps."""
     return snnlib.gated_delta(q, k, v, g, beta, state, lengths, _key_scale(q) if scale is None else scale)
 
 
