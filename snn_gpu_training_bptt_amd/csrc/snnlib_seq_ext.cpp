@@ -11,8 +11,9 @@
 //
 // and, differentiable, embed(tokens, weight, scale), gn_act(x, weight_gn, bias_gn, groups, eps_gn, act) and
 // gated_delta(q, k, v, g, beta, state, lengths, scale) -> (o, state_out).  Their autograd functions are here and not in
-// Python, unlike the fire layers': on a few thousand tokens the kernels of a forward and backward are over in 20 us, and
-// two Python frames and the wait for the interpreter in the backward's thread took 30 us more than these do.
+// Python, unlike the fire layers': on a few thousand tokens the kernels of a forward and backward are over in 16 us, and
+// two Python frames and the wait for the interpreter in the backward's thread cost 4 us more than these (embedding of 1665
+// tokens in a loop: 38 us a pass, 34 here, 16 without autograd).
 //
 // As in snnlib_ext.cpp: this file validates tensors, allocates outputs and workspaces and forwards raw device
 // pointers to the C ABI (include/snnlib_seq.h) on the current stream of the tensors' device; it holds no device
